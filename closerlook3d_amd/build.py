@@ -34,6 +34,10 @@ FLAGS = [
     # DESIGN 6; csrc/fused_pwmlp.hip pk_low).  The packed code that is left is written out by hand and checked by
     # tests/test_isa_packed_operands.py
     "-fno-slp-vectorize",
+    # ... and none from hand-written float pairs either: without the feature the compiler emits the two scalar instructions
+    # for each pair (the same bits; PseudoGrid, the last user of packed pairs, measured 0.8-1 % slower).  hipcc's host pass
+    # warns that it does not know the feature: harmless
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wextra", "-Wno-unused-parameter",
 ]
 

@@ -20,6 +20,7 @@ VAR = os.path.join(ROOT, "scripts", "micro", "var")
 LIB = os.path.join(VAR, "libcl3d_gemm_plan_env.so")
 HIPCC = "/opt/rocm/bin/hipcc"
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-munsafe-fp-atomics", "-fno-slp-vectorize",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-DCL3D_D2_FORM=0", "-DCL3D_GEMM_PLAN_ENV"]
 
 LAYERS = [  # C, points per cloud, Co  (B = 16 clouds)

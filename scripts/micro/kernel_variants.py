@@ -18,6 +18,7 @@ CSRC = os.path.join(ROOT, "closerlook3d_amd", "csrc")
 VAR = os.path.join(ROOT, "scripts", "micro", "var")
 HIPCC = "/opt/rocm/bin/hipcc"
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-munsafe-fp-atomics", "-fno-slp-vectorize",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-DCL3D_D2_FORM=0"]
 
 VARIANTS = {  # tag: (source file, extra defines)
