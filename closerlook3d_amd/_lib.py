@@ -19,6 +19,18 @@ _I = ctypes.c_int
 _F = ctypes.c_float
 _Z = ctypes.c_size_t
 
+
+class NormResidual(ctypes.Structure):
+    """cl3d_norm_residual of include/cl3d.h (csrc/point_norm.hip): field for field."""
+    _fields_ = (
+        [(n, _I) for n in ("B", "N", "C", "dtype", "param_f32", "kind", "next_kind", "gate_cloud")]
+        + [(n, _F) for n in ("residual_scale", "eps", "next_eps")]
+        + [("reserved", _I), ("p", ctypes.c_double)]
+        + [(n, _P) for n in ("rng", "x", "y", "weight", "bias", "gate", "next_weight", "next_bias", "out", "next", "stats",
+                             "dout", "dnext", "dx", "dy", "dweight", "dbias", "dgate", "dnext_weight", "dnext_bias", "ws")]
+        + [("ws_bytes", _Z)])
+
+
 # name -> argtypes; restype is int for every op.  Mirrors include/cl3d.h (tests/test_abi.py checks
 # that every symbol declared in the header is exported by the library and listed here).
 SIGNATURES = {
@@ -75,6 +87,13 @@ SIGNATURES = {
     "cl3d_gemm_autotune": [_I],
     "cl3d_gemm_autotune_stats": [_P, _P],
     "cl3d_sgd_step": [_P, _P, _P, ctypes.c_longlong, _F, _F, _F, _F, _I, _I, _I, _P],
+    "cl3d_gated_ffn_fwd": [_P] * 4 + [_I] * 8 + [_P, _P, _Z, _P],
+    "cl3d_gated_ffn_bwd": [_P] * 5 + [_I] * 8 + [_P] * 5 + [_Z, _P],
+    "cl3d_transpose16": [_P, _I, _I, _I, _P, _P],
+    "cl3d_norm_residual_fwd": [ctypes.POINTER(NormResidual), _P],
+    "cl3d_norm_residual_bwd": [ctypes.POINTER(NormResidual), _P],
+    "cl3d_dropout": [_P, _I, ctypes.c_longlong, ctypes.c_double, _P, _P, _P],
+    "cl3d_rng_take": [_P, ctypes.c_longlong, _P, _P],
     "cl3d_pwmlp_split_weight": [_P, _I, _I, _P, _P, _P],
     "cl3d_pwmlp_merge_weight_grad": [_P, _P, _I, _I, _I, _P, _P],
     "cl3d_pwmlp_stats": [_P] * 6 + [_I] * 5 + [_F, _P, _P, _P, _P, _I, _P],

@@ -11,6 +11,7 @@ import torch.nn as nn
 
 from .local_aggregation_operators import LocalAggregation, _cfg
 from . import pt_utils
+from .feed_forward import CounterDropout, FeedForwardBlock
 from .pt_utils import MaskedMaxPool, MaskedUpsample
 
 
@@ -71,8 +72,18 @@ class Bottleneck(nn.Module):
         self.relu = nn.ReLU(inplace=True)
         if in_channels != out_channels:
             self.shortcut = _conv_bn(in_channels, out_channels, config.bn_momentum, relu=False)
+        # beyond the reference: config.cl3d_feed_forward (hidden channels per channel, 0: none) appends a gated feed-forward
+        # block over the points' channels, with config.cl3d_feed_forward_dropout in training
+        ratio = _cfg(config, 'cl3d_feed_forward', 0)
+        self.feed_forward = None if not ratio else FeedForwardBlock(
+            out_channels, max(1, int(round(ratio * out_channels))), precision=self.precision,
+            dropout=_cfg(config, 'cl3d_feed_forward_dropout', 0.0))
 
     def forward(self, xyz, mask, features):
+        xyz, mask, features = self._bottleneck(xyz, mask, features)
+        return xyz, mask, features if self.feed_forward is None else self.feed_forward(features)
+
+    def _bottleneck(self, xyz, mask, features):
         if self.downsample:
             query_xyz, query_mask, identity = self.maxpool(xyz, mask, features)
         else:
@@ -242,15 +253,17 @@ class MaskedGlobalAvgPool1d(nn.Module):
 
 class ClassifierResNet(nn.Module):
     """logits (B, num_classes) from `res5_features`.  Reference: heads/classifier.py:17-54 (same layer indices
-    inside `classifier`, so checkpoints load unchanged)."""
+    inside `classifier`, so checkpoints load unchanged).  `config` (optional, beyond the reference's constructor arguments):
+    cl3d_counter_dropout replaces nn.Dropout by the dropout that stores no mask."""
 
-    def __init__(self, num_classes, width):
+    def __init__(self, num_classes, width, config=None):
         super().__init__()
+        dropout = CounterDropout if config is not None and _cfg(config, 'cl3d_counter_dropout', False) else nn.Dropout
         self.num_classes = num_classes
         self.pool = MaskedGlobalAvgPool1d()
         layers, cin = [], 16 * width
         for cout in (8 * width, 4 * width, 2 * width):
-            layers += [nn.Linear(cin, cout), nn.BatchNorm1d(cout), nn.ReLU(inplace=True), nn.Dropout(0.5)]
+            layers += [nn.Linear(cin, cout), nn.BatchNorm1d(cout), nn.ReLU(inplace=True), dropout(0.5)]
             cin = cout
         layers.append(nn.Linear(cin, num_classes))
         self.classifier = nn.Sequential(*layers)

@@ -118,7 +118,7 @@ class ClassificationModel(_Model):
         self.backbone = self._backbone(config)
         if config.head != 'resnet_cls':
             raise NotImplementedError(f"Head {config.head} not implemented in Classification Model")
-        self.classifier = ClassifierResNet(config.num_classes, config.width)
+        self.classifier = ClassifierResNet(config.num_classes, config.width, config=config)
 
     def forward(self, xyz, mask, features):
         return self.classifier(self.backbone(xyz, mask, features))

@@ -2,6 +2,11 @@
 #include "ball_query.h"
 #include "fused_common.h"
 
+namespace cl3d {
+size_t gated_ffn_workspace(int B, int N, int H, int flags, int C);  // gated_ffn.hip
+size_t point_norm_workspace(int B, int N, int C);                   // point_norm.hip
+}  // namespace cl3d
+
 extern "C" int cl3d_abi_version(void) { return CL3D_ABI_VERSION; }
 
 extern "C" int cl3d_d2_form(void) { return CL3D_D2_FORM; }
@@ -35,6 +40,10 @@ extern "C" size_t cl3d_workspace_bytes(int op, int B, int N, int M, int K, int C
       return cl3d::gemm_family_workspace(B, N, 2 * M, C, true);
     case CL3D_OP_CONV1X1:  // 1x1 Conv1d C -> M over B clouds of N points: K-slice partials of any of its three products
       return cl3d::gemm_family_workspace(B, N, M, C, false);
+    case CL3D_OP_GATED_FFN:  // packed operands, hidden activations, weight-gradient slices; M hidden channels, K flags
+      return cl3d::gated_ffn_workspace(B, N, M, K, C);
+    case CL3D_OP_POINT_NORM:  // partial rows of the parameters' gradients
+      return cl3d::point_norm_workspace(B, N, C);
     default:  // every other op of ABI v1 keeps its scratch in LDS
       return 0;
   }

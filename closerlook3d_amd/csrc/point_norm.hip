@@ -1,0 +1,541 @@
+// point_norm.hip -- the norms either side of a block, fused with its gate, its dropout and the residual, over the C channels of a
+// point (rows [R, C], R = clouds x points):
+//     n = norm(y) w + b          norm 0 none, 1 rms: y / sqrt(mean y^2 + eps), 2 layer: (y - mean) / sqrt(var + eps)
+//     o = alpha x + gate * drop(n)                      (exit of a block; gate per channel, or per cloud and channel)
+//     h = norm(o) w2 + b2                               (entry of the next; alone: h = norm(x) w2 + b2)
+// Each direction is one pass over the rows: a row lives in the registers of TPR lanes from the load to the store (statistics in
+// two steps over the registers, f32, so a mean far from zero costs no digits), parameters in registers across the rows of a
+// workgroup.  Bound: memory -- forward x, y in and o, h out; backward do, dh, x, y in and dx, dy out, a mean and a reciprocal
+// deviation per row kept from the forward pass.
+// Parameter gradients are sums over the rows: a workgroup keeps its rows' sums in registers, f32, one partial row per workgroup
+// goes to scratch and a second launch adds them in order (no atomics: bit-identical run to run).  A workgroup's rows are of one
+// cloud, so a gate per cloud is summed by the same partials.
+#include "ff_common.h"
+
+namespace cl3d {
+
+struct NormArgs {
+  const void *x, *y;                  // x: the residual stream (or the one input)
+  const void *w1, *b1, *gate, *w2, *b2;
+  const void *dout, *dnext;
+  void *o, *h, *dx, *dy;
+  float *stats;                       // [R][4]: mean, 1 / deviation of y; the same of o
+  float *partial;                     // [workgroup][5][C]: w, b, gate, w2, b2
+  long long N;                        // rows of a cloud
+  int B, C, chunks, per;              // workgroups and rows of one for each cloud
+  int kind1, kind2, exit, next, gate_cloud, param_f32;
+  float alpha, eps1, eps2;
+  Drop drop;
+  int has_drop;
+};
+
+template <typename T> __device__ __forceinline__ float param(const void *p, long long i, int f32) {
+  return f32 ? static_cast<const float *>(p)[i] : T::get(static_cast<const typename T::storage *>(p)[i]);
+}
+
+// sums of two values over the TPR lanes of a row
+template <int TPR> __device__ __forceinline__ void row_sum(float &a, float &b, float *s_red) {
+#pragma unroll
+  for (int off = (TPR < 64 ? TPR : 64) / 2; off >= 1; off >>= 1) {
+    a += __shfl_xor(a, off, 64);
+    b += __shfl_xor(b, off, 64);
+  }
+  if (TPR > 64) {  // the whole workgroup is one row
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) { s_red[2 * wave] = a; s_red[2 * wave + 1] = b; }
+    __syncthreads();
+    a = b = 0.f;
+#pragma unroll
+    for (int w = 0; w < TPR / 64; ++w) { a += s_red[2 * w]; b += s_red[2 * w + 1]; }
+  }
+}
+
+// V consecutive elements at p (VEC: 16 bytes, else one)
+template <typename T, int V> __device__ __forceinline__ void load_v(const void *base, long long at, float *v) {
+  const auto *p = static_cast<const typename T::storage *>(base) + at;
+  if constexpr (V == 1) {
+    v[0] = T::get(*p);
+  } else {
+    const Vec16<T> q = *reinterpret_cast<const Vec16<T> *>(p);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = T::get(q.v[e]);
+  }
+}
+template <typename T, int V> __device__ __forceinline__ void store_v(void *base, long long at, const float *v) {
+  auto *p = static_cast<typename T::storage *>(base) + at;
+  if constexpr (V == 1) {
+    *p = T::put(v[0]);
+  } else {
+    Vec16<T> q;
+#pragma unroll
+    for (int e = 0; e < V; ++e) q.v[e] = T::put(v[e]);
+    *reinterpret_cast<Vec16<T> *>(p) = q;
+  }
+}
+
+// 1 / (1 - p) or 0 for the V elements from `at` on (V > 1: at is a multiple of 4)
+template <int V> __device__ __forceinline__ void keep_v(const Drop &d, unsigned long long seed, unsigned long long offset, long long at, float *m) {
+  if (d.all) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) m[e] = 0.f;
+    return;
+  }
+  if constexpr (V == 1) {
+    const Words w = philox(offset + (unsigned long long)(at >> 2), seed);
+    const int e = (int)(at & 3);
+    const unsigned word = e < 2 ? (e ? w.w[1] : w.w[0]) : (e == 2 ? w.w[2] : w.w[3]);
+    m[0] = word >= d.threshold ? d.scale : 0.f;
+  } else {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+      const Words w = philox(offset + (unsigned long long)((at >> 2) + q), seed);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m[4 * q + e] = w.w[e] >= d.threshold ? d.scale : 0.f;
+    }
+  }
+}
+
+// mean and reciprocal deviation of a row held as v[NV][V]; `on`: which pieces exist
+template <int TPR, int NV, int V>
+__device__ __forceinline__ void row_stats(const float (&v)[NV][V], const bool (&on)[NV], int kind, float eps, int C, float *s_red, float &mean,
+                                          float &rinv) {
+  const float inv_c = 1.f / (float)C;
+  mean = 0.f;
+  if (kind == CL3D_NORM_LAYER) {
+    float a = 0.f, b = 0.f;
+#pragma unroll
+    for (int q = 0; q < NV; ++q)
+      if (on[q])
+#pragma unroll
+        for (int e = 0; e < V; ++e) a += v[q][e];
+    row_sum<TPR>(a, b, s_red);
+    mean = a * inv_c;
+  }
+  float a = 0.f, b = 0.f;
+#pragma unroll
+  for (int q = 0; q < NV; ++q)
+    if (on[q])
+#pragma unroll
+      for (int e = 0; e < V; ++e) a = __builtin_fmaf(v[q][e] - mean, v[q][e] - mean, a);
+  row_sum<TPR>(a, b, s_red);
+  rinv = 1.f / sqrtf(a * inv_c + eps);
+}
+
+template <typename T, int TPR, int NV, int V>
+__global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
+  __shared__ float s_red[8];
+  const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const int b = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+  const long long first = (long long)b * a.N + (long long)chunk * a.per;
+  long long last = first + a.per, end = (long long)(b + 1) * a.N;
+  if (last > end) last = end;
+  bool on[NV];
+  int col[NV];
+  float w1[NV][V], b1[NV][V], gate[NV][V], w2[NV][V], b2[NV][V];
+#pragma unroll
+  for (int q = 0; q < NV; ++q) {
+    col[q] = (q * TPR + lane) * V;
+    on[q] = col[q] < a.C;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int c = on[q] ? col[q] + e : 0;
+      w1[q][e] = a.w1 ? param<T>(a.w1, c, a.param_f32) : 1.f;
+      b1[q][e] = a.b1 ? param<T>(a.b1, c, a.param_f32) : 0.f;
+      gate[q][e] = a.gate ? param<T>(a.gate, a.gate_cloud ? (long long)b * a.C + c : c, a.param_f32) : 1.f;
+      w2[q][e] = a.w2 ? param<T>(a.w2, c, a.param_f32) : 1.f;
+      b2[q][e] = a.b2 ? param<T>(a.b2, c, a.param_f32) : 0.f;
+    }
+  }
+  unsigned long long seed = 0, offset = 0;
+  if (a.has_drop) { seed = a.drop.state[0]; offset = a.drop.state[1]; }
+  // every lane walks the same number of rows (row_sum's barriers): a group behind the last row works on the last one, unstored
+  for (long long r0 = first; r0 < last; r0 += 256 / TPR) {
+    const bool live = r0 + group < last;
+    const long long r = live ? r0 + group : last - 1;
+    float v[NV][V];
+#pragma unroll
+    for (int q = 0; q < NV; ++q)
+      if (on[q]) load_v<T, V>(a.x, r * a.C + col[q], v[q]);
+    if (a.exit) {
+      float y[NV][V];
+#pragma unroll
+      for (int q = 0; q < NV; ++q)
+        if (on[q]) load_v<T, V>(a.y, r * a.C + col[q], y[q]);
+      float mean = 0.f, rinv = 1.f;
+      if (a.kind1 != CL3D_NORM_NONE) row_stats<TPR, NV, V>(y, on, a.kind1, a.eps1, a.C, s_red, mean, rinv);
+      if (a.stats && live && lane == 0) *reinterpret_cast<float2 *>(a.stats + 4 * r) = make_float2(mean, rinv);
+#pragma unroll
+      for (int q = 0; q < NV; ++q) {
+        if (!on[q]) continue;
+        float m[V];
+        if (a.has_drop) keep_v<V>(a.drop, seed, offset, r * a.C + col[q], m);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          float n = __builtin_fmaf((y[q][e] - mean) * rinv, w1[q][e], b1[q][e]);
+          if (a.has_drop) n = m[e] == 0.f ? 0.f : n * m[e];
+          v[q][e] = __builtin_fmaf(a.alpha, v[q][e], gate[q][e] * n);
+        }
+        if (live) store_v<T, V>(a.o, r * a.C + col[q], v[q]);
+      }
+    }
+    if (a.next) {
+      float mean = 0.f, rinv = 1.f;
+      row_stats<TPR, NV, V>(v, on, a.kind2, a.eps2, a.C, s_red, mean, rinv);
+      if (a.stats && live && lane == 0) *reinterpret_cast<float2 *>(a.stats + 4 * r + 2) = make_float2(mean, rinv);
+#pragma unroll
+      for (int q = 0; q < NV; ++q) {
+        if (!on[q]) continue;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[q][e] = __builtin_fmaf((v[q][e] - mean) * rinv, w2[q][e], b2[q][e]);
+        if (live) store_v<T, V>(a.h, r * a.C + col[q], v[q]);
+      }
+    }
+  }
+}
+
+// d of norm: dhat -> d = rinv (dhat - hat mean(dhat hat) - [layer] mean(dhat))
+template <typename T, int TPR, int NV, int V>
+__global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
+  __shared__ float s_red[8];
+  __shared__ float s_sum[TPR < 256 ? 256 / TPR : 1][TPR < 256 ? TPR * NV * V : 1];
+  const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const int b = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+  const long long first = (long long)b * a.N + (long long)chunk * a.per;
+  long long last = first + a.per, end = (long long)(b + 1) * a.N;
+  if (last > end) last = end;
+  const float inv_c = 1.f / (float)a.C;
+  bool on[NV];
+  int col[NV];
+  float w1[NV][V], b1[NV][V], gate[NV][V], w2[NV][V];
+  float s_w1[NV][V], s_b1[NV][V], s_gate[NV][V], s_w2[NV][V], s_b2[NV][V];
+#pragma unroll
+  for (int q = 0; q < NV; ++q) {
+    col[q] = (q * TPR + lane) * V;
+    on[q] = col[q] < a.C;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int c = on[q] ? col[q] + e : 0;
+      w1[q][e] = a.w1 ? param<T>(a.w1, c, a.param_f32) : 1.f;
+      b1[q][e] = a.b1 ? param<T>(a.b1, c, a.param_f32) : 0.f;
+      gate[q][e] = a.gate ? param<T>(a.gate, a.gate_cloud ? (long long)b * a.C + c : c, a.param_f32) : 1.f;
+      w2[q][e] = a.w2 ? param<T>(a.w2, c, a.param_f32) : 1.f;
+      s_w1[q][e] = s_b1[q][e] = s_gate[q][e] = s_w2[q][e] = s_b2[q][e] = 0.f;
+    }
+  }
+  unsigned long long seed = 0, offset = 0;
+  if (a.has_drop) { seed = a.drop.state[0]; offset = a.drop.state[1]; }
+  for (long long r0 = first; r0 < last; r0 += 256 / TPR) {
+    const bool live = r0 + group < last;
+    const long long r = live ? r0 + group : last - 1;
+    const f32x4 st = *reinterpret_cast<const f32x4 *>(a.stats + 4 * r);
+    // the exit once more, from x and y: out as the forward pass had it before it was rounded costs no more traffic than the
+    // rounded one, and the y hats are needed below anyway.  keep: 1 / (1 - p) or 0; hat1, n: of y
+    float hat1[NV][V], keep[NV][V], d[NV][V];
+    if (a.exit) {
+#pragma unroll
+      for (int q = 0; q < NV; ++q) {
+        if (!on[q]) continue;
+        load_v<T, V>(a.y, r * a.C + col[q], hat1[q]);
+        if (a.has_drop) keep_v<V>(a.drop, seed, offset, r * a.C + col[q], keep[q]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          hat1[q][e] = (hat1[q][e] - st[0]) * st[1];
+          if (!a.has_drop) keep[q][e] = 1.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[q][e] = 0.f;
+      if (a.dout && on[q]) load_v<T, V>(a.dout, r * a.C + col[q], d[q]);
+    }
+    if (a.dnext) {
+      float hat[NV][V], dh[NV][V], p1 = 0.f, p2 = 0.f;
+#pragma unroll
+      for (int q = 0; q < NV; ++q) {
+        if (!on[q]) continue;
+        load_v<T, V>(a.x, r * a.C + col[q], hat[q]);
+        load_v<T, V>(a.dnext, r * a.C + col[q], dh[q]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          if (a.exit) {
+            const float n = keep[q][e] == 0.f ? 0.f : __builtin_fmaf(hat1[q][e], w1[q][e], b1[q][e]) * keep[q][e];
+            hat[q][e] = __builtin_fmaf(a.alpha, hat[q][e], gate[q][e] * n);
+          }
+          hat[q][e] = (hat[q][e] - st[2]) * st[3];
+          if (live) {
+            s_w2[q][e] = __builtin_fmaf(dh[q][e], hat[q][e], s_w2[q][e]);
+            s_b2[q][e] += dh[q][e];
+          }
+          dh[q][e] *= w2[q][e];
+          p1 = __builtin_fmaf(dh[q][e], hat[q][e], p1);
+          p2 += dh[q][e];
+        }
+      }
+      row_sum<TPR>(p1, p2, s_red);
+      p1 *= inv_c;
+      p2 = a.kind2 == CL3D_NORM_LAYER ? p2 * inv_c : 0.f;
+#pragma unroll
+      for (int q = 0; q < NV; ++q)
+        if (on[q])
+#pragma unroll
+          for (int e = 0; e < V; ++e) d[q][e] += st[3] * (dh[q][e] - __builtin_fmaf(hat[q][e], p1, p2));
+    }
+    if (a.dx && live) {
+#pragma unroll
+      for (int q = 0; q < NV; ++q) {
+        if (!on[q]) continue;
+        float o[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = a.exit ? a.alpha * d[q][e] : d[q][e];
+        store_v<T, V>(a.dx, r * a.C + col[q], o);
+      }
+    }
+    if (a.exit) {
+      float p1 = 0.f, p2 = 0.f;
+#pragma unroll
+      for (int q = 0; q < NV; ++q) {
+        if (!on[q]) continue;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          float dm = keep[q][e] == 0.f ? 0.f : d[q][e] * keep[q][e];
+          if (live && keep[q][e] != 0.f)  // (a dropped element: n is not looked at)
+            s_gate[q][e] = __builtin_fmaf(dm, __builtin_fmaf(hat1[q][e], w1[q][e], b1[q][e]), s_gate[q][e]);
+          dm *= gate[q][e];
+          if (live) {
+            s_w1[q][e] = __builtin_fmaf(dm, hat1[q][e], s_w1[q][e]);
+            s_b1[q][e] += dm;
+          }
+          dm *= w1[q][e];
+          p1 = __builtin_fmaf(dm, hat1[q][e], p1);
+          p2 += dm;
+          d[q][e] = dm;
+        }
+      }
+      if (a.dy) {
+        if (a.kind1 != CL3D_NORM_NONE) {
+          row_sum<TPR>(p1, p2, s_red);
+          p1 *= inv_c;
+          p2 = a.kind1 == CL3D_NORM_LAYER ? p2 * inv_c : 0.f;
+        } else {
+          p1 = p2 = 0.f;
+        }
+        if (live)
+#pragma unroll
+          for (int q = 0; q < NV; ++q) {
+            if (!on[q]) continue;
+            float o[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = st[1] * (d[q][e] - __builtin_fmaf(hat1[q][e], p1, p2));
+            store_v<T, V>(a.dy, r * a.C + col[q], o);
+          }
+      }
+    }
+  }
+  if (!a.partial) return;
+  // the groups' sums of a column, in group order
+  auto flush = [&](const float (&s)[NV][V], int which) {
+    float *dst = a.partial + ((long long)blockIdx.x * 5 + which) * a.C;
+    if constexpr (TPR == 256) {
+#pragma unroll
+      for (int q = 0; q < NV; ++q)
+        if (on[q])
+#pragma unroll
+          for (int e = 0; e < V; ++e) dst[col[q] + e] = s[q][e];
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < NV; ++q)
+#pragma unroll
+        for (int e = 0; e < V; ++e) s_sum[group][(q * TPR + lane) * V + e] = s[q][e];
+      __syncthreads();
+      for (int c = threadIdx.x; c < a.C; c += 256) {
+        float t = 0.f;
+#pragma unroll
+        for (int g = 0; g < 256 / TPR; ++g) t += s_sum[g][c];
+        dst[c] = t;
+      }
+    }
+  };
+  if (a.exit) {
+    if (a.w1) flush(s_w1, 0);
+    if (a.b1) flush(s_b1, 1);
+    if (a.gate) flush(s_gate, 2);
+  }
+  if (a.w2) flush(s_w2, 3);
+  if (a.b2) flush(s_b2, 4);
+}
+
+// sums of the partial rows [first row of the sum ...][which][C]: 64 columns a workgroup, 16 rows at a time, joined in order
+struct NormSums {
+  const float *partial;
+  void *out[5];
+  int C, rows, chunks, gate_cloud, param_f32;
+};
+template <typename T>
+__global__ __launch_bounds__(1024) void norm_sums_kernel(NormSums a) {
+  __shared__ float s[16][64];
+  const int which = blockIdx.y, c = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+  const bool cloud = which == 2 && a.gate_cloud;
+  const int b = blockIdx.z;
+  if (a.out[which] == nullptr || (!cloud && b > 0)) return;
+  const int rows = cloud ? a.chunks : a.rows, first = cloud ? b * a.chunks : 0;
+  float t = 0.f;
+  if (c < a.C)
+    for (int r = part; r < rows; r += 16) t += a.partial[((long long)(first + r) * 5 + which) * a.C + c];
+  s[part][threadIdx.x & 63] = t;
+  __syncthreads();
+  if (part != 0 || c >= a.C) return;
+  t = 0.f;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) t += s[q][threadIdx.x];
+  const long long at = (cloud ? (long long)b * a.C : 0) + c;
+  if (a.param_f32) static_cast<float *>(a.out[which])[at] = t;
+  else static_cast<typename T::storage *>(a.out[which])[at] = T::put(t);
+}
+
+// ---- host side -----------------------------------------------------------------------------------------------------
+constexpr int kNormMaxC = 8192;
+
+// workgroups of a cloud and rows of each: about 8 workgroups a CU forward, 4 backward (each leaves a partial row behind)
+static void norm_grid(NormArgs &a, int rows_per_pass, int target) {
+  long long want = ((long long)target + a.B - 1) / a.B;
+  const long long passes = (a.N + rows_per_pass - 1) / rows_per_pass;
+  if (want > passes) want = passes;
+  if (want < 1) want = 1;
+  const long long per = ((passes + want - 1) / want) * rows_per_pass;
+  a.per = (int)per;
+  a.chunks = (int)((a.N + per - 1) / per);
+}
+
+struct NormMap {
+  int tpr, nv, v;
+};
+// lanes of a row and pieces of a lane: 16-byte pieces where C and the pointers allow, else single elements.  As few lanes as hold
+// the row in one piece each (several rows a wave), the whole workgroup where 64 do not.
+static NormMap norm_map(int dtype, int C, bool aligned) {
+  const int kv = dtype == CL3D_F32 ? 4 : 8;
+  const int v = aligned && C % kv == 0 ? kv : 1;
+  const int pieces = C / v;
+  NormMap m{256, 1, v};
+  if (v > 1 && pieces <= 16) m.tpr = 16;
+  else if (pieces <= 64) m.tpr = 64;
+  while (m.tpr * m.nv < pieces) m.nv = m.nv == 1 ? (v == 1 ? 8 : v == 4 ? 8 : 4) : 32;
+  return m;
+}
+
+template <typename T, int TPR, int NV, int V> static void norm_run(bool backward, const NormArgs &a, hipStream_t st) {
+  const dim3 grid((unsigned)((long long)a.B * a.chunks));
+  if (backward) hipLaunchKernelGGL((norm_bwd_kernel<T, TPR, NV, V>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((norm_fwd_kernel<T, TPR, NV, V>), grid, dim3(256), 0, st, a);
+}
+template <typename T> static void norm_pick(const NormMap &m, bool backward, const NormArgs &a, hipStream_t st) {
+  constexpr int V = T::kVec, NW = V == 4 ? 8 : 4;
+  if (m.v == 1) {
+    if (m.tpr == 64) norm_run<T, 64, 1, 1>(backward, a, st);
+    else if (m.nv == 1) norm_run<T, 256, 1, 1>(backward, a, st);
+    else if (m.nv == 8) norm_run<T, 256, 8, 1>(backward, a, st);
+    else norm_run<T, 256, 32, 1>(backward, a, st);
+  } else {
+    if (m.tpr == 16) norm_run<T, 16, 1, V>(backward, a, st);
+    else if (m.tpr == 64) norm_run<T, 64, 1, V>(backward, a, st);
+    else if (m.nv == 1) norm_run<T, 256, 1, V>(backward, a, st);
+    else norm_run<T, 256, NW, V>(backward, a, st);
+  }
+}
+static void norm_launch(int dtype, const NormMap &m, bool backward, const NormArgs &a, hipStream_t st) {
+  if (dtype == CL3D_F32) norm_pick<F32>(m, backward, a, st);
+  else if (dtype == CL3D_BF16) norm_pick<Bf16>(m, backward, a, st);
+  else norm_pick<F16>(m, backward, a, st);
+}
+
+static int norm_checks(const cl3d_norm_residual *p, bool backward, const char *who) {
+  CL3D_REQUIRE(p != nullptr, "%s: null argument block", who);
+  CL3D_REQUIRE(p->dtype == CL3D_F32 || p->dtype == CL3D_BF16 || p->dtype == CL3D_F16, "%s: unknown element type %d", who, p->dtype);
+  CL3D_REQUIRE(p->B >= 0 && p->N >= 0 && p->C > 0, "%s: bad sizes", who);
+  CL3D_REQUIRE(p->kind >= CL3D_NORM_NONE && p->kind <= CL3D_NORM_LAYER && p->next_kind >= CL3D_NORM_NONE && p->next_kind <= CL3D_NORM_LAYER,
+               "%s: unknown norm", who);
+  CL3D_REQUIRE(p->y != nullptr || p->next_kind != CL3D_NORM_NONE, "%s: neither a block to leave nor a norm to enter", who);
+  CL3D_REQUIRE(p->y != nullptr || (!p->weight && !p->bias && !p->gate && p->p == 0.0), "%s: a gate, dropout or norm of a block that is not there", who);
+  if (p->C > kNormMaxC || (long long)p->B * p->N > 0x7fffff00ll)
+    return fail(CL3D_E_UNSUPPORTED, "%s: more than %d channels, or points than 31 bits count", who, kNormMaxC);
+  if (p->gate_cloud && p->B > 65535) return fail(CL3D_E_UNSUPPORTED, "%s: a gate per cloud for more than 65535 clouds", who);
+  return CL3D_OK;
+}
+
+static void norm_args(NormArgs &a, const cl3d_norm_residual *p) {
+  a = NormArgs{};
+  a.x = p->x; a.y = p->y;
+  a.w1 = p->weight; a.b1 = p->bias; a.gate = p->gate; a.w2 = p->next_weight; a.b2 = p->next_bias;
+  a.stats = p->stats;
+  a.N = p->N; a.B = p->B; a.C = p->C;
+  if (!p->gate_cloud) { a.N *= a.B; a.B = 1; }  // nothing differs from cloud to cloud: one run of rows
+  a.kind1 = p->kind; a.kind2 = p->next_kind;
+  a.exit = p->y != nullptr; a.next = p->next_kind != CL3D_NORM_NONE;
+  a.gate_cloud = p->gate_cloud; a.param_f32 = p->param_f32 || p->dtype == CL3D_F32;
+  a.alpha = p->residual_scale; a.eps1 = p->eps; a.eps2 = p->next_eps;
+  a.has_drop = p->p > 0.0;
+}
+
+constexpr int kNormBwdGroups = 1024;
+size_t point_norm_workspace(int B, int N, int C) {
+  // partial rows of the backward pass: at most kNormBwdGroups + B workgroups
+  (void)N;
+  return ((size_t)kNormBwdGroups + (B > 0 ? B : 0)) * 5 * (size_t)(C > 0 ? C : 0) * sizeof(float);
+}
+
+}  // namespace cl3d
+
+extern "C" int cl3d_norm_residual_fwd(const cl3d_norm_residual *p, cl3d_stream_t stream) {
+  using namespace cl3d;
+  int rc = norm_checks(p, false, "norm_residual_fwd");
+  if (rc != CL3D_OK) return rc;
+  NormArgs a;
+  norm_args(a, p);
+  rc = make_drop(a.drop, p->rng, p->p, "norm_residual_fwd");
+  if (rc != CL3D_OK) return rc;
+  if (p->B == 0 || p->N == 0) return CL3D_OK;
+  CL3D_REQUIRE(p->x && (!a.exit || p->out) && (!a.next || p->next), "norm_residual_fwd: null pointer");
+  a.o = p->out; a.h = p->next;
+  const NormMap m = norm_map(p->dtype, p->C, aligned16(p->x) && aligned16(p->y) && aligned16(p->out) && aligned16(p->next));
+  norm_grid(a, 256 / m.tpr, 2048);
+  norm_launch(p->dtype, m, false, a, (hipStream_t)stream);
+  return check_launch("cl3d_norm_residual_fwd");
+}
+
+extern "C" int cl3d_norm_residual_bwd(const cl3d_norm_residual *p, cl3d_stream_t stream) {
+  using namespace cl3d;
+  int rc = norm_checks(p, true, "norm_residual_bwd");
+  if (rc != CL3D_OK) return rc;
+  NormArgs a;
+  norm_args(a, p);
+  rc = make_drop(a.drop, p->rng, p->p, "norm_residual_bwd");
+  if (rc != CL3D_OK) return rc;
+  CL3D_REQUIRE(p->B > 0 && p->N > 0, "norm_residual_bwd: no points (their gradients are zeros: nothing to launch)");
+  CL3D_REQUIRE(p->stats && (p->dout || p->dnext), "norm_residual_bwd: null pointer");
+  CL3D_REQUIRE(!p->dnext || (a.next && p->x), "norm_residual_bwd: a gradient of a norm that was not formed");
+  CL3D_REQUIRE(!p->dout || a.exit, "norm_residual_bwd: a gradient of a sum that was not formed");
+  a.dout = p->dout; a.dnext = p->dnext; a.dx = p->dx; a.dy = p->dy;
+  const NormMap m = norm_map(p->dtype, p->C, aligned16(p->x) && aligned16(p->y) && aligned16(p->dout) && aligned16(p->dnext) &&
+                                                 aligned16(p->dx) && aligned16(p->dy));
+  norm_grid(a, 256 / m.tpr, kNormBwdGroups);
+  const bool sums = p->dweight || p->dbias || p->dgate || p->dnext_weight || p->dnext_bias;
+  if (sums) {
+    const size_t need = (size_t)a.B * a.chunks * 5 * a.C * sizeof(float);
+    if (!p->ws || p->ws_bytes < need) return fail(CL3D_E_WORKSPACE, "norm_residual_bwd: %zu bytes of scratch, %zu needed", p->ws_bytes, need);
+    a.partial = static_cast<float *>(p->ws);
+  }
+  const hipStream_t st = (hipStream_t)stream;
+  norm_launch(p->dtype, m, true, a, st);
+  if (sums) {
+    NormSums s{a.partial, {a.exit ? p->dweight : nullptr, a.exit ? p->dbias : nullptr, a.exit ? p->dgate : nullptr, p->dnext_weight, p->dnext_bias},
+               a.C, a.B * a.chunks, a.chunks, a.gate_cloud, a.param_f32};
+    const dim3 grid(ceil_div(a.C, 64), 5, a.gate_cloud && p->dgate ? a.B : 1);
+    if (p->dtype == CL3D_F32) hipLaunchKernelGGL(norm_sums_kernel<F32>, grid, dim3(1024), 0, st, s);
+    else if (p->dtype == CL3D_BF16) hipLaunchKernelGGL(norm_sums_kernel<Bf16>, grid, dim3(1024), 0, st, s);
+    else hipLaunchKernelGGL(norm_sums_kernel<F16>, grid, dim3(1024), 0, st, s);
+  }
+  return check_launch("cl3d_norm_residual_bwd");
+}

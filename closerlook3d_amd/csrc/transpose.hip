@@ -124,6 +124,23 @@ static void tile_shape(int R, int C, int *tr, int *tc) {
   *tc = TC;
 }
 
+// [b][R][C] -> [b][C][R], 16-bit elements: a 64 x 64 tile through LDS, rows of 66 elements (33 banks: conflict-free both ways)
+__global__ __launch_bounds__(256) void transpose16_kernel(const unsigned short *__restrict__ src, int R, int C, unsigned short *__restrict__ dst) {
+  __shared__ unsigned short tile[64][66];
+  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+  src += (long long)blockIdx.z * R * C;
+  dst += (long long)blockIdx.z * R * C;
+  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+    const int r = e >> 6, c = e & 63;
+    if (r0 + r < R && c0 + c < C) tile[r][c] = src[(long long)(r0 + r) * C + c0 + c];
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+    const int r = e & 63, c = e >> 6;
+    if (r0 + r < R && c0 + c < C) dst[(long long)(c0 + c) * R + r0 + r] = tile[r][c];
+  }
+}
+
 }  // namespace cl3d
 
 static int transpose_launch(const float *src, int B, int R, int C, float *dst, const float *row_scale,
@@ -161,4 +178,15 @@ extern "C" int cl3d_transpose_bn_relu(const float *src, const float *row_scale, 
                                       float *dst, cl3d_stream_t stream) {
   CL3D_REQUIRE(row_scale && row_shift, "transpose_bn_relu: null scale / shift");
   return transpose_launch(src, B, R, C, dst, row_scale, row_shift, (hipStream_t)stream, "cl3d_transpose_bn_relu");
+}
+
+extern "C" int cl3d_transpose16(const void *src, int B, int R, int C, void *dst, cl3d_stream_t stream) {
+  using namespace cl3d;
+  CL3D_REQUIRE(B >= 0 && R >= 0 && C >= 0, "transpose16: bad sizes");
+  if (B == 0 || R == 0 || C == 0) return CL3D_OK;
+  CL3D_REQUIRE(src && dst, "transpose16: null pointer");
+  if (B > 65535 || R > 65535 * 64) return fail(CL3D_E_UNSUPPORTED, "transpose16: more than 65535 clouds or 4194240 rows");
+  hipLaunchKernelGGL(transpose16_kernel, dim3(ceil_div(C, 64), ceil_div(R, 64), B), dim3(256), 0, (hipStream_t)stream,
+                     static_cast<const unsigned short *>(src), R, C, static_cast<unsigned short *>(dst));
+  return check_launch("cl3d_transpose16");
 }

@@ -1,0 +1,562 @@
+"""Per-point feed-forward operators: csrc/gated_ffn.hip, point_norm.hip, dropout.hip.
+
+    gated_feed_forward   (act(x Wg^T) * (x Wu^T)) Wd^T for every point, with its gradients
+    point_norm           an rms or layer norm over the channels of a point: the entry of a block
+    norm_gate_residual   the exit of a block -- norm, dropout, gate, scaled residual -- and the entry of the next, in one pass
+    dropout              from a counter-based generator: the mask is formed again in the backward pass, never stored
+
+and the modules on top of them: GatedFeedForward, CounterDropout, FeedForwardBlock (what backbones.Bottleneck appends when the
+configuration asks for it).
+
+Tensors are features (B, C, N), as everywhere in this package, or rows (R, C): pooled vectors, the input of nn.Linear.  (B, C, N)
+features may lie channel-major (dense) or point-major (a transposed view of dense (B, N, C) rows); results lie as the first
+input does.  The kernels work on point-major rows: of channel-major features they take and leave a transposed copy, so a chain
+of these operators is best kept point-major (to_point_major, once, at its beginning; FeedForwardBlock does).  Types: float32,
+bfloat16, float16.  Everything is formed in f32 and rounded once, to the type of the result.
+
+Points are independent of each other (only parameter gradients sum over them); padding points are computed like the others.  The
+results of a point depend on no other point, and every gradient is summed in a fixed order: bit-identical run to run.  There is no
+CPU fallback.  The operators can be captured into HIP graphs, forward and backward.
+"""
+import ctypes
+import weakref
+
+import torch
+import torch.nn as nn
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # CL3D_F32 / _BF16 / _F16
+_POINT, _CHANNEL = 0, 1                                             # CL3D_POINT_MAJOR / _CHANNEL_MAJOR
+_ACTIVATIONS = {'silu': 0, 'gelu': 1, 'relu': 2}
+_NORMS = {'none': 0, 'rms': 1, 'layer': 2}
+_PRECISIONS = {'f32': 0, 'bf16': 1}
+_OP_GATED_FFN, _OP_POINT_NORM = 17, 18
+_MAX_NORM_CHANNELS = 8192
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _check_features(x, who, name='x'):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{who}: {name} is a tensor, got {type(x).__name__}")
+    if not x.is_cuda:
+        raise RuntimeError(f"{who}: CPU not supported")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"{who}: {name} is float32, bfloat16 or float16, got {x.dtype}")
+    if x.dim() not in (2, 3):
+        raise ValueError(f"{who}: {name} is (B, C, N) features or (R, C) rows, got {tuple(x.shape)}")
+
+
+def _sizes(x):
+    """(B, C, N) of features; rows are clouds of one point."""
+    return (x.shape[0], x.shape[1], 1) if x.dim() == 2 else tuple(x.shape)
+
+
+def _check_param(t, shape, x, who, name, optional=True, f32=True):
+    if t is None:
+        if optional:
+            return
+        raise TypeError(f"{who}: {name} is missing")
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{who}: {name} is a tensor, got {type(t).__name__}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{who}: {name} has the shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.device != x.device:
+        raise RuntimeError(f"{who}: {name} is on {t.device}, x on {x.device}")
+    if t.dtype != x.dtype and not (f32 and t.dtype == torch.float32):
+        raise TypeError(f"{who}: {name} is {t.dtype}, x is {x.dtype}")
+
+
+def _point_major(t):
+    return t.is_contiguous() if t.dim() == 2 else t.transpose(1, 2).is_contiguous()
+
+
+def _aligned(t):
+    """Dense memory that starts on 16 bytes (what the kernels load)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.preserve_format)
+
+
+def _order(t):
+    """(dense tensor, its memory order)."""
+    if _point_major(t):
+        return _aligned(t), _POINT
+    if t.dim() == 2:
+        return _aligned(t.contiguous()), _POINT
+    return _aligned(t.contiguous()), _CHANNEL
+
+
+def _empty(shape, order, dtype, device):
+    if len(shape) == 3 and order == _POINT:
+        return torch.empty((shape[0], shape[2], shape[1]), dtype=dtype, device=device).transpose(1, 2)
+    return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _zeros(shape, order, dtype, device):
+    return _empty(shape, order, dtype, device).zero_()
+
+
+def _swap(src, B, R, C, dst):
+    """[B, R, C] -> [B, C, R], dense memory of the same type."""
+    lib = _lib.lib()
+    fn = lib.cl3d_transpose if src.dtype == torch.float32 else lib.cl3d_transpose16
+    with _lib.on_device(src.device):
+        _lib.check(fn(_p(src), B, R, C, _p(dst), _lib.stream_ptr(src.device)))
+    return dst
+
+
+def _as_order(t, order):
+    """t in the given memory order: itself, or a copy by the engine's transpose."""
+    t, have = _order(t)
+    if t.dim() == 2 or have == order or t.numel() == 0:
+        return t
+    if order == _CHANNEL and t.is_contiguous():
+        return t
+    B, C, N = t.shape
+    out = _empty(t.shape, order, t.dtype, t.device)
+    if order == _POINT:
+        _swap(t, B, C, N, out)
+    else:
+        _swap(t, B, N, C, out)
+    return out
+
+
+class _Reorder(Function):
+    @staticmethod
+    def forward(ctx, x, order):
+        ctx.back = _order(x)[1]
+        return _as_order(x, order).view_as(x)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        return _as_order(g, ctx.back), None
+
+
+def to_point_major(features):
+    """(B, C, N) features as a view of dense (B, N, C) rows, by the engine's transpose where they do not lie so already."""
+    _check_features(features, 'to_point_major', 'features')
+    return features if _point_major(features) else _Reorder.apply(features, _POINT)
+
+
+def to_channel_major(features):
+    """(B, C, N) features as dense channel-major memory, what the other operators of this package read."""
+    _check_features(features, 'to_channel_major', 'features')
+    return features if features.is_contiguous() else _Reorder.apply(features, _CHANNEL)
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# Autograd runs a leaf's gradient on the stream that was current when the leaf's node was made, and keeps that node while any
+# graph of the leaf lives.  A backward pass captured meanwhile, on another stream, is handed over to that stream, which no capture
+# joins: ending it takes the process down.  Every eager graph of these operators is therefore known by its context while it lives
+# (autograd frees the context with the graph), and a captured backward pass of the same leaves says so instead.
+_LIVE = weakref.WeakSet()
+
+
+def _track(ctx, *inputs):
+    """Called by a forward pass that autograd records, with the tensors it was given."""
+    leaves = [weakref.ref(t) for t in inputs if t is not None and t.is_leaf and t.requires_grad]
+    if leaves and not torch.cuda.is_current_stream_capturing():
+        ctx.leaves, ctx.made_on = leaves, torch.cuda.current_stream(inputs[0].device).cuda_stream
+        _LIVE.add(ctx)
+    elif leaves:
+        ctx.leaves, ctx.made_on = leaves, None
+
+
+def _check_capture(ctx, device):
+    """Called by a backward pass."""
+    if not _LIVE or not torch.cuda.is_current_stream_capturing():
+        return
+    mine = {id(t) for t in (r() for r in getattr(ctx, 'leaves', ())) if t is not None}
+    stream = torch.cuda.current_stream(device).cuda_stream
+    for other in list(_LIVE):
+        if other is not ctx and other.made_on != stream and any(id(r()) in mine for r in other.leaves if r() is not None):
+            raise RuntimeError("a backward pass is being captured while an eager graph of the same leaves, made on another stream, is "
+                               "alive: delete its outputs first, or warm up and capture on one stream (closerlook3d_amd.step_stream())")
+
+
+# ------------------------------------------------------------------------------------------------- gated feed-forward
+class _GatedFeedForward(Function):
+    """One C-ABI call per direction.  Kept for the backward pass: x and the weights (the hidden activations are formed again)."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, activation, precision, need_grad):
+        shape = x.shape
+        B, C, N = _sizes(x)
+        if need_grad:
+            _track(ctx, x, w_gate, w_up, w_down)
+        x, order = _order(x)
+        w_gate, w_up = _aligned(w_gate.contiguous()), _aligned(w_up.contiguous())
+        w_down = None if w_down is None else _aligned(w_down.contiguous())
+        H = w_gate.shape[0]
+        y = _empty((shape[0], C if w_down is not None else H) + tuple(shape[2:]), order, x.dtype, x.device)
+        dtype = _DTYPES[x.dtype]
+        if y.numel():
+            lib = _lib.lib()
+            flags = dtype | order << 2 | precision << 3 | (w_down is not None) << 4
+            nbytes = lib.cl3d_workspace_bytes(_OP_GATED_FFN, B, N, H, flags, C)
+            ws = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device=x.device)
+            with _lib.on_device(x.device):
+                _lib.check(lib.cl3d_gated_ffn_fwd(_p(x), _p(w_gate), _p(w_up), _p(w_down), dtype, order, B, C, N, H, activation,
+                                                  precision, _p(y), _p(ws), nbytes, _lib.stream_ptr(x.device)))
+        ctx.save_for_backward(x, w_gate, w_up, w_down)
+        ctx.args = (order, B, C, N, H, activation, precision)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w_gate, w_up, w_down = ctx.saved_tensors
+        _check_capture(ctx, x.device)
+        order, B, C, N, H, activation, precision = ctx.args
+        need = ctx.needs_input_grad
+        new = torch.empty_like if x.numel() else torch.zeros_like
+        dx = _empty(x.shape, order, x.dtype, x.device) if need[0] else None
+        dwg = new(w_gate) if need[1] else None
+        dwu = new(w_up) if need[2] else None
+        dwd = new(w_down) if w_down is not None and need[3] else None
+        if x.numel():
+            dy = _as_order(dy, order)
+            lib, dtype = _lib.lib(), _DTYPES[x.dtype]
+            wants = (dx is not None) | (dwg is not None or dwu is not None) << 1 | (dwd is not None) << 2
+            flags = dtype | order << 2 | precision << 3 | (w_down is not None) << 4 | 32 | wants << 6
+            nbytes = lib.cl3d_workspace_bytes(_OP_GATED_FFN, B, N, H, flags, C)
+            ws = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device=x.device)
+            with _lib.on_device(x.device):
+                _lib.check(lib.cl3d_gated_ffn_bwd(_p(x), _p(w_gate), _p(w_up), _p(w_down), _p(dy), dtype, order, B, C, N, H,
+                                                  activation, precision, _p(dx), _p(dwg), _p(dwu), _p(dwd), _p(ws), nbytes,
+                                                  _lib.stream_ptr(x.device)))
+        return dx, dwg, dwu, dwd, None, None, None
+
+
+def gated_feed_forward(x, w_gate, w_up, w_down=None, activation='silu', precision='f32'):
+    """y = (act(x w_gate^T) * (x w_up^T)) w_down^T for every point of x, (B, C, N) features or (R, C) rows.
+
+    w_gate, w_up (H, C) and w_down (C, H) have x's type; w_down None: the product of the two projections itself, with H channels.
+    activation 'silu', 'gelu' (by the error function) or 'relu'.  precision, of float32 tensors: 'f32' multiplies at f32 accuracy,
+    'bf16' rounds what enters a product to bfloat16, as in the other operators of this package; 16-bit tensors enter as they are.
+    The hidden activations are rounded to the tensors' type (f32: kept) in front of the last product."""
+    who = 'gated_feed_forward'
+    _check_features(x, who)
+    C = x.shape[1]
+    _check_param(w_gate, (w_gate.shape[0] if isinstance(w_gate, torch.Tensor) and w_gate.dim() == 2 else 'H', C), x, who, 'w_gate',
+                 optional=False, f32=False)
+    H = w_gate.shape[0]
+    _check_param(w_up, (H, C), x, who, 'w_up', optional=False, f32=False)
+    _check_param(w_down, (C, H), x, who, 'w_down', f32=False)
+    if C == 0 or H == 0:
+        raise ValueError(f"{who}: no channels")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"{who}: activation is one of {sorted(_ACTIVATIONS)}, got {activation!r}")
+    if precision not in _PRECISIONS:
+        raise ValueError(f"{who}: precision is one of {sorted(_PRECISIONS)}, got {precision!r}")
+    return _GatedFeedForward.apply(x, w_gate, w_up, w_down, _ACTIVATIONS[activation], _PRECISIONS[precision],
+                                   _wants_grad(x, w_gate, w_up, w_down))
+
+
+# ---------------------------------------------------------------------------------------------- norms around a block
+class _NormResidual(Function):
+    """cl3d_norm_residual_fwd / _bwd on point-major rows."""
+
+    @staticmethod
+    def forward(ctx, x, y, weight, bias, gate, next_weight, next_bias, rng, opts):
+        kind, next_kind, eps, next_eps, scale, p, need_grad = opts
+        shape, dtype, device = x.shape, x.dtype, x.device
+        B, C, N = _sizes(x)
+        order = _order(x)[1]
+        xr = _as_order(x, _POINT)
+        yr = None if y is None else _as_order(y, _POINT)
+        params = [weight, bias, gate, next_weight, next_bias]
+        f32 = any(t is not None and t.dtype == torch.float32 for t in params)
+        # (one type for all of them: a mixture goes to f32)
+        held = [None if t is None else (t.float() if f32 else t).contiguous() for t in params]
+        block = _lib.NormResidual(B=B, N=N, C=C, dtype=_DTYPES[dtype], param_f32=int(f32), kind=kind, next_kind=next_kind,
+                                  gate_cloud=int(gate is not None and gate.dim() == 2), residual_scale=scale, eps=eps,
+                                  next_eps=next_eps, p=p)
+        out = _empty(shape, _POINT, dtype, device) if y is not None else None
+        nxt = _empty(shape, _POINT, dtype, device) if next_kind else None
+        stats = torch.empty((B * N, 4), dtype=torch.float32, device=device) if need_grad else None
+        _fill(block, rng=rng, x=xr, y=yr, weight=held[0], bias=held[1], gate=held[2], next_weight=held[3], next_bias=held[4], out=out,
+              next=nxt, stats=stats)
+        if x.numel():
+            with _lib.on_device(device):
+                _lib.check(_lib.lib().cl3d_norm_residual_fwd(ctypes.byref(block), _lib.stream_ptr(device)))
+        ctx.set_materialize_grads(False)
+        if need_grad:
+            _track(ctx, x, y, *params)
+            ctx.save_for_backward(xr if next_kind else None, yr, *held, rng, stats)  # (an exit alone: x is not looked at again)
+            ctx.args = (order, B, C, N, f32, shape, dtype, kind, next_kind, scale, p, eps, next_eps,
+                        [None if t is None else t.dtype for t in params])
+        out = None if out is None else _as_order(out, order)
+        nxt = None if nxt is None else _as_order(nxt, order)
+        return out, nxt
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dnext):
+        xr, yr, weight, bias, gate, next_weight, next_bias, rng, stats = ctx.saved_tensors
+        order, B, C, N, f32, shape, dtype, kind, next_kind, scale, p, eps, next_eps, types = ctx.args
+        need, device = ctx.needs_input_grad, stats.device
+        _check_capture(ctx, device)
+        if dout is None and dnext is None:
+            return (None,) * 9
+        dout = None if dout is None else _as_order(dout, _POINT)
+        dnext = None if dnext is None else _as_order(dnext, _POINT)
+        dx = _empty(shape, _POINT, dtype, device) if need[0] else None
+        dy = _empty(shape, _POINT, dtype, device) if yr is not None and need[1] else None
+        empty = B * N == 0
+        grads = [None if t is None or not n else (torch.zeros_like(t) if empty else torch.empty_like(t))
+                 for t, n in zip((weight, bias, gate, next_weight, next_bias), need[2:7])]
+        if not empty:
+            lib = _lib.lib()
+            block = _lib.NormResidual(B=B, N=N, C=C, dtype=_DTYPES[dtype], param_f32=int(f32), kind=kind, next_kind=next_kind,
+                                      gate_cloud=int(gate is not None and gate.dim() == 2), residual_scale=scale, eps=eps,
+                                      next_eps=next_eps, p=p)
+            nbytes = lib.cl3d_workspace_bytes(_OP_POINT_NORM, B, N, 0, 0, C) if any(g is not None for g in grads) else 0
+            ws = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device=device)
+            _fill(block, rng=rng, x=xr, y=yr, weight=weight, bias=bias, gate=gate, next_weight=next_weight, next_bias=next_bias,
+                  stats=stats, dout=dout, dnext=dnext, dx=dx, dy=dy, dweight=grads[0], dbias=grads[1], dgate=grads[2],
+                  dnext_weight=grads[3], dnext_bias=grads[4], ws=ws)
+            block.ws_bytes = nbytes
+            with _lib.on_device(device):
+                _lib.check(lib.cl3d_norm_residual_bwd(ctypes.byref(block), _lib.stream_ptr(device)))
+        grads = [None if g is None else g.to(t) for g, t in zip(grads, types)]
+        return (None if dx is None else _as_order(dx, order), None if dy is None else _as_order(dy, order), *grads, None, None)
+
+
+def _fill(block, **tensors):
+    for name, t in tensors.items():
+        setattr(block, name, _p(t))
+
+
+def _check_norm(x, kind, eps, who, none=False):
+    if kind not in _NORMS or (kind == 'none' and not none):
+        raise ValueError(f"{who}: a norm is one of {[k for k in _NORMS if none or k != 'none']}, got {kind!r}")
+    if not eps >= 0:
+        raise ValueError(f"{who}: eps is not negative, got {eps}")
+    if not 0 < x.shape[1] <= _MAX_NORM_CHANNELS:
+        raise ValueError(f"{who}: 1 to {_MAX_NORM_CHANNELS} channels, got {x.shape[1]}")
+
+
+def point_norm(x, weight=None, bias=None, kind='rms', eps=1e-6):
+    """norm(x) weight + bias over the channels of every point: the entry of a block.
+
+    kind 'rms': x / sqrt(mean x^2 + eps); 'layer': (x - mean) / sqrt(var + eps), the variance over all C.  weight, bias (C,), of x's
+    type or float32; None: 1 and 0."""
+    who = 'point_norm'
+    _check_features(x, who)
+    _check_norm(x, kind, eps, who)
+    C = x.shape[1]
+    _check_param(weight, (C,), x, who, 'weight')
+    _check_param(bias, (C,), x, who, 'bias')
+    need = _wants_grad(x, weight, bias)
+    return _NormResidual.apply(x, None, None, None, None, weight, bias, None, (0, _NORMS[kind], 0.0, float(eps), 1.0, 0.0, need))[1]
+
+
+def norm_gate_residual(x, y, weight=None, bias=None, gate=None, residual_scale=1.0, kind='rms', eps=1e-6, p=0.0, rng=None,
+                       next_kind=None, next_weight=None, next_bias=None, next_eps=None):
+    """The exit of a block, and with next_kind the entry of the one that follows, in one pass over the points:
+
+        out = residual_scale * x + gate * dropout(norm(y) weight + bias, p)          next = norm(out) next_weight + next_bias
+
+    x: the residual stream, y: the block's result, same shape and type.  kind 'rms', 'layer' or 'none' (y is added as it is).  gate
+    (C,), or (B, C) for a gate of each cloud (for rows: of each row), or None.  p, rng: as in dropout(); element (b, c, n) is number
+    (b N + n) C + c of the draw.  next is formed from out before out is rounded.  Returns out, or (out, next) with next_kind."""
+    who = 'norm_gate_residual'
+    _check_features(x, who)
+    _check_features(y, who, 'y')
+    if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device:
+        raise ValueError(f"{who}: x and y have one shape, type and device, got {tuple(x.shape)} {x.dtype} and {tuple(y.shape)} {y.dtype}")
+    _check_norm(x, kind, eps, who, none=True)
+    B, C, _ = _sizes(x)
+    _check_param(weight, (C,), x, who, 'weight')
+    _check_param(bias, (C,), x, who, 'bias')
+    _check_param(gate, (B, C) if isinstance(gate, torch.Tensor) and gate.dim() == 2 else (C,), x, who, 'gate')
+    if next_kind is None:
+        if next_weight is not None or next_bias is not None:
+            raise ValueError(f"{who}: a weight or bias of a norm that is not asked for (next_kind)")
+        next_kind = 'none'
+    else:
+        _check_norm(x, next_kind, eps if next_eps is None else next_eps, who)
+    _check_param(next_weight, (C,), x, who, 'next_weight')
+    _check_param(next_bias, (C,), x, who, 'next_bias')
+    p = _check_p(p, who)
+    if p > 0:
+        _check_rng(rng, x, who)
+    need = _wants_grad(x, y, weight, bias, gate, next_weight, next_bias)
+    out, nxt = _NormResidual.apply(x, y, weight, bias, gate, next_weight, next_bias, rng if p > 0 else None,
+                                   (_NORMS[kind], _NORMS[next_kind], float(eps), float(eps if next_eps is None else next_eps),
+                                    float(residual_scale), p, need))
+    return out if next_kind == 'none' else (out, nxt)
+
+
+# ---------------------------------------------------------------------------------------------------------- dropout
+def _check_p(p, who):
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"{who}: a probability is in [0, 1], got {p}")
+    return p
+
+
+def _check_rng(rng, x, who):
+    if not isinstance(rng, torch.Tensor) or rng.dtype != torch.int64 or tuple(rng.shape) != (2,) or not rng.is_contiguous():
+        raise TypeError(f"{who}: rng is a dense int64 tensor (seed, offset)")
+    if rng.device != x.device:
+        raise RuntimeError(f"{who}: rng is on {rng.device}, x on {x.device}")
+
+
+class _Dropout(Function):
+    @staticmethod
+    def forward(ctx, x, p, rng):
+        ctx.save_for_backward(rng)
+        ctx.p = p
+        _track(ctx, x)
+        return _drop(x, p, rng)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        _check_capture(ctx, g.device)
+        return _drop(g, ctx.p, ctx.saved_tensors[0]), None, None
+
+
+def _drop(x, p, rng):
+    x = x.contiguous()
+    out = torch.empty_like(x)
+    with _lib.on_device(x.device):
+        _lib.check(_lib.lib().cl3d_dropout(_p(x), _DTYPES[x.dtype], x.numel(), p, _p(rng), _p(out), _lib.stream_ptr(x.device)))
+    return out
+
+
+def dropout(x, p, rng):
+    """x / (1 - p) where word i of the draw is at least floor(p 2^32), else 0; i counts x's elements in the order of its dimensions.
+
+    rng: int64 (2,) on x's device, (seed, offset).  Word i is number i % 4 of block offset + i / 4 of Philox 4x32-10 under the key
+    `seed`: a draw of n elements uses ceil(n / 4) blocks (CounterRng hands out draws that do not overlap).  The numbers are read on
+    the device, by the backward pass too: they must not be changed in between (autograd notices).  A dropped element is 0 whatever
+    it was.  p = 0 returns x, p = 1 zeros.  x: any shape; float32, bfloat16 or float16."""
+    who = 'dropout'
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{who}: x is a tensor, got {type(x).__name__}")
+    if not x.is_cuda:
+        raise RuntimeError(f"{who}: CPU not supported")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"{who}: x is float32, bfloat16 or float16, got {x.dtype}")
+    p = _check_p(p, who)
+    if p == 0.0:
+        return x
+    _check_rng(rng, x, who)
+    return _Dropout.apply(x, p, rng)
+
+
+class CounterRng:
+    """The state of a counter-based generator on one device: take(n) returns the (seed, offset) of a draw of n elements and moves
+    on, by one small launch on the current stream -- a captured step draws anew in every replay."""
+
+    def __init__(self, seed, device):
+        seed = int(seed)
+        if not -2 ** 63 <= seed < 2 ** 64:
+            raise ValueError(f"CounterRng: a seed has 64 bits, got {seed}")
+        self.state = torch.tensor([seed - 2 ** 64 if seed >= 2 ** 63 else seed, 0], dtype=torch.int64).to(device)
+        if not self.state.is_cuda:
+            raise RuntimeError("CounterRng: CPU not supported")
+
+    def take(self, n):
+        if n < 0:
+            raise ValueError(f"CounterRng.take: {n} elements")
+        out = torch.empty_like(self.state)
+        with _lib.on_device(out.device):
+            _lib.check(_lib.lib().cl3d_rng_take(_p(self.state), (n + 3) // 4, _p(out), _lib.stream_ptr(out.device)))
+        return out
+
+
+# ---------------------------------------------------------------------------------------------------------- modules
+class _Draws:
+    """A module's generator: made on the device of its first input, from `seed` or, when that is None, from torch's CPU generator."""
+
+    def __init__(self, seed):
+        self.seed, self.rng = seed, None
+
+    def take(self, x):
+        if self.rng is None or self.rng.state.device != x.device:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("dropout: run the module once before its step is captured (its generator is made on first use)")
+            if self.seed is None:
+                self.seed = int(torch.randint(0, 2 ** 62, (1,)).item())
+            self.rng = CounterRng(self.seed, x.device)
+        return self.rng.take(x.numel())
+
+
+class CounterDropout(nn.Module):
+    """nn.Dropout by dropout(): no mask in memory.  Every call in training mode is a draw of its own."""
+
+    def __init__(self, p=0.5, seed=None):
+        super().__init__()
+        self.p = _check_p(p, 'CounterDropout')
+        self._draws = _Draws(seed)
+
+    def forward(self, x):
+        if not self.training or self.p == 0.0:
+            return x
+        return dropout(x, self.p, self._draws.take(x))
+
+    def extra_repr(self):
+        return f"p={self.p}"
+
+
+class GatedFeedForward(nn.Module):
+    """gated_feed_forward() with its weights, initialised as nn.Linear's."""
+
+    def __init__(self, channels, hidden, activation='silu', precision='f32'):
+        super().__init__()
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"GatedFeedForward: activation is one of {sorted(_ACTIVATIONS)}, got {activation!r}")
+        self.activation, self.precision = activation, precision
+        self.w_gate = nn.Parameter(torch.empty(hidden, channels))
+        self.w_up = nn.Parameter(torch.empty(hidden, channels))
+        self.w_down = nn.Parameter(torch.empty(channels, hidden))
+        for w in (self.w_gate, self.w_up, self.w_down):
+            nn.init.kaiming_uniform_(w, a=5 ** 0.5)
+
+    def forward(self, x):
+        return gated_feed_forward(x, self.w_gate, self.w_up, self.w_down, self.activation, self.precision)
+
+
+class FeedForwardBlock(nn.Module):
+    """features -> residual_scale * features + gate * dropout(post_norm(gated_feed_forward(pre_norm(features)))).
+
+    pre_norm and post_norm: 'rms', 'layer', or for post_norm 'none' (the default).  gate: a learned number per channel, from
+    `gate_init`; None: none.  (B, C, N) features in either memory order; the result is channel-major when they are."""
+
+    def __init__(self, channels, hidden, activation='silu', pre_norm='rms', post_norm='none', eps=1e-6, gate_init=1.0,
+                 residual_scale=1.0, dropout=0.0, precision='f32', seed=None):
+        super().__init__()
+        if pre_norm not in ('rms', 'layer') or post_norm not in _NORMS:
+            raise ValueError(f"FeedForwardBlock: norms are 'rms' or 'layer' (post_norm: or 'none'), got {pre_norm!r}, {post_norm!r}")
+        self.pre_norm, self.post_norm, self.eps, self.residual_scale = pre_norm, post_norm, eps, residual_scale
+        self.p = _check_p(dropout, 'FeedForwardBlock')
+        self._draws = _Draws(seed)
+
+        def vector(value, present):
+            return nn.Parameter(torch.full((channels,), float(value))) if present else None
+
+        self.pre_weight, self.pre_bias = vector(1.0, True), vector(0.0, pre_norm == 'layer')
+        self.post_weight, self.post_bias = vector(1.0, post_norm != 'none'), vector(0.0, post_norm == 'layer')
+        self.gate = vector(gate_init, gate_init is not None) if gate_init is not None else None
+        self.feed_forward = GatedFeedForward(channels, hidden, activation, precision)
+
+    def forward(self, features):
+        channel_major = features.dim() == 3 and not _point_major(features)
+        x = to_point_major(features)
+        y = self.feed_forward(point_norm(x, self.pre_weight, self.pre_bias, self.pre_norm, self.eps))
+        p = self.p if self.training else 0.0
+        out = norm_gate_residual(x, y, self.post_weight, self.post_bias, self.gate, self.residual_scale, self.post_norm, self.eps,
+                                 p, self._draws.take(x) if p > 0 else None)
+        return to_channel_major(out) if channel_major else out

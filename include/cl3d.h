@@ -65,6 +65,9 @@ typedef void *cl3d_stream_t; /* hipStream_t */
 #define CL3D_OP_CONV1X1 15       /* cl3d_conv1x1_bwd_weight: (B, N, M = Cout, K unused, C = Cin) */
 #define CL3D_OP_SPHERE_CROP 16   /* cl3d_sphere_crop_query: N = scene points; _assemble: N = num_points */
 
+#define CL3D_OP_GATED_FFN 17     /* cl3d_gated_ffn_fwd/bwd: (B, N, M = hidden, K = CL3D_FFN_* flags, C) */
+#define CL3D_OP_POINT_NORM 18    /* cl3d_norm_residual_bwd: (B, N, M, K unused, C) */
+
 int cl3d_abi_version(void);
 const char *cl3d_last_error_string(void);
 /* operation order of the squared distance this build compares against radius^2 (build-time CL3D_D2_FORM, see
@@ -533,6 +536,75 @@ typedef struct cl3d_reduce_pass {
 } cl3d_reduce_pass;
 int cl3d_reduce_train_forward(const cl3d_reduce_pass *p, cl3d_stream_t stream);
 int cl3d_reduce_train_backward(const cl3d_reduce_pass *p, cl3d_stream_t stream);
+
+/* ---- per-point feed-forward operators: csrc/gated_ffn.hip, point_norm.hip, dropout.hip ------------------------------------
+ * Tensors of one call share an element type and a memory order: features are point-major rows [B,N,C] or, as everywhere else in
+ * this header, channel-major [B,C,N].  Arithmetic is f32 inside, a 16-bit result is rounded once. */
+#define CL3D_F32 0
+#define CL3D_BF16 1
+#define CL3D_F16 2
+#define CL3D_POINT_MAJOR 0
+#define CL3D_CHANNEL_MAJOR 1
+#define CL3D_ACT_SILU 0
+#define CL3D_ACT_GELU 1 /* x Phi(x), Phi by the error function */
+#define CL3D_ACT_RELU 2
+
+/* y = (act(x w_gate^T) * (x w_up^T)) w_down^T for every point.  w_gate, w_up [H,C], w_down [C,H] (NULL: y is the product of the
+ * two projections, H channels).  precision 0: f32 tensors are multiplied at f32 accuracy; 1: their values are rounded to bf16 in
+ * front of every product (16-bit tensors: no difference).  Tensors start on 16 bytes.  Scratch:
+ * cl3d_workspace_bytes(CL3D_OP_GATED_FFN, B, N, H, flags, C) with the flags below. */
+#define CL3D_FFN_FLAGS(dtype, order, precision, down) ((dtype) | (order) << 2 | (precision) << 3 | (down) << 4)
+#define CL3D_FFN_BACKWARD 32
+#define CL3D_FFN_DX 1u      /* which gradients: << 6 in the flags */
+#define CL3D_FFN_DW_IN 2u
+#define CL3D_FFN_DW_DOWN 4u
+int cl3d_gated_ffn_fwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, int dtype, int order, int B, int C,
+                       int N, int H, int activation, int precision, void *y, void *ws, size_t ws_bytes, cl3d_stream_t stream);
+/* gradients for dy (shape, type and order of y); dx, dw_gate, dw_up, dw_down: NULL where not wanted.  Products of the two
+ * projections are formed again from x.  Weight gradients are summed in a fixed order: bit-identical run to run. */
+int cl3d_gated_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *dy, int dtype,
+                       int order, int B, int C, int N, int H, int activation, int precision, void *dx, void *dw_gate,
+                       void *dw_up, void *dw_down, void *ws, size_t ws_bytes, cl3d_stream_t stream);
+
+/* [B,R,C] -> [B,C,R] of 16-bit elements (cl3d_transpose: f32) */
+int cl3d_transpose16(const void *src, int B, int R, int C, void *dst, cl3d_stream_t stream);
+
+/* Exit of a block and entry of the next, one pass over the points (point-major rows [B,N,C]):
+ *     n = norm(y) weight + bias;  out = residual_scale x + gate * drop(n);  next = next_norm(out) next_weight + next_bias
+ * y NULL: there is no block to leave, next = next_norm(x) next_weight + next_bias.  next_kind CL3D_NORM_NONE: no entry.
+ * rms: v / sqrt(mean v^2 + eps); layer: (v - mean) / sqrt(var + eps), over the channels of a point.  weight, bias, gate,
+ * next_weight, next_bias: [C] (gate [B,C] with gate_cloud), NULL: 1, 0, 1, 1, 0; of the tensors' type, or f32 with param_f32.
+ * p, rng: as in cl3d_dropout, element (b, n, c) being number (b N + n) C + c.  stats [B,N,4]: what the backward pass needs of
+ * the forward pass, besides its inputs (NULL: no backward pass follows).
+ * Backward (x, y and the parameters as in the forward pass, out and next not read): dout, dnext are the gradients of out and next (either may be NULL: zero); dx, dy and the parameters' gradients
+ * (shapes and types of what they belong to) NULL where not wanted; ws: cl3d_workspace_bytes(CL3D_OP_POINT_NORM, B, N, 0, 0, C)
+ * where a parameter's gradient is.  Sums over the points are taken in a fixed order: bit-identical run to run. */
+#define CL3D_NORM_NONE 0
+#define CL3D_NORM_RMS 1
+#define CL3D_NORM_LAYER 2
+typedef struct cl3d_norm_residual {
+  int B, N, C, dtype, param_f32, kind, next_kind, gate_cloud;
+  float residual_scale, eps, next_eps;
+  int reserved; /* (what would be padding) */
+  double p;
+  const int64_t *rng;
+  const void *x, *y, *weight, *bias, *gate, *next_weight, *next_bias;
+  void *out, *next;
+  float *stats;
+  const void *dout, *dnext;
+  void *dx, *dy, *dweight, *dbias, *dgate, *dnext_weight, *dnext_bias, *ws;
+  size_t ws_bytes;
+} cl3d_norm_residual;
+int cl3d_norm_residual_fwd(const cl3d_norm_residual *p, cl3d_stream_t stream);
+int cl3d_norm_residual_bwd(const cl3d_norm_residual *p, cl3d_stream_t stream);
+
+/* Dropout from a counter.  rng: two numbers in device memory, (seed, offset); element i of the n stays when word i % 4 of
+ * Philox 4x32-10 (counter offset + i / 4, key seed) is at least floor(p 2^32), and is multiplied by 1 / (1 - p); the others
+ * become 0.  The same call on a gradient is the backward pass: no mask is stored.  p in [0, 1]. */
+int cl3d_dropout(const void *x, int dtype, long long n, double p, const int64_t *rng, void *out, cl3d_stream_t stream);
+/* out = state, then state's offset += blocks: the counters of one draw (blocks = ceil(n / 4)), on the stream, so that a captured
+ * step draws anew in every replay. */
+int cl3d_rng_take(int64_t *state, long long blocks, int64_t *out, cl3d_stream_t stream);
 
 #ifdef __cplusplus
 }
