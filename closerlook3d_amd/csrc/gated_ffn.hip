@@ -18,22 +18,17 @@
 //     whose row index is contiguous (Wd in dh, Wg / Wu in dX, all operands of the weight gradients) lies as [64 k][row] and is
 //     read by ds_read_b64_tr_b16, which hands a lane four k of its row: no operand is transposed in memory;
 //   * workgroups are numbered so that neighbours in i, which share the rows of Q, run on one XCD and share its L2.
-// f32 tensors: an f32 value is the exact sum of three bf16 values (8 significant bits each, by truncation); the product takes the
-// six largest of the nine partial products on the bf16 units, smallest first, into one f32 accumulator.  What is left out is
-// below 2^-23 of |x||y|, as much as the rounding of an f32 product.  Six passes at the bf16 rate outrun the f32 MFMA (1/16 of it).
-// A value that is not finite takes part in the leading product only (a fourth plane holds 0 for it), so an infinity stays one.
+// f32 tensors: an f32 value is the exact sum of three bf16 values (8 significant bits each, by truncation: planes 0, 1, 2); a
+// product takes the six largest of the nine partial products on the bf16 units, smallest first, into one f32 accumulator.  What is
+// left out is below 2^-23 of |x||y|, as much as the rounding of an f32 product.  Six passes at the bf16 rate outrun the f32 MFMA
+// (1/16 of it).  A tile holds the three planes of 32 k, so each fragment is read once for its two or three products.  A value
+// that is not finite takes part in the product of the leading planes only, so an infinity stays one (not_finite below).
 #include "ff_common.h"
+#include <type_traits>
 
 namespace cl3d {
 
 typedef unsigned short u16;
-
-constexpr int kBK = 64;                // k per LDS tile
-constexpr int kRowBytes = kBK * 2;
-
-// which plane of P and Q each pass of a split product takes (0 leading, 1 middle, 2 last, 3 leading but 0 if not finite): hex
-// digits, the first pass lowest -- (2,3) (3,2) (1,1) (1,3) (3,1) (0,0)
-constexpr unsigned kSegP = 0x031132u, kSegQ = 0x013123u;
 
 template <typename E> __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c);
 template <> __device__ __forceinline__ f32x4 mfma16<Bf16>(s16x8 a, s16x8 b, f32x4 c) {
@@ -61,25 +56,35 @@ __device__ __forceinline__ void barrier_lds() {
 // ---- one operand's way into LDS.  KM false: rows of 64 k; true: 64 rows of ROWS elements.  `swz` is the XOR of a 16-byte
 // piece's place, chosen so that the 16 lanes of a fragment read cover all 64 banks: a k-contiguous fragment reads rows
 // r .. r + 15 (or, PAIRED, rows 8 a + b, a and b in 0..3) of which every second starts at the same bank.
-template <bool PAIRED> __device__ __forceinline__ int swz_kc(int row) {
+template <bool PAIRED, int BK> __device__ __forceinline__ int swz_kc(int row) {
+  if (BK == 32) return PAIRED ? (row >> 3) & 3 : (row >> 2) & 3;
   return PAIRED ? (((row >> 1) & 1) | ((row >> 2) & 6)) : ((row >> 1) & 7);
 }
 template <int ROWS> __device__ __forceinline__ int swz_km(int k) {  // (32-byte blocks: ds_read_b64_tr_b16 takes them whole)
-  return ROWS >= 128 ? (((k & 3) | ((k >> 1) & 4)) << 1) : ((((k >> 1) & 1) | ((k >> 2) & 2)) << 1);
+  if (ROWS % 128 == 0) return ((k & 3) | ((k >> 1) & 4)) << 1;
+  if (ROWS == 96) return ((k >> 3) & 1) << 1;
+  return (((k >> 1) & 1) | ((k >> 2) & 2)) << 1;  // 64
 }
 
-template <int ROWS, bool KM, bool PAIRED, int NW> struct Loader {
-  static constexpr int kPer = ROWS * 8 / (64 * NW);  // 16-byte pieces per lane
-  static_assert(kPer >= 1 && kPer * 64 * NW == ROWS * 8, "tile and workgroup do not match");
+template <int ROWS, bool KM, bool PAIRED, int NW, int BK> struct Loader {
+  static constexpr int kPieces = BK / 8;  // 16-byte pieces of a row of k
+  // loads of a wave, 64 pieces each; where the tile has fewer than the waves could fetch, the last waves fetch the first pieces
+  // again (the same bytes to the same place)
+  static constexpr int kAll = ROWS * kPieces / 64, kPer = (kAll + NW - 1) / NW;
+  static_assert(kAll * 64 == ROWS * kPieces, "a tile is a whole number of loads");
   unsigned off[kPer];
   int at[kPer];  // KM false: k of the piece
 
+  static __device__ __forceinline__ int load_of(int wave, int q) {
+    const int n = wave * kPer + q;
+    return n < kAll ? n : n - kAll;
+  }
   __device__ __forceinline__ void init(int ld, int rows, int wave, int lane) {
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
-      const int slot = (wave * kPer + q) * 64 + lane;
+      const int slot = load_of(wave, q) * 64 + lane;
       if (!KM) {
-        const int row = slot >> 3, chunk = (slot & 7) ^ swz_kc<PAIRED>(row);
+        const int row = slot / kPieces, chunk = (slot % kPieces) ^ swz_kc<PAIRED, BK>(row);
         at[q] = chunk * 8;
         off[q] = (unsigned)(row * ld + chunk * 8) * 2u;
       } else {
@@ -93,23 +98,23 @@ template <int ROWS, bool KM, bool PAIRED, int NW> struct Loader {
   // base: the tile's first row (KM false) or first k; rows / kleft: what is left of the tensor from there (multiples of 8
   // along the contiguous axis)
   __device__ __forceinline__ void issue(const u16 *base, int ld, int rows, int kleft, char *lds, int wave) const {
-    const int outer = KM ? (kleft < kBK ? kleft : kBK) : (rows < ROWS ? rows : ROWS), inner = KM ? rows : kleft;
+    const int outer = KM ? (kleft < BK ? kleft : BK) : (rows < ROWS ? rows : ROWS), inner = KM ? rows : kleft;
     const unsigned bytes = (unsigned)((outer - 1) * ld + inner) * 2u;
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, bytes, 0x00020000);
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
       unsigned o = off[q];
-      if (!KM && kleft < kBK) o = at[q] < kleft ? o : 0x80000000u;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, CL3D_LDS(void, lds + (wave * kPer + q) * 1024), 16, o, 0, 0, 0);
+      if (!KM && kleft < BK) o = at[q] < kleft ? o : 0x80000000u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, CL3D_LDS(void, lds + load_of(wave, q) * 1024), 16, o, 0, 0, 0);
     }
   }
 };
 
 // fragment of 16 rows for k = 32 kk .. 32 kk + 31: lane l holds row l & 15, k = 8 (l >> 4) .. + 7.
 // r0: first row of the 16 (PAIRED: of the 32; t says which half of every eight)
-template <bool PAIRED> __device__ __forceinline__ s16x8 frag_kc(const char *lds, int r0, int t, int kk, int lane) {
+template <bool PAIRED, int BK> __device__ __forceinline__ s16x8 frag_kc(const char *lds, int r0, int t, int kk, int lane) {
   const int m = lane & 15, row = r0 + (PAIRED ? 8 * (m >> 2) + 4 * t + (m & 3) : m);
-  return *reinterpret_cast<const s16x8 *>(lds + row * kRowBytes + (((kk * 4 + (lane >> 4)) ^ swz_kc<PAIRED>(row)) << 4));
+  return *reinterpret_cast<const s16x8 *>(lds + row * (BK * 2) + (((kk * 4 + (lane >> 4)) ^ swz_kc<PAIRED, BK>(row)) << 4));
 }
 template <int ROWS, bool PAIRED> __device__ __forceinline__ s16x8 frag_km(const char *lds, int r0, int t, int kk, int lane) {
   const int i = lane & 15, piece = i & 3;
@@ -134,103 +139,179 @@ struct Pair {
   int K, kp;  // k of the product (a multiple of 8 unless both operands are row-contiguous); rows a row-contiguous P really has
 };
 
-// acc[a][b] += the product over steps [s0, s1) of nseg * ceil(K / 64).  PR: rows of P in a tile (TWO: the first half from P, the
-// second from P2).  The wave (wi, wj) owns TI / 16 x TJ / 16 accumulators; TWO: first TI / 32 of P, then as many of P2, same rows.
-template <typename E, int PR, bool PKM, bool PAIRED, bool TWO, int QR, bool QKM, int TI, int TJ, int NW>
-__device__ __forceinline__ void product(f32x4 (&acc)[TI / 16][TJ / 16], const Pair &a, int nseg, int s0, int s1, char *smem,
-                                        int wave, int lane, int wi, int wj) {
-  constexpr int kPBytes = PR * kRowBytes, kStage = (PR + QR) * kRowBytes;
+// bit 15 of either half: a bf16 whose exponent is all ones
+__device__ __forceinline__ unsigned not_finite(unsigned two) { return (two & 0x7f807f80u) + 0x00800080u; }
+// ... and 0 in its place
+__device__ __forceinline__ s16x8 finite_or_0(s16x8 v) {
+  union { s16x8 s; unsigned u[4]; } f{v};
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const unsigned t = (not_finite(f.u[d]) & 0x80008000u) >> 15;
+    f.u[d] &= ~(t * 0xffffu);
+  }
+  return f.s;
+}
+
+// acc[a][b] += the product over the tiles of k [s0, s1).  PR: rows of P in a tile (TWO: the first half from P, the second from P2).
+// The wave (wi, wj) owns TI / 16 x TJ / 16 accumulators; TWO: first TI / 32 of P, then as many of P2, same rows.
+template <typename E, int NP, int BK, int kTiles, int PR, bool PKM, bool PAIRED, bool TWO, int QR, bool QKM, int TI, int TJ, int NW>
+__device__ __forceinline__ void product(f32x4 (&acc)[TI / 16][TJ / 16], const Pair &a, int s0, int s1, char *smem, int wave, int lane,
+                                        int wi, int wj) {
+  constexpr int kPBytes = PR * BK * 2, kQBytes = QR * BK * 2, kTile = NP * (kPBytes + kQBytes);
   constexpr int kPR = TWO ? PR / 2 : PR;
-  Loader<PR, PKM, PAIRED, NW> lp;
-  Loader<QR, QKM, false, NW> lq;
+  Loader<PR, PKM, PAIRED, NW, BK> lp;
+  Loader<QR, QKM, false, NW, BK> lq;
+  constexpr int kLoads = NP * (lp.kPer + lq.kPer);
   static_assert(!(TWO && PKM), "two matrices: k contiguous");
   // TWO: this wave's pieces are all of one matrix (kPR rows are a whole number of waves' shares)
-  const bool second = TWO && wave * lp.kPer * 8 >= kPR;
+  const bool second = TWO && lp.load_of(wave, 0) * 64 / lp.kPieces >= kPR;
+  static_assert(!TWO || kPR * lp.kPieces / 64 % lp.kPer == 0, "a wave loads of one matrix");
   lp.init(a.ldp, a.rows_p, wave, lane);
   lq.init(a.ldq, a.rows_q, wave, lane);
-  const int ksteps = (a.K + kBK - 1) / kBK;
   const u16 *Pb = a.P;
   if (TWO && second) Pb = a.P2 - (long long)kPR * a.ldp;
+  // rows behind the tile's end: beyond the descriptor (TWO: its rows are counted from the tile's first row)
+  const int rows_p = TWO ? (second ? a.rows_p + kPR : (a.rows_p < kPR ? a.rows_p : kPR)) : a.rows_p;
 
-  // (what a step reads is counted up, not divided out: a quotient is formed in vector registers, and the descriptors with it)
-  int seg = 0, k_next = 0, k_now = 0;
-  if (s0 > 0) {
-    seg = __builtin_amdgcn_readfirstlane(s0 / ksteps);
-    k_next = k_now = (s0 - seg * ksteps) * kBK;
-  }
-  auto issue = [&](int buf) {
-    const long long pp = nseg > 1 ? (long long)((kSegP >> 4 * seg) & 15u) * a.plane_p : 0, pq = nseg > 1 ? (long long)((kSegQ >> 4 * seg) & 15u) * a.plane_q : 0;
-    char *lds = smem + buf * kStage;
-    const u16 *P = Pb + pp + (PKM ? (long long)k_next * a.ldp : k_next), *Q = a.Q + pq + (QKM ? (long long)k_next * a.ldq : k_next);
-    // rows behind the tile's end: beyond the descriptor (TWO: its rows are counted from the tile's first row)
-    lp.issue(P, a.ldp, TWO && second ? a.rows_p + kPR : (TWO ? (a.rows_p < kPR ? a.rows_p : kPR) : a.rows_p),
-             (PKM ? a.kp : a.K) - k_next, lds, wave);
-    lq.issue(Q, a.ldq, a.rows_q, a.K - k_next, lds + kPBytes, wave);
-    k_next += kBK;
-    if (k_next >= a.K) {
-      k_next = 0;
-      ++seg;
+  auto issue = [&](int s, int place) {
+    const int k0 = s * BK;
+    char *lds = smem + place * kTile;
+    const u16 *P = Pb + (PKM ? (long long)k0 * a.ldp : k0), *Q = a.Q + (QKM ? (long long)k0 * a.ldq : k0);
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+      lp.issue(P + n * a.plane_p, a.ldp, rows_p, (PKM ? a.kp : a.K) - k0, lds + n * kPBytes, wave);
+      lq.issue(Q + n * a.plane_q, a.ldq, a.rows_q, a.K - k0, lds + NP * kPBytes + n * kQBytes, wave);
     }
   };
   if (s0 >= s1) return;
-  issue(0);
-  int buf = 0;
-  for (int s = s0; s < s1; ++s) {
-    if (s + 1 < s1) {
-      issue(buf ^ 1);
-      wait_vm<lp.kPer + lq.kPer>();
-    } else {
-      wait_vm<0>();
-    }
-    barrier_lds();
-    const char *lds = smem + buf * kStage;
-    const int k0 = k_now;
-    k_now = k_now + kBK >= a.K ? 0 : k_now + kBK;
+  int put = 0, get = 0;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      if (k0 + kk * 32 < a.K) {
-        s16x8 p[TI / 16], q[TJ / 16];
+  for (int q = 0; q < kTiles - 1; ++q)
+    if (s0 + q < s1) issue(s0 + q, put++);
+  for (int s = s0; s < s1; ++s) {
+    // this step's tile has arrived when no more than the loads of the later ones are outstanding; behind the barrier it has for
+    // every wave, and every wave has read the tile of the step before, whose place the next load takes
+    const int later = s1 - 1 - s < kTiles - 2 ? s1 - 1 - s : kTiles - 2;
+    if (later == 0) wait_vm<0>();
+    else if (later == 1) wait_vm<kLoads>();
+    else wait_vm<2 * kLoads>();
+    barrier_lds();
+    if (s + kTiles - 1 < s1) issue(s + kTiles - 1, put);
+    put = put + 1 == kTiles ? 0 : put + 1;
+    const char *lds = smem + get * kTile;
+    get = get + 1 == kTiles ? 0 : get + 1;
+#pragma unroll
+    for (int kk = 0; kk < BK / 32; ++kk) {
+      if (s * BK + kk * 32 >= a.K) break;
+      s16x8 p[NP][TI / 16], q[NP][TJ / 16];
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
 #pragma unroll
         for (int u = 0; u < TI / 16; ++u) {
           const int half = TWO ? u / (TI / 32) : 0, v = TWO ? u % (TI / 32) : u;
           const int r0 = half * kPR + wi * (TWO ? TI / 2 : TI) + (PAIRED ? (v >> 1) * 32 : v * 16);
-          p[u] = PKM ? frag_km<PR, PAIRED>(lds, r0, v & 1, kk, lane) : frag_kc<PAIRED>(lds, r0, v & 1, kk, lane);
+          const char *at = lds + n * kPBytes;
+          if constexpr (PKM) p[n][u] = frag_km<PR, PAIRED>(at, r0, v & 1, kk, lane);
+          else p[n][u] = frag_kc<PAIRED, BK>(at, r0, v & 1, kk, lane);
         }
 #pragma unroll
         for (int u = 0; u < TJ / 16; ++u) {
-          const int r0 = wj * TJ + u * 16;
-          q[u] = QKM ? frag_km<QR, false>(lds + kPBytes, r0, 0, kk, lane) : frag_kc<false>(lds + kPBytes, r0, 0, kk, lane);
+          const char *at = lds + NP * kPBytes + n * kQBytes;
+          if constexpr (QKM) q[n][u] = frag_km<QR, false>(at, wj * TJ + u * 16, 0, kk, lane);
+          else q[n][u] = frag_kc<false, BK>(at, wj * TJ + u * 16, 0, kk, lane);
         }
+      }
+      if constexpr (NP == 1) {
 #pragma unroll
         for (int u = 0; u < TI / 16; ++u)
 #pragma unroll
-          for (int v = 0; v < TJ / 16; ++v) acc[u][v] = mfma16<E>(p[u], q[v], acc[u][v]);
+          for (int v = 0; v < TJ / 16; ++v) acc[u][v] = mfma16<E>(p[0][u], q[0][v], acc[u][v]);
+      } else {
+        auto all = [&](const s16x8 (&x)[TI / 16], const s16x8 (&y)[TJ / 16]) {
+#pragma unroll
+          for (int u = 0; u < TI / 16; ++u)
+#pragma unroll
+            for (int v = 0; v < TJ / 16; ++v) acc[u][v] = mfma16<E>(x[u], y[v], acc[u][v]);
+        };
+        unsigned odd = 0;
+#pragma unroll
+        for (int u = 0; u < TI / 16; ++u) {
+          union { s16x8 s; unsigned d[4]; } f{p[0][u]};
+#pragma unroll
+          for (int d = 0; d < 4; ++d) odd |= not_finite(f.d[d]);
+        }
+#pragma unroll
+        for (int u = 0; u < TJ / 16; ++u) {
+          union { s16x8 s; unsigned d[4]; } f{q[0][u]};
+#pragma unroll
+          for (int d = 0; d < 4; ++d) odd |= not_finite(f.d[d]);
+        }
+        if (__builtin_expect(__any((odd & 0x80008000u) != 0u), 0)) {
+          s16x8 pf[TI / 16], qf[TJ / 16];
+#pragma unroll
+          for (int u = 0; u < TI / 16; ++u) pf[u] = finite_or_0(p[0][u]);
+#pragma unroll
+          for (int u = 0; u < TJ / 16; ++u) qf[u] = finite_or_0(q[0][u]);
+          all(p[2], qf);  // (in the order of the other branch: what is finite keeps its bits beside an infinity)
+          all(pf, q[2]);
+          all(p[1], q[1]);
+          all(p[1], qf);
+          all(pf, q[1]);
+          all(p[0], q[0]);
+        } else {
+          all(p[2], q[0]);
+          all(p[0], q[2]);
+          all(p[1], q[1]);
+          all(p[1], q[0]);
+          all(p[0], q[1]);
+          all(p[0], q[0]);
+        }
       }
     }
-    barrier_lds();
-    buf ^= 1;
   }
+  barrier_lds();  // (another product may follow in the same tiles)
 }
 
-// ---- activations (CL3D_ACT_SILU / _GELU / _RELU): value and slope at g
-__device__ __forceinline__ void activate(int act, float g, float &value, float &slope) {
+// ---- activations (CL3D_ACT_SILU / _GELU / _RELU): value and slope at g.  FAST: on the way to a 16-bit result, by the hardware's
+// exp2 and reciprocal (one step each) and the error function by Press et al., Numerical Recipes 6.2 (erfc to 1.2e-7 of itself
+// everywhere, so the tails keep their digits); otherwise by the math library.
+template <bool FAST> __device__ __forceinline__ void activate(int act, float g, float &value, float &slope) {
   if (act == CL3D_ACT_SILU) {
-    const float s = 1.f / (1.f + expf(-g));
+    const float s = FAST ? __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g)) : 1.f / (1.f + expf(-g));
     value = g * s;
     slope = s * __builtin_fmaf(g, 1.f - s, 1.f);
   } else if (act == CL3D_ACT_GELU) {
-    const float c = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+    float c, e;
+    if (FAST) {
+      const float z = 0.70710678118654752f * fabsf(g), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.5f, z, 1.f));
+      float q = 0.17087277f;
+      q = __builtin_fmaf(q, t, -0.82215223f);
+      q = __builtin_fmaf(q, t, 1.48851587f);
+      q = __builtin_fmaf(q, t, -1.13520398f);
+      q = __builtin_fmaf(q, t, 0.27886807f);
+      q = __builtin_fmaf(q, t, -0.18628806f);
+      q = __builtin_fmaf(q, t, 0.09678418f);
+      q = __builtin_fmaf(q, t, 0.37409196f);
+      q = __builtin_fmaf(q, t, 1.00002368f);
+      q = __builtin_fmaf(q, t, -1.26551223f);
+      e = __builtin_amdgcn_exp2f(-1.4426950408889634f * z * z);
+      const float tail = 0.5f * t * e * __builtin_amdgcn_exp2f(1.4426950408889634f * q);
+      c = g < 0.f ? tail : 1.f - tail;
+    } else {
+      c = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+      e = expf(-0.5f * g * g);
+    }
     value = g * c;
-    slope = __builtin_fmaf(g, 0.3989422804014327f * expf(-0.5f * g * g), c);
+    slope = __builtin_fmaf(g, 0.3989422804014327f * e, c);
   } else {  // relu; a NaN stays one, the slope at 0 is 0
     value = g < 0.f ? 0.f : g;
     slope = g > 0.f ? 1.f : (g <= 0.f ? 0.f : g);
   }
 }
 
-// an f32 value as the exact sum of three bf16 values by truncation; plane 3 is the leading one, 0 where x is not finite
+// an f32 value as the exact sum of three bf16 values by truncation (not finite: the leading one alone)
 struct Split {
-  u16 p[4];
+  u16 p[3];
 };
 __device__ __forceinline__ Split split3(float x) {
   const unsigned b = __float_as_uint(x), hi = b & 0xffff0000u;
@@ -238,14 +319,13 @@ __device__ __forceinline__ Split split3(float x) {
   s.p[0] = (u16)(hi >> 16);
   if ((b & 0x7f800000u) == 0x7f800000u) {
     if (b & 0x007fffffu) s.p[0] |= 0x40;  // a NaN whose payload sits in the low half stays a NaN
-    s.p[1] = s.p[2] = s.p[3] = 0;
+    s.p[1] = s.p[2] = 0;
     return s;
   }
   const float r = x - __uint_as_float(hi);
   const unsigned mid = __float_as_uint(r) & 0xffff0000u;
   s.p[1] = (u16)(mid >> 16);
   s.p[2] = (u16)(__float_as_uint(r - __uint_as_float(mid)) >> 16);
-  s.p[3] = s.p[0];
   return s;
 }
 
@@ -255,19 +335,19 @@ struct GemmArgs {
   long long plane_p, plane_q, plane_pb, plane_qb;
   int ldp, ldq, ldpb, ldqb;
   int I, J, K, Kb, kp;       // K, Kb multiples of 8 (zero-padded operands); kp: rows of the P whose rows run along i
-  int nseg, act;
+  int act;
   int slices;                // weight gradients: pieces of k
   int batch_q, batch_d;      // weight gradients: blockIdx.z picks Q + z * batch_q, D + z * batch_d
   void *D;                   // result rows of ldd elements of the tensor type (or f32 partials [slice][J][I])
   int ldd, vec;              // vec: rows start 16-byte aligned
-  u16 *h, *dgu;              // operand-type intermediates, ldh and 2 ldh a row, zero up to ldh; 4 planes when split
+  u16 *h, *dgu;              // operand-type intermediates, ldh and 2 ldh a row, zero up to ldh; 3 planes when split
   long long plane_h, plane_dgu;
   int ldh, planes;
   const void *dh;            // GATED_BWD without a down projection: dh itself, rows of lddh
   int lddh;
 };
 
-// four or eight consecutive elements of an internal row: operand type, or the four planes
+// four or eight consecutive elements of an internal row: operand type, or the three planes
 template <typename E, int N> __device__ __forceinline__ void put_internal(u16 *row, long long plane, int planes, const float *v) {
   if (planes == 1) {
     u16 o[N];
@@ -277,15 +357,15 @@ template <typename E, int N> __device__ __forceinline__ void put_internal(u16 *r
     else *reinterpret_cast<s16x4 *>(row) = *reinterpret_cast<s16x4 *>(o);
     return;
   }
-  u16 o[4][N];
+  u16 o[3][N];
 #pragma unroll
   for (int e = 0; e < N; ++e) {
     const Split s = split3(v[e]);
 #pragma unroll
-    for (int p = 0; p < 4; ++p) o[p][e] = s.p[p];
+    for (int p = 0; p < 3; ++p) o[p][e] = s.p[p];
   }
 #pragma unroll
-  for (int p = 0; p < 4; ++p) {
+  for (int p = 0; p < 3; ++p) {
     if constexpr (N == 8) *reinterpret_cast<s16x8 *>(row + p * plane) = *reinterpret_cast<s16x8 *>(o[p]);
     else *reinterpret_cast<s16x4 *>(row + p * plane) = *reinterpret_cast<s16x4 *>(o[p]);
   }
@@ -319,7 +399,7 @@ __device__ __forceinline__ int xcd_order(int id, int total) {
 
 // E: operand type; T: type of the caller's tensors.  A workgroup of WI x WJ waves owns BI x BJ results (GATED*: BI is twice the
 // channels).
-template <int KIND, typename E, typename T, int BI, int BJ, int WI, int WJ>
+template <int KIND, typename E, typename T, int NP, int BI, int BJ, int WI, int WJ, int BK, int TILES>
 __global__ __launch_bounds__(64 * WI * WJ) void ffn_gemm_kernel(GemmArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   constexpr int NW = WI * WJ, TI = BI / WI, TJ = BJ / WJ;
@@ -344,8 +424,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void ffn_gemm_kernel(GemmArgs a) {
   if constexpr (KIND == GEMM_GATED || KIND == GEMM_GATED_BWD) {
     Pair pr{a.P + (long long)i0 * a.ldp, a.P2 + (long long)i0 * a.ldp, a.Q + (long long)j0 * a.ldq, a.plane_p, a.plane_q,
             a.ldp, a.ldq, a.I - i0, a.J - j0, a.K, a.K};
-    const int steps = (a.K + kBK - 1) / kBK * a.nseg;
-    product<E, BI, false, true, true, BJ, false, TI, TJ, NW>(acc, pr, a.nseg, 0, steps, smem, wave, lane, wi, wj);
+    const int steps = (a.K + BK - 1) / BK;
+    product<E, NP, BK, TILES, BI, false, true, true, BJ, false, TI, TJ, NW>(acc, pr, 0, steps, smem, wave, lane, wi, wj);
     f32x4 dh[TI / 32][TJ / 16];
     if constexpr (KIND == GEMM_GATED_BWD) {
 #pragma unroll
@@ -355,8 +435,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void ffn_gemm_kernel(GemmArgs a) {
       if (a.Qb != nullptr) {
         Pair pb{a.Pb + i0, nullptr, a.Qb + (long long)j0 * a.ldqb, a.plane_pb, a.plane_qb, a.ldpb, a.ldqb, ip - i0, a.J - j0, a.Kb,
                 a.kp};
-        const int sb = (a.Kb + kBK - 1) / kBK * a.nseg;
-        product<E, BI / 2, true, true, false, BJ, false, TI / 2, TJ, NW>(dh, pb, a.nseg, 0, sb, smem, wave, lane, wi, wj);
+        const int sb = (a.Kb + BK - 1) / BK;
+        product<E, NP, BK, TILES, BI / 2, true, true, false, BJ, false, TI / 2, TJ, NW>(dh, pb, 0, sb, smem, wave, lane, wi, wj);
       }
     }
 #pragma unroll
@@ -372,7 +452,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void ffn_gemm_kernel(GemmArgs a) {
         for (int e = 0; e < 8; ++e) {
           const float gv = acc[2 * b + (e >> 2)][v][e & 3], uv = acc[TI / 32 + 2 * b + (e >> 2)][v][e & 3];
           float val, slope;
-          activate(a.act, gv, val, slope);
+          activate<!std::is_same<T, F32>::value>(a.act, gv, val, slope);
           h[e] = val * uv;
           if constexpr (KIND == GEMM_GATED_BWD) {
             float d = dh[2 * b + (e >> 2)][v][e & 3];
@@ -397,21 +477,22 @@ __global__ __launch_bounds__(64 * WI * WJ) void ffn_gemm_kernel(GemmArgs a) {
     }
   } else if constexpr (KIND == GEMM_NT || KIND == GEMM_NN) {
     constexpr bool kKm = KIND == GEMM_NN;  // NN: P's rows are contiguous in i
+    constexpr bool kPair = !kKm && TI % 32 == 0;  // eight consecutive results a lane instead of four
     Pair pr{kKm ? a.P + i0 : a.P + (long long)i0 * a.ldp, nullptr, a.Q + (long long)j0 * a.ldq, a.plane_p, a.plane_q, a.ldp, a.ldq,
             kKm ? ip - i0 : a.I - i0, a.J - j0, a.K, a.kp};
-    const int steps = (a.K + kBK - 1) / kBK * a.nseg;
-    product<E, BI, kKm, !kKm, false, BJ, false, TI, TJ, NW>(acc, pr, a.nseg, 0, steps, smem, wave, lane, wi, wj);
+    const int steps = (a.K + BK - 1) / BK;
+    product<E, NP, BK, TILES, BI, kKm, kPair, false, BJ, false, TI, TJ, NW>(acc, pr, 0, steps, smem, wave, lane, wi, wj);
     if (kKm && a.Pb != nullptr) {  // dX = dG Wg + dU Wu
       pr.P = a.Pb + i0;
       pr.Q = a.Qb + (long long)j0 * a.ldq;
-      product<E, BI, kKm, !kKm, false, BJ, false, TI, TJ, NW>(acc, pr, a.nseg, 0, steps, smem, wave, lane, wi, wj);
+      product<E, NP, BK, TILES, BI, kKm, kPair, false, BJ, false, TI, TJ, NW>(acc, pr, 0, steps, smem, wave, lane, wi, wj);
     }
     auto *D = static_cast<typename T::storage *>(a.D);
 #pragma unroll
     for (int v = 0; v < TJ / 16; ++v) {
       const int j = j0 + wj * TJ + v * 16 + (lane & 15);
       if (j >= a.J) continue;
-      if constexpr (!kKm) {
+      if constexpr (kPair) {
 #pragma unroll
         for (int b = 0; b < TI / 32; ++b) {
           const int c0 = i0 + wi * TI + b * 32 + 8 * g;
@@ -435,10 +516,10 @@ __global__ __launch_bounds__(64 * WI * WJ) void ffn_gemm_kernel(GemmArgs a) {
     const int z = blockIdx.z, jp = (a.J + 7) & ~7;
     Pair pr{a.P + i0, nullptr, a.Q + (long long)z * a.batch_q + j0, a.plane_p, a.plane_q, a.ldp, a.ldq, ip - i0, jp - j0, a.K,
             a.K};
-    const long long steps = (long long)((a.K + kBK - 1) / kBK) * a.nseg;
+    const long long steps = (a.K + BK - 1) / BK;
     const int s0 = __builtin_amdgcn_readfirstlane((int)(steps * slice / a.slices));
     const int s1 = __builtin_amdgcn_readfirstlane((int)(steps * (slice + 1) / a.slices));
-    product<E, BI, true, false, false, BJ, true, TI, TJ, NW>(acc, pr, a.nseg, s0, s1, smem, wave, lane, wi, wj);
+    product<E, NP, BK, TILES, BI, true, false, false, BJ, true, TI, TJ, NW>(acc, pr, s0, s1, smem, wave, lane, wi, wj);
     float *D = static_cast<float *>(a.D) + ((long long)z * a.slices + slice) * a.J * a.I;
 #pragma unroll
     for (int v = 0; v < TJ / 16; ++v) {
@@ -469,7 +550,7 @@ __global__ __launch_bounds__(256) void ffn_slices_kernel(const float *__restrict
 
 // ---- operands that are not what the products read: another memory order, odd rows, f32 ---------------------------------
 // source element (b, r, c) at src + b sb + r sr + c sc, one of sr, sc being 1; out rows [(b, r)] of ld elements, zero behind C.
-// `planes` 4: the split of an f32 value; 1: one rounding to E (none when S is E).
+// `planes` 3: the split of an f32 value; 1: one rounding to E (none when S is E).
 template <typename S, typename E>
 __global__ __launch_bounds__(256) void ffn_pack_kernel(const typename S::storage *__restrict__ src, long long sb, long long sr,
                                                        long long sc, int Rb, int C, u16 *__restrict__ dst, int ld, long long plane,
@@ -489,6 +570,106 @@ __global__ __launch_bounds__(256) void ffn_pack_kernel(const typename S::storage
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = tile[r][c + e];
   put_internal<E, 8>(dst + ((long long)b * Rb + r0 + r) * ld + c0 + c, plane, planes, v);
+}
+
+// ---- few points: the weights are read once, straight into fragments -------------------------------------------------------
+// A workgroup of eight waves owns 16 results i (GATED: of both projections) for up to JT x 16 points; its waves take pieces of k in
+// turn and their accumulators are joined in LDS, in wave order.  No operand passes through LDS (each weight is used by one wave
+// only), U pieces of every matrix are in flight per wave, the tensors are read as they are: no packed copies, f32 by the f32 MFMA.
+// Bound: the read of the weights.  VEC: rows start on 16 bytes (K a multiple of a piece); else element by element.
+template <typename T, bool VEC> struct Piece {
+  typename T::storage v[T::kVec];
+  __device__ __forceinline__ void load(const typename T::storage *row, int k, int K) {
+    if (VEC) {
+      if (k < K) *reinterpret_cast<Vec16<T> *>(v) = *reinterpret_cast<const Vec16<T> *>(row + k);
+      else *reinterpret_cast<Vec16<T> *>(v) = Vec16<T>{};
+    } else {
+#pragma unroll
+      for (int e = 0; e < T::kVec; ++e) v[e] = k + e < K ? row[k + e] : typename T::storage(0);
+    }
+  }
+} __attribute__((aligned(16)));
+template <typename T, bool VEC> __device__ __forceinline__ f32x4 mul_piece(const Piece<T, VEC> &p, const Piece<T, VEC> &q, f32x4 c) {
+  if constexpr (std::is_same<T, F32>::value) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(p.v[e], q.v[e], c, 0, 0, 0);
+    return c;
+  } else {
+    return mfma16<T>(*reinterpret_cast<const s16x8 *>(p.v), *reinterpret_cast<const s16x8 *>(q.v), c);
+  }
+}
+
+struct RowsArgs {
+  const void *P, *P2, *Q;
+  void *D;
+  int I, J, K, ldp, ldq, ldd, act, vec_out;
+};
+
+constexpr int kRowsWaves = 8, kRowsMost = 64;  // points of a call that goes this way, at most
+
+template <bool GATED, typename T, int JT, bool VEC>
+__global__ __launch_bounds__(64 * kRowsWaves) void ffn_rows_kernel(RowsArgs a) {
+  using S = typename T::storage;
+  constexpr int M = GATED ? 2 : 1, U = JT == 1 ? 8 : 4, V = T::kVec;
+  __shared__ f32x4 s_acc[kRowsWaves][M][JT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+  const int i0 = blockIdx.x * 16;
+  const long long i = i0 + (lane & 15) < a.I ? i0 + (lane & 15) : a.I - 1;  // (a row behind the end: read, not stored)
+  const S *P = static_cast<const S *>(a.P) + i * a.ldp, *P2 = GATED ? static_cast<const S *>(a.P2) + i * a.ldp : nullptr;
+  const S *Q[JT];
+  f32x4 acc[M][JT];
+#pragma unroll
+  for (int t = 0; t < JT; ++t) {
+    const int j = t * 16 + (lane & 15);
+    Q[t] = static_cast<const S *>(a.Q) + (long long)(j < a.J ? j : a.J - 1) * a.ldq;
+#pragma unroll
+    for (int m = 0; m < M; ++m) acc[m][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+  for (int k0 = wave * U * 4 * V; k0 < a.K; k0 += kRowsWaves * U * 4 * V) {
+    Piece<T, VEC> p[U], p2[GATED ? U : 1], q[JT][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + (u * 4 + g) * V;
+      p[u].load(P, k, a.K);
+      if (GATED) p2[u].load(P2, k, a.K);
+#pragma unroll
+      for (int t = 0; t < JT; ++t) q[t][u].load(Q[t], k, a.K);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < JT; ++t) {
+        acc[0][t] = mul_piece<T, VEC>(p[u], q[t][u], acc[0][t]);
+        if (GATED) acc[M - 1][t] = mul_piece<T, VEC>(p2[u], q[t][u], acc[M - 1][t]);
+      }
+  }
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int t = 0; t < JT; ++t) s_acc[wave][m][t][lane] = acc[m][t];
+  __syncthreads();
+  if (threadIdx.x >= JT * 64) return;
+  const int t = threadIdx.x >> 6;  // (a wave per 16 points)
+  f32x4 sum[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    sum[m] = s_acc[0][m][t][lane];
+#pragma unroll
+    for (int w = 1; w < kRowsWaves; ++w) sum[m] += s_acc[w][m][t][lane];
+  }
+  const int j = t * 16 + (lane & 15), c0 = i0 + 4 * g;
+  if (j >= a.J || c0 >= a.I) return;
+  float o[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    o[e] = sum[0][e];
+    if (GATED) {
+      float slope;
+      activate<!std::is_same<T, F32>::value>(a.act, sum[0][e], o[e], slope);
+      o[e] *= sum[M - 1][e];
+    }
+  }
+  put_row<T, 4>(static_cast<S *>(a.D) + (long long)j * a.ldd + c0, a.I - c0, a.vec_out, o);
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------
@@ -532,7 +713,7 @@ static Operand operand(Arena &ar, const FfnShape &s, const void *src, bool chann
   const int ld = (C + 7) & ~7;
   if (!s.convert() && !channel && C % 8 == 0) return {static_cast<const u16 *>(src), C, 0};
   const long long plane = (long long)B * Rb * ld;
-  const int planes = s.split ? 4 : 1;
+  const int planes = s.split ? 3 : 1;
   u16 *dst = static_cast<u16 *>(ar.take((size_t)plane * planes * 2));
   if (launch) {
     // rows that follow each other without regard to the cloud are one batch
@@ -551,11 +732,11 @@ static int transposed(int dtype, const void *src, int B, int R, int C, void *dst
   return cl3d_transpose16(src, B, R, C, dst, st);
 }
 
-template <int KIND, typename E, typename T, int BI, int BJ, int WI, int WJ>
+template <int KIND, typename E, typename T, int NP, int BI, int BJ, int WI, int WJ, int BK, int TILES>
 static int gemm_as(const GemmArgs &a, int batches, hipStream_t st) {
   constexpr int kCh = KIND == GEMM_GATED || KIND == GEMM_GATED_BWD ? BI / 2 : BI;
-  constexpr int kLds = 2 * (BI + BJ) * kRowBytes;
-  const auto kernel = ffn_gemm_kernel<KIND, E, T, BI, BJ, WI, WJ>;
+  constexpr int kLds = TILES * NP * (BI + BJ) * BK * 2;
+  const auto kernel = ffn_gemm_kernel<KIND, E, T, NP, BI, BJ, WI, WJ, BK, TILES>;
   static std::atomic<unsigned long long> granted{0};
   if (kLds > 65536) {
     const int rc = lds_opt_in(granted, reinterpret_cast<const void *>(kernel), kLds, "gated_ffn");
@@ -566,20 +747,44 @@ static int gemm_as(const GemmArgs &a, int batches, hipStream_t st) {
   return CL3D_OK;
 }
 
+// The tile of a product.  Measured at 16 384 x 288 x 1152 in bf16 and 16 384 x 144 x 576 in f32 (us):
+//   * dX and Y: rows of tiles of 96 results where they pad the width less than 128 do (widths 144, 288, 576 fit 96), 64 points a
+//     tile, so that three workgroups share a CU and 768 of them come out even: dX 34 (96 x 128: 39, 128 x 128: 42), Y 22 (23, 24);
+//     split: 96 x 128 by eight waves 62, 27 (128 x 128: 67, 30);
+//   * projections, forward and backward: 64 channels of both x 128 points by eight waves, 43 and 73 (four waves: 50, 86); split:
+//     64 points by four waves, two workgroups a CU: 70, 119 (128 points: 72, 131);
+//   * weight gradients: 128 x 128 by eight waves, 34 (four: 39).
+// Two tiles of k in LDS: a third one costs a workgroup of the CU (dX 44 -> 64).
+template <int KIND, typename E, typename T, int NP> static int gemm_tile(const GemmArgs &a, int batches, hipStream_t st) {
+  const bool by96 = ceil_div(a.I, 96) * 96 < ceil_div(a.I, 128) * 128;
+  if constexpr (KIND == GEMM_NT || KIND == GEMM_NN) {
+    if constexpr (NP == 3) return by96 ? gemm_as<KIND, E, T, 3, 96, 128, 2, 4, 32, 2>(a, batches, st) : gemm_as<KIND, E, T, 3, 128, 128, 2, 4, 32, 2>(a, batches, st);
+    else return by96 ? gemm_as<KIND, E, T, 1, 96, 64, 2, 2, 64, 2>(a, batches, st) : gemm_as<KIND, E, T, 1, 128, 64, 2, 2, 64, 2>(a, batches, st);
+  } else if constexpr (KIND == GEMM_TN) {
+    return gemm_as<KIND, E, T, NP, 128, 128, 2, 4, NP == 1 ? 64 : 32, 2>(a, batches, st);
+  } else {
+    if constexpr (NP == 3) return gemm_as<KIND, E, T, 3, 128, 64, 2, 2, 32, 2>(a, batches, st);
+    else return gemm_as<KIND, E, T, 1, 128, 128, 2, 4, 64, 2>(a, batches, st);
+  }
+}
+
 template <int KIND> static int gemm(const FfnShape &s, const GemmArgs &a, int batches, hipStream_t st) {
   if (a.I <= 0 || a.J <= 0) return CL3D_OK;
-  if (s.dtype == CL3D_F32) return gemm_as<KIND, Bf16, F32, 128, 128, 2, 2>(a, batches, st);
-  if (s.dtype == CL3D_BF16) return gemm_as<KIND, Bf16, Bf16, 128, 128, 2, 2>(a, batches, st);
-  return gemm_as<KIND, F16, F16, 128, 128, 2, 2>(a, batches, st);
+  if (s.split) return gemm_tile<KIND, Bf16, F32, 3>(a, batches, st);
+  if (s.dtype == CL3D_F32) return gemm_tile<KIND, Bf16, F32, 1>(a, batches, st);
+  if (s.dtype == CL3D_BF16) return gemm_tile<KIND, Bf16, Bf16, 1>(a, batches, st);
+  return gemm_tile<KIND, F16, F16, 1>(a, batches, st);
 }
 
 static bool row_vec(const FfnShape &s, const void *D, int ldd) { return aligned16(D) && ldd % (s.dtype == CL3D_F32 ? 4 : 8) == 0; }
 
-// pieces of k in a weight gradient: enough workgroups for two on every CU, four tiles of k in each at least
+// pieces of k in a weight gradient: as many workgroups as the chip holds at once (two on a CU, split products one), not one more
+// -- a few workgroups of a second round would take as long as the whole first one (540 on 512 places: 49 us, 486: 30) --, four
+// tiles of k in each at least
 static int weight_slices(const FfnShape &s, int I, int J, int batches) {
   const long long tiles = (long long)ceil_div(I, 128) * ceil_div(J, 128) * batches;
-  const long long steps = (s.R() + kBK - 1) / kBK * (s.split ? 6 : 1);
-  long long n = (512 + tiles - 1) / tiles;
+  const long long steps = (s.R() + 63) / 64;
+  long long n = (s.split ? 256 : 512) / tiles;
   if (n > steps / 4) n = steps / 4;
   return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
 }
@@ -598,23 +803,58 @@ static int slices_sum(const FfnShape &s, const float *src, long long n, int slic
 
 static GemmArgs gemm_args(const FfnShape &s) {
   GemmArgs a{};
-  a.nseg = s.split ? 6 : 1;
-  a.planes = s.split ? 4 : 1;
+  a.planes = s.split ? 3 : 1;
   a.act = s.act;
   a.slices = 1;
   return a;
+}
+
+template <bool GATED, typename T> static void rows_launch(const RowsArgs &a, hipStream_t st) {
+  const bool vec = a.ldp % T::kVec == 0 && a.ldq % T::kVec == 0 && a.K % T::kVec == 0;
+  const dim3 grid(ceil_div(a.I, 16)), block(64 * kRowsWaves);
+#define CL3D_ROWS(JT) \
+  do { \
+    if (vec) hipLaunchKernelGGL((ffn_rows_kernel<GATED, T, JT, true>), grid, block, 0, st, a); \
+    else hipLaunchKernelGGL((ffn_rows_kernel<GATED, T, JT, false>), grid, block, 0, st, a); \
+  } while (0)
+  if (a.J <= 16) CL3D_ROWS(1);
+  else if (a.J <= 32) CL3D_ROWS(2);
+  else CL3D_ROWS(4);
+#undef CL3D_ROWS
+}
+template <bool GATED> static void rows(int dtype, const RowsArgs &a, hipStream_t st) {
+  if (dtype == CL3D_F32) rows_launch<GATED, F32>(a, st);
+  else if (dtype == CL3D_BF16) rows_launch<GATED, Bf16>(a, st);
+  else rows_launch<GATED, F16>(a, st);
+}
+
+// x and y as point-major rows, at most kRowsMost of them
+static void ffn_forward_rows(const FfnShape &s, const void *x, const void *wg, const void *wu, const void *wd, void *y, void *h, hipStream_t st) {
+  const int R = (int)s.R(), hp = (s.H + 7) & ~7, quad = s.dtype == CL3D_F32 ? 4 : 8;
+  rows<true>(s.dtype, {wg, wu, x, s.down ? h : y, s.H, R, s.C, s.C, s.C, s.down ? hp : s.H, s.act, s.down || s.H % quad == 0}, st);
+  if (s.down) rows<false>(s.dtype, {wd, nullptr, h, y, s.C, R, s.H, s.H, hp, s.C, s.act, s.C % quad == 0}, st);
 }
 
 // x in the layout of `s`, its rows of C
 static int ffn_forward(const FfnShape &s, const void *x, const void *wg, const void *wu, const void *wd, void *y, Arena &ar, bool launch,
                        hipStream_t st) {
   const int R = (int)s.R(), hp = (s.H + 7) & ~7, out = s.down ? s.C : s.H;
+  if (R <= kRowsMost && (s.split || !s.convert())) {
+    const size_t e = elem_bytes(s.dtype);
+    void *h = s.down ? ar.take((size_t)R * hp * e) : nullptr, *xr = s.channel() ? ar.take((size_t)R * s.C * e) : nullptr;
+    void *yr = s.channel() ? ar.take((size_t)R * out * e) : y;
+    if (!launch) return CL3D_OK;
+    int rc = s.channel() ? transposed(s.dtype, x, s.B, s.C, s.N, xr, st) : CL3D_OK;
+    if (rc != CL3D_OK) return rc;
+    ffn_forward_rows(s, s.channel() ? xr : x, wg, wu, wd, yr, h, st);
+    return s.channel() ? transposed(s.dtype, yr, s.B, s.N, out, y, st) : CL3D_OK;
+  }
   const Operand X = operand(ar, s, x, s.channel(), s.B, s.N, s.C, launch, st);
   const Operand G = operand(ar, s, wg, false, 1, s.H, s.C, launch, st), U = operand(ar, s, wu, false, 1, s.H, s.C, launch, st);
   Operand D, h;
   if (s.down) {
     D = operand(ar, s, wd, false, 1, s.C, s.H, launch, st);
-    h = {static_cast<u16 *>(ar.take((size_t)R * hp * 2 * (s.split ? 4 : 1))), hp, (long long)R * hp};
+    h = {static_cast<u16 *>(ar.take((size_t)R * hp * 2 * (s.split ? 3 : 1))), hp, (long long)R * hp};
   }
   void *rows = s.channel() ? ar.take((size_t)R * out * elem_bytes(s.dtype)) : y;
   if (!launch) return CL3D_OK;
@@ -645,7 +885,7 @@ static int ffn_forward(const FfnShape &s, const void *x, const void *wg, const v
 
 static int ffn_backward(const FfnShape &s, const void *x, const void *wg, const void *wu, const void *wd, const void *dy, void *dx,
                         void *dwg, void *dwu, void *dwd, unsigned wants, Arena &ar, bool launch, hipStream_t st) {
-  const int R = (int)s.R(), hp = (s.H + 7) & ~7, planes = s.split ? 4 : 1;
+  const int R = (int)s.R(), hp = (s.H + 7) & ~7, planes = s.split ? 3 : 1;
   const bool want_x = wants & CL3D_FFN_DX, want_gu = wants & CL3D_FFN_DW_IN, want_d = s.down && (wants & CL3D_FFN_DW_DOWN);
   const Operand X = operand(ar, s, x, s.channel(), s.B, s.N, s.C, launch, st);
   const Operand G = operand(ar, s, wg, false, 1, s.H, s.C, launch, st), U = operand(ar, s, wu, false, 1, s.H, s.C, launch, st);
