@@ -25,7 +25,7 @@ class NormResidual(ctypes.Structure):
     _fields_ = (
         [(n, _I) for n in ("B", "N", "C", "dtype", "param_f32", "kind", "next_kind", "gate_cloud")]
         + [(n, _F) for n in ("residual_scale", "eps", "next_eps")]
-        + [("reserved", _I), ("p", ctypes.c_double)]
+        + [("order", _I), ("p", ctypes.c_double)]
         + [(n, _P) for n in ("rng", "x", "y", "weight", "bias", "gate", "next_weight", "next_bias", "out", "next", "stats",
                              "dout", "dnext", "dx", "dy", "dweight", "dbias", "dgate", "dnext_weight", "dnext_bias", "ws")]
         + [("ws_bytes", _Z)])
@@ -87,8 +87,8 @@ SIGNATURES = {
     "cl3d_gemm_autotune": [_I],
     "cl3d_gemm_autotune_stats": [_P, _P],
     "cl3d_sgd_step": [_P, _P, _P, ctypes.c_longlong, _F, _F, _F, _F, _I, _I, _I, _P],
-    "cl3d_gated_ffn_fwd": [_P] * 4 + [_I] * 8 + [_P, _P, _Z, _P],
-    "cl3d_gated_ffn_bwd": [_P] * 5 + [_I] * 8 + [_P] * 5 + [_Z, _P],
+    "cl3d_gated_ffn_fwd": [_P] * 4 + [_I] * 8 + [_P, _P, _P, _Z, _P],
+    "cl3d_gated_ffn_bwd": [_P] * 6 + [_I] * 8 + [_P] * 5 + [_Z, _P],
     "cl3d_transpose16": [_P, _I, _I, _I, _P, _P],
     "cl3d_norm_residual_fwd": [ctypes.POINTER(NormResidual), _P],
     "cl3d_norm_residual_bwd": [ctypes.POINTER(NormResidual), _P],

@@ -4,7 +4,7 @@
 
 namespace cl3d {
 size_t gated_ffn_workspace(int B, int N, int H, int flags, int C);  // gated_ffn.hip
-size_t point_norm_workspace(int B, int N, int C);                   // point_norm.hip
+size_t point_norm_workspace(int B, int N, int C, int flags);        // point_norm.hip
 }  // namespace cl3d
 
 extern "C" int cl3d_abi_version(void) { return CL3D_ABI_VERSION; }
@@ -42,8 +42,8 @@ extern "C" size_t cl3d_workspace_bytes(int op, int B, int N, int M, int K, int C
       return cl3d::gemm_family_workspace(B, N, M, C, false);
     case CL3D_OP_GATED_FFN:  // packed operands, hidden activations, weight-gradient slices; M hidden channels, K flags
       return cl3d::gated_ffn_workspace(B, N, M, K, C);
-    case CL3D_OP_POINT_NORM:  // partial rows of the parameters' gradients
-      return cl3d::point_norm_workspace(B, N, C);
+    case CL3D_OP_POINT_NORM:  // copies of channel-major tensors, partial rows of the parameters' gradients; K flags
+      return cl3d::point_norm_workspace(B, N, C, K);
     default:  // every other op of ABI v1 keeps its scratch in LDS
       return 0;
   }

@@ -79,4 +79,23 @@ inline int make_drop(Drop &d, const void *state, double p, const char *who) {
   return CL3D_OK;
 }
 
+// scratch of a call, handed out in order; without a base it only counts
+struct Arena {
+  char *base;
+  size_t used = 0;
+  explicit Arena(void *p) : base(static_cast<char *>(p)) {}
+  void *take(size_t bytes) {
+    used = (used + 255) & ~(size_t)255;
+    char *p = base ? base + used : nullptr;
+    used += bytes;
+    return p;
+  }
+};
+
+// [b][R][C] -> [b][C][R] of the tensor type
+inline int transposed(int dtype, const void *src, int B, int R, int C, void *dst, hipStream_t st) {
+  if (dtype == CL3D_F32) return cl3d_transpose(static_cast<const float *>(src), B, R, C, static_cast<float *>(dst), st);
+  return cl3d_transpose16(src, B, R, C, dst, st);
+}
+
 }  // namespace cl3d

@@ -5,7 +5,7 @@
 //     dh = dY Wd;  dG = dh U act'(G);  dU = dh act(G);   dX = dG Wg + dU Wu;   dWg = dG^T X, dWu = dU^T X, dWd = dY^T h
 // Three products of 2 R C H operations forward and six backward.  G and U never reach memory: the forward kernel keeps both
 // accumulators of an element in one lane and writes h, the backward kernel forms G, U and dh together (two products more) and
-// writes h, dG, dU.  Against storing G and U that is 8 R H bytes less traffic for 4 R C H operations more -- at 5.1 TB/s and
+// writes dG, dU (h is kept from the forward pass where the caller has room for it, or formed again).  Against storing G and U that is 8 R H bytes less traffic for 4 R C H operations more -- at 5.1 TB/s and
 // 1.28 PFLOP/s (a large copy, a large product) it pays below C = 500 -- and dG, dU come from f32 values of G, U, dh: one
 // rounding in front of the last products instead of two.
 //
@@ -537,14 +537,35 @@ __global__ __launch_bounds__(64 * WI * WJ) void ffn_gemm_kernel(GemmArgs a) {
   }
 }
 
-// dst[e] = sum over slices of src[slice][e], in slice order
-template <typename T>
-__global__ __launch_bounds__(256) void ffn_slices_kernel(const float *__restrict__ src, long long n, int slices,
-                                                         typename T::storage *__restrict__ dst) {
-  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long long)gridDim.x * 256) {
-    float s = 0.f;
-    for (int z = 0; z < slices; ++z) s += src[(long long)z * n + e];
-    dst[e] = T::put(s);
+// dst[e] = sum over slices of src[slice][e], in slice order, for up to three weight gradients (blockIdx.y); V elements a lane
+struct SliceSums {
+  const float *src[3];
+  void *dst[3];
+  long long n[3];
+  int slices[3];
+};
+template <typename T, int V> __global__ __launch_bounds__(256) void ffn_slices_kernel(SliceSums a) {
+  const int w = blockIdx.y, slices = a.slices[w];
+  const long long n = a.n[w], stride = (long long)gridDim.x * 256 * V;
+  const float *src = a.src[w];
+  auto *dst = static_cast<typename T::storage *>(a.dst[w]);
+  if (dst == nullptr) return;
+  for (long long e = ((long long)blockIdx.x * 256 + threadIdx.x) * V; e < n; e += stride) {
+    float s[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] = 0.f;
+#pragma unroll 4
+    for (int z = 0; z < slices; ++z) {
+      if constexpr (V == 4) {
+        const f32x4 t = *reinterpret_cast<const f32x4 *>(src + (long long)z * n + e);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s[v] += t[v];
+      } else {
+        s[0] += src[(long long)z * n + e];
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) dst[e + v] = T::put(s[v]);
   }
 }
 
@@ -605,7 +626,7 @@ struct RowsArgs {
   int I, J, K, ldp, ldq, ldd, act, vec_out;
 };
 
-constexpr int kRowsWaves = 8, kRowsMost = 64;  // points of a call that goes this way, at most
+constexpr int kRowsWaves = 8, kRowsMost = CL3D_FFN_FEW;  // points of a call that goes this way, at most
 
 template <bool GATED, typename T, int JT, bool VEC>
 __global__ __launch_bounds__(64 * kRowsWaves) void ffn_rows_kernel(RowsArgs a) {
@@ -673,19 +694,6 @@ __global__ __launch_bounds__(64 * kRowsWaves) void ffn_rows_kernel(RowsArgs a) {
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------
-// scratch in order; without a base it only counts
-struct Arena {
-  char *base;
-  size_t used = 0;
-  explicit Arena(void *p) : base(static_cast<char *>(p)) {}
-  void *take(size_t bytes) {
-    used = (used + 255) & ~(size_t)255;
-    char *p = base ? base + used : nullptr;
-    used += bytes;
-    return p;
-  }
-};
-
 struct Operand {
   const u16 *p = nullptr;
   int ld = 0;
@@ -724,12 +732,6 @@ static Operand operand(Arena &ar, const FfnShape &s, const void *src, bool chann
     else pack_launch<F16, F16>(src, sb, sr, sc, b, rb, C, dst, ld, plane, planes, st);
   }
   return {dst, ld, plane};
-}
-
-// [b][R][C] -> [b][C][R] of the tensor type
-static int transposed(int dtype, const void *src, int B, int R, int C, void *dst, hipStream_t st) {
-  if (dtype == CL3D_F32) return cl3d_transpose(static_cast<const float *>(src), B, R, C, static_cast<float *>(dst), st);
-  return cl3d_transpose16(src, B, R, C, dst, st);
 }
 
 template <int KIND, typename E, typename T, int NP, int BI, int BJ, int WI, int WJ, int BK, int TILES>
@@ -789,16 +791,17 @@ static int weight_slices(const FfnShape &s, int I, int J, int batches) {
   return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
 }
 
-static int slices_sum(const FfnShape &s, const float *src, long long n, int slices, void *dst, hipStream_t st) {
-  long long grid = (n + 255) / 256;
-  if (grid > 2048) grid = 2048;
-  if (s.dtype == CL3D_F32)
-    hipLaunchKernelGGL(ffn_slices_kernel<F32>, dim3((unsigned)grid), dim3(256), 0, st, src, n, slices, static_cast<float *>(dst));
-  else if (s.dtype == CL3D_BF16)
-    hipLaunchKernelGGL(ffn_slices_kernel<Bf16>, dim3((unsigned)grid), dim3(256), 0, st, src, n, slices, static_cast<u16 *>(dst));
-  else
-    hipLaunchKernelGGL(ffn_slices_kernel<F16>, dim3((unsigned)grid), dim3(256), 0, st, src, n, slices, static_cast<u16 *>(dst));
-  return CL3D_OK;
+template <typename T> static void slices_sum(const SliceSums &a, hipStream_t st) {
+  long long most = 0;
+  bool quads = true;
+  for (int w = 0; w < 3; ++w) {
+    most = a.n[w] > most ? a.n[w] : most;
+    quads = quads && a.n[w] % 4 == 0;
+  }
+  const long long lanes = quads ? most / 4 : most;
+  const dim3 grid((unsigned)(lanes < 256 * 1024 ? (lanes + 255) / 256 : 1024), 3);
+  if (quads) hipLaunchKernelGGL((ffn_slices_kernel<T, 4>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((ffn_slices_kernel<T, 1>), grid, dim3(256), 0, st, a);
 }
 
 static GemmArgs gemm_args(const FfnShape &s) {
@@ -836,8 +839,8 @@ static void ffn_forward_rows(const FfnShape &s, const void *x, const void *wg, c
 }
 
 // x in the layout of `s`, its rows of C
-static int ffn_forward(const FfnShape &s, const void *x, const void *wg, const void *wu, const void *wd, void *y, Arena &ar, bool launch,
-                       hipStream_t st) {
+static int ffn_forward(const FfnShape &s, const void *x, const void *wg, const void *wu, const void *wd, void *y, void *hidden, Arena &ar,
+                       bool launch, hipStream_t st) {
   const int R = (int)s.R(), hp = (s.H + 7) & ~7, out = s.down ? s.C : s.H;
   if (R <= kRowsMost && (s.split || !s.convert())) {
     const size_t e = elem_bytes(s.dtype);
@@ -854,7 +857,7 @@ static int ffn_forward(const FfnShape &s, const void *x, const void *wg, const v
   Operand D, h;
   if (s.down) {
     D = operand(ar, s, wd, false, 1, s.C, s.H, launch, st);
-    h = {static_cast<u16 *>(ar.take((size_t)R * hp * 2 * (s.split ? 3 : 1))), hp, (long long)R * hp};
+    h = {static_cast<u16 *>(hidden ? hidden : ar.take((size_t)R * hp * 2 * (s.split ? 3 : 1))), hp, (long long)R * hp};
   }
   void *rows = s.channel() ? ar.take((size_t)R * out * elem_bytes(s.dtype)) : y;
   if (!launch) return CL3D_OK;
@@ -883,8 +886,8 @@ static int ffn_forward(const FfnShape &s, const void *x, const void *wg, const v
   return s.channel() ? transposed(s.dtype, rows, s.B, s.N, out, y, st) : CL3D_OK;
 }
 
-static int ffn_backward(const FfnShape &s, const void *x, const void *wg, const void *wu, const void *wd, const void *dy, void *dx,
-                        void *dwg, void *dwu, void *dwd, unsigned wants, Arena &ar, bool launch, hipStream_t st) {
+static int ffn_backward(const FfnShape &s, const void *x, const void *wg, const void *wu, const void *wd, const void *dy,
+                        const void *hidden, void *dx, void *dwg, void *dwu, void *dwd, unsigned wants, Arena &ar, bool launch, hipStream_t st) {
   const int R = (int)s.R(), hp = (s.H + 7) & ~7, planes = s.split ? 3 : 1;
   const bool want_x = wants & CL3D_FFN_DX, want_gu = wants & CL3D_FFN_DW_IN, want_d = s.down && (wants & CL3D_FFN_DW_DOWN);
   const Operand X = operand(ar, s, x, s.channel(), s.B, s.N, s.C, launch, st);
@@ -894,7 +897,7 @@ static int ffn_backward(const FfnShape &s, const void *x, const void *wg, const 
   if (s.down) {
     D = operand(ar, s, wd, false, 1, s.C, s.H, launch, st);
     dY = operand(ar, s, dy, s.channel(), s.B, s.N, s.C, launch, st);
-    if (want_d) h = {static_cast<u16 *>(ar.take((size_t)R * hp * 2 * planes)), hp, (long long)R * hp};
+    if (want_d) h = {static_cast<const u16 *>(hidden ? hidden : ar.take((size_t)R * hp * 2 * planes)), hp, (long long)R * hp};
   } else if (s.channel()) {
     void *t = ar.take((size_t)R * s.H * elem_bytes(s.dtype));
     if (launch) {
@@ -921,7 +924,7 @@ static int ffn_backward(const FfnShape &s, const void *x, const void *wg, const 
     a.plane_pb = D.plane; a.plane_qb = dY.plane;
     a.ldpb = D.ld; a.ldqb = dY.ld;
     a.Kb = dY.ld; a.kp = s.C;
-    a.h = const_cast<u16 *>(h.p); a.plane_h = h.plane;
+    if (!hidden) { a.h = const_cast<u16 *>(h.p); a.plane_h = h.plane; }
   } else {
     a.dh = dh_rows; a.lddh = s.H;
   }
@@ -950,9 +953,6 @@ static int ffn_backward(const FfnShape &s, const void *x, const void *wg, const 
     a.D = part_in; a.vec = s.C % 4 == 0;
     rc = gemm<GEMM_TN>(s, a, 2, st);
     if (rc != CL3D_OK) return rc;
-    const long long n = (long long)s.H * s.C;
-    if (dwg) slices_sum(s, part_in, n, slices_in, dwg, st);
-    if (dwu) slices_sum(s, part_in + n * slices_in, n, slices_in, dwu, st);
   }
   if (want_d) {
     a = gemm_args(s);
@@ -964,7 +964,13 @@ static int ffn_backward(const FfnShape &s, const void *x, const void *wg, const 
     a.D = part_d; a.vec = s.H % 4 == 0;
     rc = gemm<GEMM_TN>(s, a, 1, st);
     if (rc != CL3D_OK) return rc;
-    slices_sum(s, part_d, (long long)s.H * s.C, slices_d, dwd, st);
+  }
+  if (want_gu || want_d) {
+    const long long n = (long long)s.H * s.C;
+    const SliceSums sums{{part_in, part_in + (want_gu ? n * slices_in : 0), part_d}, {dwg, dwu, dwd}, {n, n, n}, {slices_in, slices_in, slices_d}};
+    if (s.dtype == CL3D_F32) slices_sum<F32>(sums, st);
+    else if (s.dtype == CL3D_BF16) slices_sum<Bf16>(sums, st);
+    else slices_sum<F16>(sums, st);
   }
   return CL3D_OK;
 }
@@ -985,20 +991,23 @@ static int ffn_shape(FfnShape &s, int dtype, int order, int B, int N, int C, int
 }
 
 size_t gated_ffn_workspace(int B, int N, int H, int flags, int C) {
-  // flags: element type | order << 2 | precision << 3 | down << 4 | backward << 5 | wanted gradients << 6
+  // flags: element type | order << 2 | precision << 3 | down << 4 | backward << 5 | wanted gradients << 6 | hidden kept << 9
   FfnShape s;
   if (ffn_shape(s, flags & 3, (flags >> 2) & 1, B, N, C, H, CL3D_ACT_SILU, (flags >> 3) & 1, (flags >> 4) & 1, "gated_ffn") != CL3D_OK)
     return 0;
   Arena ar(nullptr);
-  if ((flags >> 5) & 1) ffn_backward(s, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, (unsigned)flags >> 6, ar, false, nullptr);
-  else ffn_forward(s, nullptr, nullptr, nullptr, nullptr, nullptr, ar, false, nullptr);
+  char kept;  // (only asked whether it is there)
+  void *hidden = (flags >> 9) & 1 ? &kept : nullptr;
+  if ((flags >> 5) & 1)
+    ffn_backward(s, nullptr, nullptr, nullptr, nullptr, nullptr, hidden, nullptr, nullptr, nullptr, nullptr, ((unsigned)flags >> 6) & 7u, ar, false, nullptr);
+  else ffn_forward(s, nullptr, nullptr, nullptr, nullptr, nullptr, hidden, ar, false, nullptr);
   return ar.used;
 }
 
 }  // namespace cl3d
 
 extern "C" int cl3d_gated_ffn_fwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, int dtype, int order, int B,
-                                  int C, int N, int H, int activation, int precision, void *y, void *ws, size_t ws_bytes,
+                                  int C, int N, int H, int activation, int precision, void *y, void *hidden, void *ws, size_t ws_bytes,
                                   cl3d_stream_t stream) {
   using namespace cl3d;
   FfnShape s;
@@ -1006,17 +1015,19 @@ extern "C" int cl3d_gated_ffn_fwd(const void *x, const void *w_gate, const void 
   if (rc != CL3D_OK) return rc;
   if (s.R() == 0) return CL3D_OK;
   CL3D_REQUIRE(x && w_gate && w_up && y, "gated_ffn_fwd: null pointer");
-  CL3D_REQUIRE(aligned16(x) && aligned16(w_gate) && aligned16(w_up) && aligned16(w_down) && aligned16(y) && aligned16(ws),
+  CL3D_REQUIRE(aligned16(x) && aligned16(w_gate) && aligned16(w_up) && aligned16(w_down) && aligned16(y) && aligned16(hidden) &&
+                   aligned16(ws),
                "gated_ffn_fwd: tensors start on 16 bytes");
+  CL3D_REQUIRE(!hidden || (w_down && s.R() > CL3D_FFN_FEW), "gated_ffn_fwd: no hidden activations are kept here");
   Arena need(nullptr), ar(ws);
-  ffn_forward(s, x, w_gate, w_up, w_down, y, need, false, nullptr);
+  ffn_forward(s, x, w_gate, w_up, w_down, y, hidden, need, false, nullptr);
   if (ws_bytes < need.used || (need.used && !ws)) return fail(CL3D_E_WORKSPACE, "gated_ffn_fwd: %zu bytes of scratch, %zu needed", ws_bytes, need.used);
-  rc = ffn_forward(s, x, w_gate, w_up, w_down, y, ar, true, (hipStream_t)stream);
+  rc = ffn_forward(s, x, w_gate, w_up, w_down, y, hidden, ar, true, (hipStream_t)stream);
   return rc != CL3D_OK ? rc : check_launch("cl3d_gated_ffn_fwd");
 }
 
-extern "C" int cl3d_gated_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *dy, int dtype,
-                                  int order, int B, int C, int N, int H, int activation, int precision, void *dx, void *dw_gate,
+extern "C" int cl3d_gated_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *dy,
+                                  const void *hidden, int dtype, int order, int B, int C, int N, int H, int activation, int precision, void *dx, void *dw_gate,
                                   void *dw_up, void *dw_down, void *ws, size_t ws_bytes, cl3d_stream_t stream) {
   using namespace cl3d;
   FfnShape s;
@@ -1025,14 +1036,14 @@ extern "C" int cl3d_gated_ffn_bwd(const void *x, const void *w_gate, const void 
   CL3D_REQUIRE(s.R() > 0, "gated_ffn_bwd: no points (their gradients are zeros: nothing to launch)");
   CL3D_REQUIRE(x && w_gate && w_up && dy, "gated_ffn_bwd: null pointer");
   CL3D_REQUIRE(w_down != nullptr || dw_down == nullptr, "gated_ffn_bwd: a gradient for a projection that is not there");
-  CL3D_REQUIRE(aligned16(x) && aligned16(w_gate) && aligned16(w_up) && aligned16(w_down) && aligned16(dy) && aligned16(dx) &&
+  CL3D_REQUIRE(aligned16(x) && aligned16(w_gate) && aligned16(w_up) && aligned16(w_down) && aligned16(dy) && aligned16(hidden) && aligned16(dx) &&
                    aligned16(dw_gate) && aligned16(dw_up) && aligned16(dw_down) && aligned16(ws),
                "gated_ffn_bwd: tensors start on 16 bytes");
   const unsigned wants = (dx ? CL3D_FFN_DX : 0u) | (dw_gate || dw_up ? CL3D_FFN_DW_IN : 0u) | (dw_down ? CL3D_FFN_DW_DOWN : 0u);
   if (wants == 0) return CL3D_OK;
   Arena need(nullptr), ar(ws);
-  ffn_backward(s, x, w_gate, w_up, w_down, dy, dx, dw_gate, dw_up, dw_down, wants, need, false, nullptr);
+  ffn_backward(s, x, w_gate, w_up, w_down, dy, hidden, dx, dw_gate, dw_up, dw_down, wants, need, false, nullptr);
   if (ws_bytes < need.used || (need.used && !ws)) return fail(CL3D_E_WORKSPACE, "gated_ffn_bwd: %zu bytes of scratch, %zu needed", ws_bytes, need.used);
-  rc = ffn_backward(s, x, w_gate, w_up, w_down, dy, dx, dw_gate, dw_up, dw_down, wants, ar, true, (hipStream_t)stream);
+  rc = ffn_backward(s, x, w_gate, w_up, w_down, dy, hidden, dx, dw_gate, dw_up, dw_down, wants, ar, true, (hipStream_t)stream);
   return rc != CL3D_OK ? rc : check_launch("cl3d_gated_ffn_bwd");
 }

@@ -11,6 +11,7 @@
 // goes to scratch and a second launch adds them in order (no atomics: bit-identical run to run).  A workgroup's rows are of one
 // cloud, so a gate per cloud is summed by the same partials.
 #include "ff_common.h"
+#include <type_traits>
 
 namespace cl3d {
 
@@ -33,13 +34,32 @@ template <typename T> __device__ __forceinline__ float param(const void *p, long
   return f32 ? static_cast<const float *>(p)[i] : T::get(static_cast<const typename T::storage *>(p)[i]);
 }
 
+// v + v of the lane that the DPP control names (within 16 lanes)
+template <int CTRL> __device__ __forceinline__ float add_dpp(float v) {
+  return v + __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+// the sum over 16, 32 or 64 lanes, in every one of them: neighbour, pair, half row and row by DPP, rows and halves of the wave by the
+// swaps of gfx950 (a shuffle through LDS costs a round trip a step, and a row takes up to eight sums)
+template <int LANES> __device__ __forceinline__ float lane_sum(float v) {
+  v = add_dpp<0xB1>(v);   // quad_perm [1, 0, 3, 2]
+  v = add_dpp<0x4E>(v);   // quad_perm [2, 3, 0, 1]
+  v = add_dpp<0x141>(v);  // row_half_mirror
+  v = add_dpp<0x140>(v);  // row_mirror
+  if (LANES > 16) {
+    auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    if (LANES > 32) {
+      s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+      v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+  }
+  return v;
+}
+
 // sums of two values over the TPR lanes of a row
 template <int TPR> __device__ __forceinline__ void row_sum(float &a, float &b, float *s_red) {
-#pragma unroll
-  for (int off = (TPR < 64 ? TPR : 64) / 2; off >= 1; off >>= 1) {
-    a += __shfl_xor(a, off, 64);
-    b += __shfl_xor(b, off, 64);
-  }
+  a = lane_sum<(TPR < 64 ? TPR : 64)>(a);
+  b = lane_sum<(TPR < 64 ? TPR : 64)>(b);
   if (TPR > 64) {  // the whole workgroup is one row
     const int wave = threadIdx.x >> 6;
     __syncthreads();
@@ -51,17 +71,7 @@ template <int TPR> __device__ __forceinline__ void row_sum(float &a, float &b, f
   }
 }
 
-// V consecutive elements at p (VEC: 16 bytes, else one)
-template <typename T, int V> __device__ __forceinline__ void load_v(const void *base, long long at, float *v) {
-  const auto *p = static_cast<const typename T::storage *>(base) + at;
-  if constexpr (V == 1) {
-    v[0] = T::get(*p);
-  } else {
-    const Vec16<T> q = *reinterpret_cast<const Vec16<T> *>(p);
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = T::get(q.v[e]);
-  }
-}
+// V consecutive elements to p (16 bytes, or one)
 template <typename T, int V> __device__ __forceinline__ void store_v(void *base, long long at, const float *v) {
   auto *p = static_cast<typename T::storage *>(base) + at;
   if constexpr (V == 1) {
@@ -73,6 +83,22 @@ template <typename T, int V> __device__ __forceinline__ void store_v(void *base,
     *reinterpret_cast<Vec16<T> *>(p) = q;
   }
 }
+
+// V consecutive elements on their way, and their values
+template <typename T, int V> struct Raw {
+  typename std::conditional<V == 1, typename T::storage, Vec16<T>>::type v;
+  __device__ __forceinline__ void load(const void *base, long long at) {
+    v = *reinterpret_cast<const decltype(v) *>(static_cast<const typename T::storage *>(base) + at);
+  }
+  __device__ __forceinline__ void get(float *f) const {
+    if constexpr (V == 1) {
+      f[0] = T::get(v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = T::get(v.v[e]);
+    }
+  }
+};
 
 // 1 / (1 - p) or 0 for the V elements from `at` on (V > 1: at is a multiple of 4)
 template <int V> __device__ __forceinline__ void keep_v(const Drop &d, unsigned long long seed, unsigned long long offset, long long at, float *m) {
@@ -103,22 +129,22 @@ __device__ __forceinline__ void row_stats(const float (&v)[NV][V], const bool (&
   const float inv_c = 1.f / (float)C;
   mean = 0.f;
   if (kind == CL3D_NORM_LAYER) {
-    float a = 0.f, b = 0.f;
+    float a = 0.f, none = 0.f;
 #pragma unroll
     for (int q = 0; q < NV; ++q)
       if (on[q])
 #pragma unroll
         for (int e = 0; e < V; ++e) a += v[q][e];
-    row_sum<TPR>(a, b, s_red);
+    row_sum<TPR>(a, none, s_red);
     mean = a * inv_c;
   }
-  float a = 0.f, b = 0.f;
+  float a = 0.f, none = 0.f;
 #pragma unroll
   for (int q = 0; q < NV; ++q)
     if (on[q])
 #pragma unroll
       for (int e = 0; e < V; ++e) a = __builtin_fmaf(v[q][e] - mean, v[q][e] - mean, a);
-  row_sum<TPR>(a, b, s_red);
+  row_sum<TPR>(a, none, s_red);
   rinv = 1.f / sqrtf(a * inv_c + eps);
 }
 
@@ -149,19 +175,32 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
   }
   unsigned long long seed = 0, offset = 0;
   if (a.has_drop) { seed = a.drop.state[0]; offset = a.drop.state[1]; }
-  // every lane walks the same number of rows (row_sum's barriers): a group behind the last row works on the last one, unstored
-  for (long long r0 = first; r0 < last; r0 += 256 / TPR) {
-    const bool live = r0 + group < last;
-    const long long r = live ? r0 + group : last - 1;
-    float v[NV][V];
+  // every lane walks the same number of rows (row_sum's barriers): a group behind the last row works on the last one, unstored.
+  // The next rows are on their way while these are worked on: a wave's time is the latency of its row, and few rows fit a CU
+  constexpr int kStep = 256 / TPR;
+  Raw<T, V> nx[NV], ny[NV];
+  auto fetch = [&](long long r) {
+    r = r < last ? r : last - 1;
 #pragma unroll
     for (int q = 0; q < NV; ++q)
-      if (on[q]) load_v<T, V>(a.x, r * a.C + col[q], v[q]);
-    if (a.exit) {
-      float y[NV][V];
+      if (on[q]) {
+        nx[q].load(a.x, r * a.C + col[q]);
+        if (a.exit) ny[q].load(a.y, r * a.C + col[q]);
+      }
+  };
+  fetch(first + group);
+  for (long long r0 = first; r0 < last; r0 += kStep) {
+    const bool live = r0 + group < last;
+    const long long r = live ? r0 + group : last - 1;
+    float v[NV][V], y[NV][V];
 #pragma unroll
-      for (int q = 0; q < NV; ++q)
-        if (on[q]) load_v<T, V>(a.y, r * a.C + col[q], y[q]);
+    for (int q = 0; q < NV; ++q)
+      if (on[q]) {
+        nx[q].get(v[q]);
+        if (a.exit) ny[q].get(y[q]);
+      }
+    if (r0 + kStep < last) fetch(r0 + kStep + group);
+    if (a.exit) {
       float mean = 0.f, rinv = 1.f;
       if (a.kind1 != CL3D_NORM_NONE) row_stats<TPR, NV, V>(y, on, a.kind1, a.eps1, a.C, s_red, mean, rinv);
       if (a.stats && live && lane == 0) *reinterpret_cast<float2 *>(a.stats + 4 * r) = make_float2(mean, rinv);
@@ -225,18 +264,48 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
   }
   unsigned long long seed = 0, offset = 0;
   if (a.has_drop) { seed = a.drop.state[0]; offset = a.drop.state[1]; }
-  for (long long r0 = first; r0 < last; r0 += 256 / TPR) {
+  constexpr int kStep = 256 / TPR;
+  Raw<T, V> nx[NV], ny[NV], nd[NV], nh[NV];
+  f32x4 ns;
+  auto fetch = [&](long long r) {  // (as in the forward kernel)
+    r = r < last ? r : last - 1;
+    ns = *reinterpret_cast<const f32x4 *>(a.stats + 4 * r);
+#pragma unroll
+    for (int q = 0; q < NV; ++q)
+      if (on[q]) {
+        if (a.exit) ny[q].load(a.y, r * a.C + col[q]);
+        if (a.dout) nd[q].load(a.dout, r * a.C + col[q]);
+        if (a.dnext) {
+          nx[q].load(a.x, r * a.C + col[q]);
+          nh[q].load(a.dnext, r * a.C + col[q]);
+        }
+      }
+  };
+  fetch(first + group);
+  for (long long r0 = first; r0 < last; r0 += kStep) {
     const bool live = r0 + group < last;
     const long long r = live ? r0 + group : last - 1;
-    const f32x4 st = *reinterpret_cast<const f32x4 *>(a.stats + 4 * r);
+    const f32x4 st = ns;
+    float hat1[NV][V], keep[NV][V], d[NV][V], hat[NV][V], dh[NV][V];
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[q][e] = 0.f;
+      if (!on[q]) continue;
+      if (a.exit) ny[q].get(hat1[q]);
+      if (a.dout) nd[q].get(d[q]);
+      if (a.dnext) {
+        nx[q].get(hat[q]);
+        nh[q].get(dh[q]);
+      }
+    }
+    if (r0 + kStep < last) fetch(r0 + kStep + group);
     // the exit once more, from x and y: out as the forward pass had it before it was rounded costs no more traffic than the
     // rounded one, and the y hats are needed below anyway.  keep: 1 / (1 - p) or 0; hat1, n: of y
-    float hat1[NV][V], keep[NV][V], d[NV][V];
     if (a.exit) {
 #pragma unroll
       for (int q = 0; q < NV; ++q) {
         if (!on[q]) continue;
-        load_v<T, V>(a.y, r * a.C + col[q], hat1[q]);
         if (a.has_drop) keep_v<V>(a.drop, seed, offset, r * a.C + col[q], keep[q]);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -245,19 +314,11 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
         }
       }
     }
-#pragma unroll
-    for (int q = 0; q < NV; ++q) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) d[q][e] = 0.f;
-      if (a.dout && on[q]) load_v<T, V>(a.dout, r * a.C + col[q], d[q]);
-    }
     if (a.dnext) {
-      float hat[NV][V], dh[NV][V], p1 = 0.f, p2 = 0.f;
+      float p1 = 0.f, p2 = 0.f;
 #pragma unroll
       for (int q = 0; q < NV; ++q) {
         if (!on[q]) continue;
-        load_v<T, V>(a.x, r * a.C + col[q], hat[q]);
-        load_v<T, V>(a.dnext, r * a.C + col[q], dh[q]);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           if (a.exit) {
@@ -368,7 +429,7 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
   if (a.b2) flush(s_b2, 4);
 }
 
-// sums of the partial rows [first row of the sum ...][which][C]: 64 columns a workgroup, 16 rows at a time, joined in order
+// sums of the partial rows [row][which][C]: 16 columns a workgroup, 64 runs of rows side by side, joined in order
 struct NormSums {
   const float *partial;
   void *out[5];
@@ -376,21 +437,23 @@ struct NormSums {
 };
 template <typename T>
 __global__ __launch_bounds__(1024) void norm_sums_kernel(NormSums a) {
-  __shared__ float s[16][64];
-  const int which = blockIdx.y, c = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+  __shared__ float s[64][17];
+  const int which = blockIdx.y, col = threadIdx.x & 15, part = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
   const bool cloud = which == 2 && a.gate_cloud;
   const int b = blockIdx.z;
   if (a.out[which] == nullptr || (!cloud && b > 0)) return;
   const int rows = cloud ? a.chunks : a.rows, first = cloud ? b * a.chunks : 0;
   float t = 0.f;
-  if (c < a.C)
-    for (int r = part; r < rows; r += 16) t += a.partial[((long long)(first + r) * 5 + which) * a.C + c];
-  s[part][threadIdx.x & 63] = t;
+  if (c < a.C) {
+#pragma unroll 4
+    for (int r = part; r < rows; r += 64) t += a.partial[((long long)(first + r) * 5 + which) * a.C + c];
+  }
+  s[part][col] = t;
   __syncthreads();
-  if (part != 0 || c >= a.C) return;
+  if (threadIdx.x >= 16 || c >= a.C) return;
   t = 0.f;
 #pragma unroll
-  for (int q = 0; q < 16; ++q) t += s[q][threadIdx.x];
+  for (int q = 0; q < 64; ++q) t += s[q][col];
   const long long at = (cloud ? (long long)b * a.C : 0) + c;
   if (a.param_f32) static_cast<float *>(a.out[which])[at] = t;
   else static_cast<typename T::storage *>(a.out[which])[at] = T::put(t);
@@ -414,16 +477,19 @@ struct NormMap {
   int tpr, nv, v;
 };
 // lanes of a row and pieces of a lane: 16-byte pieces where C and the pointers allow, else single elements.  As few lanes as hold
-// the row in one piece each (several rows a wave), the whole workgroup where 64 do not.
+// the row in one piece each (several rows a wave), the whole workgroup where 64 do not; a lane's pieces cost registers (a row's
+// values and the sums of its columns: 23 per element backward), so there are variants for 1, 2, 4 ... of them.
 static NormMap norm_map(int dtype, int C, bool aligned) {
   const int kv = dtype == CL3D_F32 ? 4 : 8;
   const int v = aligned && C % kv == 0 ? kv : 1;
-  const int pieces = C / v;
-  NormMap m{256, 1, v};
-  if (v > 1 && pieces <= 16) m.tpr = 16;
-  else if (pieces <= 64) m.tpr = 64;
-  while (m.tpr * m.nv < pieces) m.nv = m.nv == 1 ? (v == 1 ? 8 : v == 4 ? 8 : 4) : 32;
-  return m;
+  const int pieces = C / v, need = (pieces + 255) / 256;
+  if (v > 1 && pieces <= 16) return {16, 1, v};
+  if (v > 1 && pieces <= 32) return {32, 1, v};
+  if (pieces <= 64) return {64, 1, v};
+  if (need <= 2) return {256, need, v};
+  if (need <= 4) return {256, 4, v};
+  if (v == 1) return {256, need <= 10 ? 10 : 32, v};
+  return {256, 8, v};
 }
 
 template <typename T, int TPR, int NV, int V> static void norm_run(bool backward, const NormArgs &a, hipStream_t st) {
@@ -432,18 +498,22 @@ template <typename T, int TPR, int NV, int V> static void norm_run(bool backward
   else hipLaunchKernelGGL((norm_fwd_kernel<T, TPR, NV, V>), grid, dim3(256), 0, st, a);
 }
 template <typename T> static void norm_pick(const NormMap &m, bool backward, const NormArgs &a, hipStream_t st) {
-  constexpr int V = T::kVec, NW = V == 4 ? 8 : 4;
+  constexpr int V = T::kVec;
   if (m.v == 1) {
-    if (m.tpr == 64) norm_run<T, 64, 1, 1>(backward, a, st);
-    else if (m.nv == 1) norm_run<T, 256, 1, 1>(backward, a, st);
-    else if (m.nv == 8) norm_run<T, 256, 8, 1>(backward, a, st);
-    else norm_run<T, 256, 32, 1>(backward, a, st);
-  } else {
-    if (m.tpr == 16) norm_run<T, 16, 1, V>(backward, a, st);
-    else if (m.tpr == 64) norm_run<T, 64, 1, V>(backward, a, st);
-    else if (m.nv == 1) norm_run<T, 256, 1, V>(backward, a, st);
-    else norm_run<T, 256, NW, V>(backward, a, st);
+    if (m.tpr == 64) return norm_run<T, 64, 1, 1>(backward, a, st);
+    if (m.nv == 1) return norm_run<T, 256, 1, 1>(backward, a, st);
+    if (m.nv == 2) return norm_run<T, 256, 2, 1>(backward, a, st);
+    if (m.nv == 4) return norm_run<T, 256, 4, 1>(backward, a, st);
+    if (m.nv == 10) return norm_run<T, 256, 10, 1>(backward, a, st);
+    return norm_run<T, 256, 32, 1>(backward, a, st);
   }
+  if (m.tpr == 16) return norm_run<T, 16, 1, V>(backward, a, st);
+  if (m.tpr == 32) return norm_run<T, 32, 1, V>(backward, a, st);
+  if (m.tpr == 64) return norm_run<T, 64, 1, V>(backward, a, st);
+  if (m.nv == 1) return norm_run<T, 256, 1, V>(backward, a, st);
+  if (m.nv == 2) return norm_run<T, 256, 2, V>(backward, a, st);
+  if (m.nv == 4) return norm_run<T, 256, 4, V>(backward, a, st);
+  if constexpr (V == 4) norm_run<T, 256, 8, V>(backward, a, st);
 }
 static void norm_launch(int dtype, const NormMap &m, bool backward, const NormArgs &a, hipStream_t st) {
   if (dtype == CL3D_F32) norm_pick<F32>(m, backward, a, st);
@@ -454,6 +524,7 @@ static void norm_launch(int dtype, const NormMap &m, bool backward, const NormAr
 static int norm_checks(const cl3d_norm_residual *p, bool backward, const char *who) {
   CL3D_REQUIRE(p != nullptr, "%s: null argument block", who);
   CL3D_REQUIRE(p->dtype == CL3D_F32 || p->dtype == CL3D_BF16 || p->dtype == CL3D_F16, "%s: unknown element type %d", who, p->dtype);
+  CL3D_REQUIRE(p->order == CL3D_POINT_MAJOR || p->order == CL3D_CHANNEL_MAJOR, "%s: unknown memory order %d", who, p->order);
   CL3D_REQUIRE(p->B >= 0 && p->N >= 0 && p->C > 0, "%s: bad sizes", who);
   CL3D_REQUIRE(p->kind >= CL3D_NORM_NONE && p->kind <= CL3D_NORM_LAYER && p->next_kind >= CL3D_NORM_NONE && p->next_kind <= CL3D_NORM_LAYER,
                "%s: unknown norm", who);
@@ -480,10 +551,38 @@ static void norm_args(NormArgs &a, const cl3d_norm_residual *p) {
 }
 
 constexpr int kNormBwdGroups = 1024;
-size_t point_norm_workspace(int B, int N, int C) {
+
+// point-major copies of channel-major tensors, and back
+struct NormCopies {
+  const cl3d_norm_residual *p;
+  Arena ar;
+  hipStream_t st;
+  bool copies;
+  int rc = CL3D_OK;
+  NormCopies(const cl3d_norm_residual *p_, void *ws, hipStream_t st_)
+      : p(p_), ar(ws), st(st_), copies(p_->order == CL3D_CHANNEL_MAJOR && p_->N > 1 && p_->C > 1) {}
+  void *place() { return ar.take((size_t)p->B * p->N * p->C * elem_bytes(p->dtype)); }
+  const void *in(const void *t) {
+    if (!copies || !t) return t;
+    void *d = place();
+    if (d && rc == CL3D_OK) rc = transposed(p->dtype, t, p->B, p->C, p->N, d, st);
+    return d;
+  }
+  void *out(void *t) { return copies && t ? place() : t; }
+  void back(const void *rows, void *t) {
+    if (copies && t && rc == CL3D_OK) rc = transposed(p->dtype, rows, p->B, p->N, p->C, t, st);
+  }
+};
+
+size_t point_norm_workspace(int B, int N, int C, int flags) {
+  // flags: element type | memory order << 2 | tensors to copy << 3 | parameter gradients << 8
+  if (B <= 0 || N <= 0 || C <= 0) return 0;
+  Arena ar(nullptr);
+  if (((flags >> 2) & 1) == CL3D_CHANNEL_MAJOR && N > 1 && C > 1)
+    for (int q = 0; q < ((flags >> 3) & 31); ++q) ar.take((size_t)B * N * C * elem_bytes(flags & 3));
   // partial rows of the backward pass: at most kNormBwdGroups + B workgroups
-  (void)N;
-  return ((size_t)kNormBwdGroups + (B > 0 ? B : 0)) * 5 * (size_t)(C > 0 ? C : 0) * sizeof(float);
+  if ((flags >> 8) & 1) ar.take(((size_t)kNormBwdGroups + B) * 5 * (size_t)C * sizeof(float));
+  return ar.used;
 }
 
 }  // namespace cl3d
@@ -498,11 +597,19 @@ extern "C" int cl3d_norm_residual_fwd(const cl3d_norm_residual *p, cl3d_stream_t
   if (rc != CL3D_OK) return rc;
   if (p->B == 0 || p->N == 0) return CL3D_OK;
   CL3D_REQUIRE(p->x && (!a.exit || p->out) && (!a.next || p->next), "norm_residual_fwd: null pointer");
-  a.o = p->out; a.h = p->next;
-  const NormMap m = norm_map(p->dtype, p->C, aligned16(p->x) && aligned16(p->y) && aligned16(p->out) && aligned16(p->next));
+  const hipStream_t st = (hipStream_t)stream;
+  NormCopies need(p, nullptr, st), c(p, p->ws, st);
+  need.in(p->x), need.in(p->y), need.out(p->out), need.out(p->next);
+  if (need.ar.used && (!p->ws || p->ws_bytes < need.ar.used))
+    return fail(CL3D_E_WORKSPACE, "norm_residual_fwd: %zu bytes of scratch, %zu needed", p->ws_bytes, need.ar.used);
+  a.x = c.in(p->x); a.y = c.in(p->y);
+  a.o = c.out(p->out); a.h = c.out(p->next);
+  if (c.rc != CL3D_OK) return c.rc;
+  const NormMap m = norm_map(p->dtype, p->C, aligned16(a.x) && aligned16(a.y) && aligned16(a.o) && aligned16(a.h));
   norm_grid(a, 256 / m.tpr, 2048);
-  norm_launch(p->dtype, m, false, a, (hipStream_t)stream);
-  return check_launch("cl3d_norm_residual_fwd");
+  norm_launch(p->dtype, m, false, a, st);
+  c.back(a.o, p->out), c.back(a.h, p->next);
+  return c.rc != CL3D_OK ? c.rc : check_launch("cl3d_norm_residual_fwd");
 }
 
 extern "C" int cl3d_norm_residual_bwd(const cl3d_norm_residual *p, cl3d_stream_t stream) {
@@ -517,22 +624,30 @@ extern "C" int cl3d_norm_residual_bwd(const cl3d_norm_residual *p, cl3d_stream_t
   CL3D_REQUIRE(p->stats && (p->dout || p->dnext), "norm_residual_bwd: null pointer");
   CL3D_REQUIRE(!p->dnext || (a.next && p->x), "norm_residual_bwd: a gradient of a norm that was not formed");
   CL3D_REQUIRE(!p->dout || a.exit, "norm_residual_bwd: a gradient of a sum that was not formed");
-  a.dout = p->dout; a.dnext = p->dnext; a.dx = p->dx; a.dy = p->dy;
-  const NormMap m = norm_map(p->dtype, p->C, aligned16(p->x) && aligned16(p->y) && aligned16(p->dout) && aligned16(p->dnext) &&
-                                                 aligned16(p->dx) && aligned16(p->dy));
-  norm_grid(a, 256 / m.tpr, kNormBwdGroups);
-  const bool sums = p->dweight || p->dbias || p->dgate || p->dnext_weight || p->dnext_bias;
-  if (sums) {
-    const size_t need = (size_t)a.B * a.chunks * 5 * a.C * sizeof(float);
-    if (!p->ws || p->ws_bytes < need) return fail(CL3D_E_WORKSPACE, "norm_residual_bwd: %zu bytes of scratch, %zu needed", p->ws_bytes, need);
-    a.partial = static_cast<float *>(p->ws);
-  }
   const hipStream_t st = (hipStream_t)stream;
+  const bool sums = p->dweight || p->dbias || p->dgate || p->dnext_weight || p->dnext_bias;
+  const void *x = p->dnext ? p->x : nullptr;  // (without the entry's gradient x is not looked at)
+  NormCopies need(p, nullptr, st), c(p, p->ws, st);
+  need.in(x), need.in(p->y), need.in(p->dout), need.in(p->dnext), need.out(p->dx), need.out(p->dy);
+  const NormMap m = norm_map(p->dtype, p->C, need.copies || (aligned16(x) && aligned16(p->y) && aligned16(p->dout) && aligned16(p->dnext) &&
+                                                             aligned16(p->dx) && aligned16(p->dy)));
+  norm_grid(a, 256 / m.tpr, kNormBwdGroups);
+  const size_t partial_bytes = sums ? (size_t)a.B * a.chunks * 5 * a.C * sizeof(float) : 0;
+  if (sums) need.ar.take(partial_bytes);
+  if (need.ar.used && (!p->ws || p->ws_bytes < need.ar.used))
+    return fail(CL3D_E_WORKSPACE, "norm_residual_bwd: %zu bytes of scratch, %zu needed", p->ws_bytes, need.ar.used);
+  CL3D_REQUIRE(aligned16(p->ws), "norm_residual_bwd: scratch starts on 16 bytes");
+  a.x = c.in(x); a.y = c.in(p->y); a.dout = c.in(p->dout); a.dnext = c.in(p->dnext);
+  a.dx = c.out(p->dx); a.dy = c.out(p->dy);
+  if (sums) a.partial = static_cast<float *>(c.ar.take(partial_bytes));
+  if (c.rc != CL3D_OK) return c.rc;
   norm_launch(p->dtype, m, true, a, st);
+  c.back(a.dx, p->dx), c.back(a.dy, p->dy);
+  if (c.rc != CL3D_OK) return c.rc;
   if (sums) {
     NormSums s{a.partial, {a.exit ? p->dweight : nullptr, a.exit ? p->dbias : nullptr, a.exit ? p->dgate : nullptr, p->dnext_weight, p->dnext_bias},
                a.C, a.B * a.chunks, a.chunks, a.gate_cloud, a.param_f32};
-    const dim3 grid(ceil_div(a.C, 64), 5, a.gate_cloud && p->dgate ? a.B : 1);
+    const dim3 grid(ceil_div(a.C, 16), 5, a.gate_cloud && p->dgate ? a.B : 1);
     if (p->dtype == CL3D_F32) hipLaunchKernelGGL(norm_sums_kernel<F32>, grid, dim3(1024), 0, st, s);
     else if (p->dtype == CL3D_BF16) hipLaunchKernelGGL(norm_sums_kernel<Bf16>, grid, dim3(1024), 0, st, s);
     else hipLaunchKernelGGL(norm_sums_kernel<F16>, grid, dim3(1024), 0, st, s);

@@ -73,7 +73,10 @@ def _check_param(t, shape, x, who, name, optional=True, f32=True):
 
 
 def _point_major(t):
-    return t.is_contiguous() if t.dim() == 2 else t.transpose(1, 2).is_contiguous()
+    if t.dim() == 2:
+        return t.is_contiguous()
+    (_, C, N), s = t.shape, t.stride()
+    return (s[1] == 1 and s[2] == C and s[0] == C * N) or t.transpose(1, 2).is_contiguous()
 
 
 def _aligned(t):
@@ -90,9 +93,30 @@ def _order(t):
     return _aligned(t.contiguous()), _CHANNEL
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # (torch.cuda.current_stream() builds an object: 3.5 us a call)
+
+
+def _stream(device):
+    return _raw_stream(device.index)
+
+
+_WORKSPACE = {}  # sizes of scratch, by what cl3d_workspace_bytes was asked
+
+
+def _workspace(op, B, N, M, K, C, device):
+    key = (op, B, N, M, K, C)
+    nbytes = _WORKSPACE.get(key)
+    if nbytes is None:
+        if len(_WORKSPACE) > 4096:
+            _WORKSPACE.clear()
+        nbytes = _WORKSPACE[key] = _lib.lib().cl3d_workspace_bytes(*key)
+    return torch.empty(nbytes or 1, dtype=torch.uint8, device=device), nbytes
+
+
 def _empty(shape, order, dtype, device):
     if len(shape) == 3 and order == _POINT:
-        return torch.empty((shape[0], shape[2], shape[1]), dtype=dtype, device=device).transpose(1, 2)
+        B, C, N = shape
+        return torch.empty_strided(shape, (N * C, 1, C), dtype=dtype, device=device)
     return torch.empty(shape, dtype=dtype, device=device)
 
 
@@ -105,7 +129,7 @@ def _swap(src, B, R, C, dst):
     lib = _lib.lib()
     fn = lib.cl3d_transpose if src.dtype == torch.float32 else lib.cl3d_transpose16
     with _lib.on_device(src.device):
-        _lib.check(fn(_p(src), B, R, C, _p(dst), _lib.stream_ptr(src.device)))
+        _lib.check(fn(_p(src), B, R, C, _p(dst), _stream(src.device)))
     return dst
 
 
@@ -162,20 +186,18 @@ _LIVE = weakref.WeakSet()
 
 def _track(ctx, *inputs):
     """Called by a forward pass that autograd records, with the tensors it was given."""
-    leaves = [weakref.ref(t) for t in inputs if t is not None and t.is_leaf and t.requires_grad]
-    if leaves and not torch.cuda.is_current_stream_capturing():
-        ctx.leaves, ctx.made_on = leaves, torch.cuda.current_stream(inputs[0].device).cuda_stream
+    ctx.leaves = [weakref.ref(t) for t in inputs if t is not None and t.requires_grad and t.is_leaf]
+    if ctx.leaves and not torch.cuda.is_current_stream_capturing():
+        ctx.made_on = _raw_stream(inputs[0].device.index)
         _LIVE.add(ctx)
-    elif leaves:
-        ctx.leaves, ctx.made_on = leaves, None
 
 
 def _check_capture(ctx, device):
     """Called by a backward pass."""
     if not _LIVE or not torch.cuda.is_current_stream_capturing():
         return
-    mine = {id(t) for t in (r() for r in getattr(ctx, 'leaves', ())) if t is not None}
-    stream = torch.cuda.current_stream(device).cuda_stream
+    mine = {id(t) for t in (r() for r in ctx.leaves) if t is not None}
+    stream = _raw_stream(device.index)
     for other in list(_LIVE):
         if other is not ctx and other.made_on != stream and any(id(r()) in mine for r in other.leaves if r() is not None):
             raise RuntimeError("a backward pass is being captured while an eager graph of the same leaves, made on another stream, is "
@@ -183,57 +205,65 @@ def _check_capture(ctx, device):
 
 
 # ------------------------------------------------------------------------------------------------- gated feed-forward
+_FEW_POINTS, _HIDDEN = 64, 512  # CL3D_FFN_FEW, CL3D_FFN_HIDDEN
+
+
+def _ffn_forward(x, w_gate, w_up, w_down, activation, precision, keep_hidden):
+    """y and what a backward pass needs: the tensors as the kernels read them, the hidden activations if asked for, the sizes."""
+    shape, dtype, device = x.shape, _DTYPES[x.dtype], x.device
+    B, C, N = _sizes(x)
+    x, order = _order(x)
+    w_gate, w_up = _aligned(w_gate.contiguous()), _aligned(w_up.contiguous())
+    w_down = None if w_down is None else _aligned(w_down.contiguous())
+    H = w_gate.shape[0]
+    y = _empty((shape[0], C if w_down is not None else H) + tuple(shape[2:]), order, x.dtype, device)
+    hidden = None
+    if keep_hidden and w_down is not None and B * N > _FEW_POINTS:
+        hidden = torch.empty((3 if dtype == 0 and precision == 0 else 1, B * N, (H + 7) // 8 * 8), dtype=torch.int16, device=device)
+    if B * N:
+        flags = dtype | order << 2 | precision << 3 | (w_down is not None) << 4 | (_HIDDEN if hidden is not None else 0)
+        ws, nbytes = _workspace(_OP_GATED_FFN, B, N, H, flags, C, device)
+        with _lib.on_device(device):
+            _lib.check(_lib.lib().cl3d_gated_ffn_fwd(_p(x), _p(w_gate), _p(w_up), _p(w_down), dtype, order, B, C, N, H, activation,
+                                                     precision, _p(y), _p(hidden), _p(ws), nbytes, _stream(device)))
+    return y, (x, w_gate, w_up, w_down, hidden), (order, B, C, N, H, activation, precision)
+
+
 class _GatedFeedForward(Function):
-    """One C-ABI call per direction.  Kept for the backward pass: x and the weights (the hidden activations are formed again)."""
+    """One C-ABI call per direction.  Kept for the backward pass: x, the weights and, if w_down has a gradient, the hidden
+    activations; the two projections are formed again."""
 
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, activation, precision, need_grad):
-        shape = x.shape
-        B, C, N = _sizes(x)
-        if need_grad:
-            _track(ctx, x, w_gate, w_up, w_down)
-        x, order = _order(x)
-        w_gate, w_up = _aligned(w_gate.contiguous()), _aligned(w_up.contiguous())
-        w_down = None if w_down is None else _aligned(w_down.contiguous())
-        H = w_gate.shape[0]
-        y = _empty((shape[0], C if w_down is not None else H) + tuple(shape[2:]), order, x.dtype, x.device)
-        dtype = _DTYPES[x.dtype]
-        if y.numel():
-            lib = _lib.lib()
-            flags = dtype | order << 2 | precision << 3 | (w_down is not None) << 4
-            nbytes = lib.cl3d_workspace_bytes(_OP_GATED_FFN, B, N, H, flags, C)
-            ws = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device=x.device)
-            with _lib.on_device(x.device):
-                _lib.check(lib.cl3d_gated_ffn_fwd(_p(x), _p(w_gate), _p(w_up), _p(w_down), dtype, order, B, C, N, H, activation,
-                                                  precision, _p(y), _p(ws), nbytes, _lib.stream_ptr(x.device)))
-        ctx.save_for_backward(x, w_gate, w_up, w_down)
-        ctx.args = (order, B, C, N, H, activation, precision)
+    def forward(ctx, x, w_gate, w_up, w_down, activation, precision):
+        _track(ctx, x, w_gate, w_up, w_down)
+        y, kept, ctx.args = _ffn_forward(x, w_gate, w_up, w_down, activation, precision, ctx.needs_input_grad[3])
+        ctx.save_for_backward(*kept)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, w_gate, w_up, w_down = ctx.saved_tensors
+        x, w_gate, w_up, w_down, hidden = ctx.saved_tensors
         _check_capture(ctx, x.device)
         order, B, C, N, H, activation, precision = ctx.args
         need = ctx.needs_input_grad
-        new = torch.empty_like if x.numel() else torch.zeros_like
+        new = torch.empty_like if B * N else torch.zeros_like
         dx = _empty(x.shape, order, x.dtype, x.device) if need[0] else None
         dwg = new(w_gate) if need[1] else None
         dwu = new(w_up) if need[2] else None
         dwd = new(w_down) if w_down is not None and need[3] else None
-        if x.numel():
+        if B * N:
             dy = _as_order(dy, order)
-            lib, dtype = _lib.lib(), _DTYPES[x.dtype]
+            dtype = _DTYPES[x.dtype]
             wants = (dx is not None) | (dwg is not None or dwu is not None) << 1 | (dwd is not None) << 2
-            flags = dtype | order << 2 | precision << 3 | (w_down is not None) << 4 | 32 | wants << 6
-            nbytes = lib.cl3d_workspace_bytes(_OP_GATED_FFN, B, N, H, flags, C)
-            ws = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device=x.device)
+            flags = (dtype | order << 2 | precision << 3 | (w_down is not None) << 4 | 32 | wants << 6
+                     | (_HIDDEN if hidden is not None else 0))
+            ws, nbytes = _workspace(_OP_GATED_FFN, B, N, H, flags, C, x.device)
             with _lib.on_device(x.device):
-                _lib.check(lib.cl3d_gated_ffn_bwd(_p(x), _p(w_gate), _p(w_up), _p(w_down), _p(dy), dtype, order, B, C, N, H,
-                                                  activation, precision, _p(dx), _p(dwg), _p(dwu), _p(dwd), _p(ws), nbytes,
-                                                  _lib.stream_ptr(x.device)))
-        return dx, dwg, dwu, dwd, None, None, None
+                _lib.check(_lib.lib().cl3d_gated_ffn_bwd(_p(x), _p(w_gate), _p(w_up), _p(w_down), _p(dy), _p(hidden), dtype, order, B,
+                                                         C, N, H, activation, precision, _p(dx), _p(dwg), _p(dwu), _p(dwd), _p(ws),
+                                                         nbytes, _stream(x.device)))
+        return dx, dwg, dwu, dwd, None, None
 
 
 def gated_feed_forward(x, w_gate, w_up, w_down=None, activation='silu', precision='f32'):
@@ -257,83 +287,79 @@ def gated_feed_forward(x, w_gate, w_up, w_down=None, activation='silu', precisio
         raise ValueError(f"{who}: activation is one of {sorted(_ACTIVATIONS)}, got {activation!r}")
     if precision not in _PRECISIONS:
         raise ValueError(f"{who}: precision is one of {sorted(_PRECISIONS)}, got {precision!r}")
-    return _GatedFeedForward.apply(x, w_gate, w_up, w_down, _ACTIVATIONS[activation], _PRECISIONS[precision],
-                                   _wants_grad(x, w_gate, w_up, w_down))
+    args = (x, w_gate, w_up, w_down, _ACTIVATIONS[activation], _PRECISIONS[precision])
+    # (without a gradient: no autograd node)
+    return _GatedFeedForward.apply(*args) if _wants_grad(x, w_gate, w_up, w_down) else _ffn_forward(*args, False)[0]
 
 
 # ---------------------------------------------------------------------------------------------- norms around a block
+def _norm_forward(x, y, weight, bias, gate, next_weight, next_bias, rng, opts, need_grad):
+    """(out, next) in x's memory order, and what a backward pass needs."""
+    kind, next_kind, eps, next_eps, scale, p = opts
+    shape, dtype, device = x.shape, x.dtype, x.device
+    B, C, N = _sizes(x)
+    x, order = _order(x)
+    y = None if y is None else _as_order(y, order)
+    params = (weight, bias, gate, next_weight, next_bias)
+    f32 = any(t is not None and t.dtype == torch.float32 for t in params)
+    # (one type for all of them: a mixture goes to f32)
+    held = [None if t is None else (t.float() if f32 else t).contiguous() for t in params]
+    out = _empty(shape, order, dtype, device) if y is not None else None
+    nxt = _empty(shape, order, dtype, device) if next_kind else None
+    stats = torch.empty((B * N, 4), dtype=torch.float32, device=device) if need_grad else None
+    sizes = (B, N, C, _DTYPES[dtype], f32, kind, next_kind, gate is not None and gate.dim() == 2, scale, eps, next_eps, order, p)
+    if B * N:
+        # (the fields of cl3d_norm_residual in their order)
+        block = _lib.NormResidual(*sizes, _p(rng), _p(x), _p(y), *map(_p, held), _p(out), _p(nxt), _p(stats))
+        if order == _CHANNEL:
+            copies = 1 + (y is not None) + (out is not None) + (nxt is not None)
+            ws, block.ws_bytes = _workspace(_OP_POINT_NORM, B, N, 0, sizes[3] | order << 2 | copies << 3, C, device)
+            block.ws = _p(ws)
+        with _lib.on_device(device):
+            _lib.check(_lib.lib().cl3d_norm_residual_fwd(ctypes.byref(block), _stream(device)))
+    # (an exit alone: x is not looked at again)
+    return out, nxt, (x if next_kind else None, y, *held, rng, stats), (order, shape, dtype, sizes, [None if t is None else t.dtype for t in params])
+
+
 class _NormResidual(Function):
-    """cl3d_norm_residual_fwd / _bwd on point-major rows."""
+    """cl3d_norm_residual_fwd / _bwd."""
 
     @staticmethod
     def forward(ctx, x, y, weight, bias, gate, next_weight, next_bias, rng, opts):
-        kind, next_kind, eps, next_eps, scale, p, need_grad = opts
-        shape, dtype, device = x.shape, x.dtype, x.device
-        B, C, N = _sizes(x)
-        order = _order(x)[1]
-        xr = _as_order(x, _POINT)
-        yr = None if y is None else _as_order(y, _POINT)
-        params = [weight, bias, gate, next_weight, next_bias]
-        f32 = any(t is not None and t.dtype == torch.float32 for t in params)
-        # (one type for all of them: a mixture goes to f32)
-        held = [None if t is None else (t.float() if f32 else t).contiguous() for t in params]
-        block = _lib.NormResidual(B=B, N=N, C=C, dtype=_DTYPES[dtype], param_f32=int(f32), kind=kind, next_kind=next_kind,
-                                  gate_cloud=int(gate is not None and gate.dim() == 2), residual_scale=scale, eps=eps,
-                                  next_eps=next_eps, p=p)
-        out = _empty(shape, _POINT, dtype, device) if y is not None else None
-        nxt = _empty(shape, _POINT, dtype, device) if next_kind else None
-        stats = torch.empty((B * N, 4), dtype=torch.float32, device=device) if need_grad else None
-        _fill(block, rng=rng, x=xr, y=yr, weight=held[0], bias=held[1], gate=held[2], next_weight=held[3], next_bias=held[4], out=out,
-              next=nxt, stats=stats)
-        if x.numel():
-            with _lib.on_device(device):
-                _lib.check(_lib.lib().cl3d_norm_residual_fwd(ctypes.byref(block), _lib.stream_ptr(device)))
+        _track(ctx, x, y, weight, bias, gate, next_weight, next_bias)
+        out, nxt, kept, ctx.args = _norm_forward(x, y, weight, bias, gate, next_weight, next_bias, rng, opts, True)
         ctx.set_materialize_grads(False)
-        if need_grad:
-            _track(ctx, x, y, *params)
-            ctx.save_for_backward(xr if next_kind else None, yr, *held, rng, stats)  # (an exit alone: x is not looked at again)
-            ctx.args = (order, B, C, N, f32, shape, dtype, kind, next_kind, scale, p, eps, next_eps,
-                        [None if t is None else t.dtype for t in params])
-        out = None if out is None else _as_order(out, order)
-        nxt = None if nxt is None else _as_order(nxt, order)
+        ctx.save_for_backward(*kept)
         return out, nxt
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dnext):
-        xr, yr, weight, bias, gate, next_weight, next_bias, rng, stats = ctx.saved_tensors
-        order, B, C, N, f32, shape, dtype, kind, next_kind, scale, p, eps, next_eps, types = ctx.args
+        x, y, weight, bias, gate, next_weight, next_bias, rng, stats = ctx.saved_tensors
+        order, shape, dtype, sizes, types = ctx.args
+        B, N, C = sizes[:3]
         need, device = ctx.needs_input_grad, stats.device
         _check_capture(ctx, device)
         if dout is None and dnext is None:
             return (None,) * 9
-        dout = None if dout is None else _as_order(dout, _POINT)
-        dnext = None if dnext is None else _as_order(dnext, _POINT)
-        dx = _empty(shape, _POINT, dtype, device) if need[0] else None
-        dy = _empty(shape, _POINT, dtype, device) if yr is not None and need[1] else None
-        empty = B * N == 0
-        grads = [None if t is None or not n else (torch.zeros_like(t) if empty else torch.empty_like(t))
-                 for t, n in zip((weight, bias, gate, next_weight, next_bias), need[2:7])]
-        if not empty:
-            lib = _lib.lib()
-            block = _lib.NormResidual(B=B, N=N, C=C, dtype=_DTYPES[dtype], param_f32=int(f32), kind=kind, next_kind=next_kind,
-                                      gate_cloud=int(gate is not None and gate.dim() == 2), residual_scale=scale, eps=eps,
-                                      next_eps=next_eps, p=p)
-            nbytes = lib.cl3d_workspace_bytes(_OP_POINT_NORM, B, N, 0, 0, C) if any(g is not None for g in grads) else 0
-            ws = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device=device)
-            _fill(block, rng=rng, x=xr, y=yr, weight=weight, bias=bias, gate=gate, next_weight=next_weight, next_bias=next_bias,
-                  stats=stats, dout=dout, dnext=dnext, dx=dx, dy=dy, dweight=grads[0], dbias=grads[1], dgate=grads[2],
-                  dnext_weight=grads[3], dnext_bias=grads[4], ws=ws)
-            block.ws_bytes = nbytes
+        dout = None if dout is None else _as_order(dout, order)
+        dnext = None if dnext is None else _as_order(dnext, order)
+        dx = _empty(shape, order, dtype, device) if need[0] else None
+        dy = _empty(shape, order, dtype, device) if y is not None and need[1] else None
+        new = torch.empty_like if B * N else torch.zeros_like
+        grads = [new(t) if t is not None and n else None for t, n in zip((weight, bias, gate, next_weight, next_bias), need[2:7])]
+        if B * N:
+            sums = any(g is not None for g in grads)
+            copies = 6 if order == _CHANNEL else 0
+            ws, nbytes = None, 0
+            if sums or copies:
+                ws, nbytes = _workspace(_OP_POINT_NORM, B, N, 0, sizes[3] | order << 2 | copies << 3 | sums << 8, C, device)
+            block = _lib.NormResidual(*sizes, _p(rng), _p(x), _p(y), _p(weight), _p(bias), _p(gate), _p(next_weight), _p(next_bias),
+                                      None, None, _p(stats), _p(dout), _p(dnext), _p(dx), _p(dy), *map(_p, grads), _p(ws), nbytes)
             with _lib.on_device(device):
-                _lib.check(lib.cl3d_norm_residual_bwd(ctypes.byref(block), _lib.stream_ptr(device)))
-        grads = [None if g is None else g.to(t) for g, t in zip(grads, types)]
-        return (None if dx is None else _as_order(dx, order), None if dy is None else _as_order(dy, order), *grads, None, None)
-
-
-def _fill(block, **tensors):
-    for name, t in tensors.items():
-        setattr(block, name, _p(t))
+                _lib.check(_lib.lib().cl3d_norm_residual_bwd(ctypes.byref(block), _stream(device)))
+        grads = [g if g is None or g.dtype == t else g.to(t) for g, t in zip(grads, types)]
+        return (dx, dy, *grads, None, None)
 
 
 def _check_norm(x, kind, eps, who, none=False):
@@ -356,8 +382,8 @@ def point_norm(x, weight=None, bias=None, kind='rms', eps=1e-6):
     C = x.shape[1]
     _check_param(weight, (C,), x, who, 'weight')
     _check_param(bias, (C,), x, who, 'bias')
-    need = _wants_grad(x, weight, bias)
-    return _NormResidual.apply(x, None, None, None, None, weight, bias, None, (0, _NORMS[kind], 0.0, float(eps), 1.0, 0.0, need))[1]
+    args = (x, None, None, None, None, weight, bias, None, (0, _NORMS[kind], 0.0, float(eps), 1.0, 0.0))
+    return (_NormResidual.apply(*args) if _wants_grad(x, weight, bias) else _norm_forward(*args, False))[1]
 
 
 def norm_gate_residual(x, y, weight=None, bias=None, gate=None, residual_scale=1.0, kind='rms', eps=1e-6, p=0.0, rng=None,
@@ -390,10 +416,10 @@ def norm_gate_residual(x, y, weight=None, bias=None, gate=None, residual_scale=1
     p = _check_p(p, who)
     if p > 0:
         _check_rng(rng, x, who)
+    args = (x, y, weight, bias, gate, next_weight, next_bias, rng if p > 0 else None,
+            (_NORMS[kind], _NORMS[next_kind], float(eps), float(eps if next_eps is None else next_eps), float(residual_scale), p))
     need = _wants_grad(x, y, weight, bias, gate, next_weight, next_bias)
-    out, nxt = _NormResidual.apply(x, y, weight, bias, gate, next_weight, next_bias, rng if p > 0 else None,
-                                   (_NORMS[kind], _NORMS[next_kind], float(eps), float(eps if next_eps is None else next_eps),
-                                    float(residual_scale), p, need))
+    out, nxt = _NormResidual.apply(*args) if need else _norm_forward(*args, False)[:2]
     return out if next_kind == 'none' else (out, nxt)
 
 
@@ -431,7 +457,7 @@ def _drop(x, p, rng):
     x = x.contiguous()
     out = torch.empty_like(x)
     with _lib.on_device(x.device):
-        _lib.check(_lib.lib().cl3d_dropout(_p(x), _DTYPES[x.dtype], x.numel(), p, _p(rng), _p(out), _lib.stream_ptr(x.device)))
+        _lib.check(_lib.lib().cl3d_dropout(_p(x), _DTYPES[x.dtype], x.numel(), p, _p(rng), _p(out), _stream(x.device)))
     return out
 
 
@@ -453,7 +479,7 @@ def dropout(x, p, rng):
     if p == 0.0:
         return x
     _check_rng(rng, x, who)
-    return _Dropout.apply(x, p, rng)
+    return _Dropout.apply(x, p, rng) if _wants_grad(x) else _drop(x, p, rng)
 
 
 class CounterRng:
@@ -473,7 +499,7 @@ class CounterRng:
             raise ValueError(f"CounterRng.take: {n} elements")
         out = torch.empty_like(self.state)
         with _lib.on_device(out.device):
-            _lib.check(_lib.lib().cl3d_rng_take(_p(self.state), (n + 3) // 4, _p(out), _lib.stream_ptr(out.device)))
+            _lib.check(_lib.lib().cl3d_rng_take(_p(self.state), (n + 3) // 4, _p(out), _stream(out.device)))
         return out
 
 

@@ -66,7 +66,7 @@ typedef void *cl3d_stream_t; /* hipStream_t */
 #define CL3D_OP_SPHERE_CROP 16   /* cl3d_sphere_crop_query: N = scene points; _assemble: N = num_points */
 
 #define CL3D_OP_GATED_FFN 17     /* cl3d_gated_ffn_fwd/bwd: (B, N, M = hidden, K = CL3D_FFN_* flags, C) */
-#define CL3D_OP_POINT_NORM 18    /* cl3d_norm_residual_bwd: (B, N, M, K unused, C) */
+#define CL3D_OP_POINT_NORM 18    /* cl3d_norm_residual_fwd/bwd: (B, N, M unused, K = CL3D_NORM_FLAGS, C) */
 
 int cl3d_abi_version(void);
 const char *cl3d_last_error_string(void);
@@ -552,24 +552,30 @@ int cl3d_reduce_train_backward(const cl3d_reduce_pass *p, cl3d_stream_t stream);
 /* y = (act(x w_gate^T) * (x w_up^T)) w_down^T for every point.  w_gate, w_up [H,C], w_down [C,H] (NULL: y is the product of the
  * two projections, H channels).  precision 0: f32 tensors are multiplied at f32 accuracy; 1: their values are rounded to bf16 in
  * front of every product (16-bit tensors: no difference).  Tensors start on 16 bytes.  Scratch:
- * cl3d_workspace_bytes(CL3D_OP_GATED_FFN, B, N, H, flags, C) with the flags below. */
+ * cl3d_workspace_bytes(CL3D_OP_GATED_FFN, B, N, H, flags, C) with the flags below.  hidden (NULL, or with w_down and more than
+ * CL3D_FFN_FEW points): receives the hidden activations, B N rows of H rounded up to 8, in 2 bytes each, 6 for f32 at precision 0;
+ * handed to the backward pass it saves forming them again for dw_down. */
 #define CL3D_FFN_FLAGS(dtype, order, precision, down) ((dtype) | (order) << 2 | (precision) << 3 | (down) << 4)
 #define CL3D_FFN_BACKWARD 32
 #define CL3D_FFN_DX 1u      /* which gradients: << 6 in the flags */
 #define CL3D_FFN_DW_IN 2u
 #define CL3D_FFN_DW_DOWN 4u
+#define CL3D_FFN_HIDDEN 512 /* flag: `hidden` is given */
+#define CL3D_FFN_FEW 64     /* up to so many points (B N) the weights are read straight into fragments, once */
 int cl3d_gated_ffn_fwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, int dtype, int order, int B, int C,
-                       int N, int H, int activation, int precision, void *y, void *ws, size_t ws_bytes, cl3d_stream_t stream);
+                       int N, int H, int activation, int precision, void *y, void *hidden, void *ws, size_t ws_bytes,
+                       cl3d_stream_t stream);
 /* gradients for dy (shape, type and order of y); dx, dw_gate, dw_up, dw_down: NULL where not wanted.  Products of the two
  * projections are formed again from x.  Weight gradients are summed in a fixed order: bit-identical run to run. */
-int cl3d_gated_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *dy, int dtype,
-                       int order, int B, int C, int N, int H, int activation, int precision, void *dx, void *dw_gate,
+int cl3d_gated_ffn_bwd(const void *x, const void *w_gate, const void *w_up, const void *w_down, const void *dy,
+                       const void *hidden, int dtype, int order, int B, int C, int N, int H, int activation, int precision,
+                       void *dx, void *dw_gate,
                        void *dw_up, void *dw_down, void *ws, size_t ws_bytes, cl3d_stream_t stream);
 
 /* [B,R,C] -> [B,C,R] of 16-bit elements (cl3d_transpose: f32) */
 int cl3d_transpose16(const void *src, int B, int R, int C, void *dst, cl3d_stream_t stream);
 
-/* Exit of a block and entry of the next, one pass over the points (point-major rows [B,N,C]):
+/* Exit of a block and entry of the next, one pass over the points (channel-major tensors: by way of transposed copies in ws):
  *     n = norm(y) weight + bias;  out = residual_scale x + gate * drop(n);  next = next_norm(out) next_weight + next_bias
  * y NULL: there is no block to leave, next = next_norm(x) next_weight + next_bias.  next_kind CL3D_NORM_NONE: no entry.
  * rms: v / sqrt(mean v^2 + eps); layer: (v - mean) / sqrt(var + eps), over the channels of a point.  weight, bias, gate,
@@ -577,15 +583,17 @@ int cl3d_transpose16(const void *src, int B, int R, int C, void *dst, cl3d_strea
  * p, rng: as in cl3d_dropout, element (b, n, c) being number (b N + n) C + c.  stats [B,N,4]: what the backward pass needs of
  * the forward pass, besides its inputs (NULL: no backward pass follows).
  * Backward (x, y and the parameters as in the forward pass, out and next not read): dout, dnext are the gradients of out and next (either may be NULL: zero); dx, dy and the parameters' gradients
- * (shapes and types of what they belong to) NULL where not wanted; ws: cl3d_workspace_bytes(CL3D_OP_POINT_NORM, B, N, 0, 0, C)
- * where a parameter's gradient is.  Sums over the points are taken in a fixed order: bit-identical run to run. */
+ * (shapes and types of what they belong to) NULL where not wanted.  ws, 16-byte aligned: cl3d_workspace_bytes(CL3D_OP_POINT_NORM,
+ * B, N, 0, flags, C), copies being the number of feature tensors that the call is given, sums whether a parameter's gradient is
+ * wanted.  Sums over the points are taken in a fixed order: bit-identical run to run. */
 #define CL3D_NORM_NONE 0
 #define CL3D_NORM_RMS 1
 #define CL3D_NORM_LAYER 2
+#define CL3D_NORM_FLAGS(dtype, order, copies, sums) ((dtype) | (order) << 2 | (copies) << 3 | (sums) << 8)
 typedef struct cl3d_norm_residual {
   int B, N, C, dtype, param_f32, kind, next_kind, gate_cloud;
   float residual_scale, eps, next_eps;
-  int reserved; /* (what would be padding) */
+  int order;
   double p;
   const int64_t *rng;
   const void *x, *y, *weight, *bias, *gate, *next_weight, *next_bias;

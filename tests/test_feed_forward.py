@@ -88,21 +88,23 @@ def test_c_entries_return_codes_and_say_why():
 
     a = 1 << 20  # a 16-byte aligned number
     ffn = lambda *args: lib.cl3d_gated_ffn_fwd(*args)  # noqa: E731
-    refused(ffn(a, a, a, a, 3, 0, 1, 8, 4, 16, 0, 0, a, a, 0, None), -1, "element type")
-    refused(ffn(a, a, a, a, 1, 2, 1, 8, 4, 16, 0, 0, a, a, 0, None), -1, "memory order")
-    refused(ffn(a, a, a, a, 1, 0, 1, 8, 4, 16, 3, 0, a, a, 0, None), -1, "activation")
-    refused(ffn(a, a, a, a, 1, 0, 1, 8, 4, 16, 0, 2, a, a, 0, None), -1, "precision")
-    refused(ffn(a, a, a, a, 1, 0, 1, 0, 4, 16, 0, 0, a, a, 0, None), -1, "bad sizes")
-    refused(ffn(a, a, a, a, 1, 0, 1, 1 << 21, 4, 16, 0, 0, a, a, 0, None), -4, "sizes outside")
-    refused(ffn(None, a, a, a, 1, 0, 1, 8, 4, 16, 0, 0, a, a, 0, None), -1, "null pointer")
-    refused(ffn(a + 2, a, a, a, 1, 0, 1, 8, 4, 16, 0, 0, a, a, 0, None), -1, "16 bytes")
-    refused(ffn(a, a, a, a, 1, 0, 1, 8, 4, 16, 0, 0, a, a, 8, None), -3, "bytes of scratch")
-    assert ffn(None, None, None, None, 1, 0, 0, 8, 4, 16, 0, 0, None, None, 0, None) == 0  # no clouds: nothing to do
+    refused(ffn(a, a, a, a, 3, 0, 1, 8, 4, 16, 0, 0, a, None, a, 0, None), -1, "element type")
+    refused(ffn(a, a, a, a, 1, 2, 1, 8, 4, 16, 0, 0, a, None, a, 0, None), -1, "memory order")
+    refused(ffn(a, a, a, a, 1, 0, 1, 8, 4, 16, 3, 0, a, None, a, 0, None), -1, "activation")
+    refused(ffn(a, a, a, a, 1, 0, 1, 8, 4, 16, 0, 2, a, None, a, 0, None), -1, "precision")
+    refused(ffn(a, a, a, a, 1, 0, 1, 0, 4, 16, 0, 0, a, None, a, 0, None), -1, "bad sizes")
+    refused(ffn(a, a, a, a, 1, 0, 1, 1 << 21, 4, 16, 0, 0, a, None, a, 0, None), -4, "sizes outside")
+    refused(ffn(None, a, a, a, 1, 0, 1, 8, 4, 16, 0, 0, a, None, a, 0, None), -1, "null pointer")
+    refused(ffn(a + 2, a, a, a, 1, 0, 1, 8, 4, 16, 0, 0, a, None, a, 0, None), -1, "16 bytes")
+    refused(ffn(a, a, a, a, 1, 0, 1, 8, 4, 16, 0, 0, a, None, a, 8, None), -3, "bytes of scratch")
+    assert ffn(None, None, None, None, 1, 0, 0, 8, 4, 16, 0, 0, None, None, None, 0, None) == 0  # no clouds: nothing to do
+    refused(ffn(a, a, a, a, 1, 0, 1, 8, 4, 16, 0, 0, a, a, a, 0, None), -1, "no hidden activations")  # few points
+    refused(ffn(a, a, a, None, 1, 0, 1, 8, 400, 16, 0, 0, a, a, a, 0, None), -1, "no hidden activations")  # no last product
     bwd = lambda *args: lib.cl3d_gated_ffn_bwd(*args)  # noqa: E731
-    refused(bwd(a, a, a, None, a, 1, 0, 1, 8, 4, 16, 0, 0, a, a, a, a, a, 0, None), -1, "not there")
-    refused(bwd(a, a, a, a, a, 1, 0, 0, 8, 4, 16, 0, 0, a, a, a, a, a, 0, None), -1, "no points")
-    refused(bwd(a, a, a, a, a, 1, 0, 1, 8, 4, 16, 0, 0, a, a, a, a, a, 0, None), -3, "bytes of scratch")
-    assert bwd(a, a, a, a, a, 1, 0, 1, 8, 4, 16, 0, 0, None, None, None, None, None, 0, None) == 0  # nothing wanted
+    refused(bwd(a, a, a, None, a, None, 1, 0, 1, 8, 4, 16, 0, 0, a, a, a, a, a, 0, None), -1, "not there")
+    refused(bwd(a, a, a, a, a, None, 1, 0, 0, 8, 4, 16, 0, 0, a, a, a, a, a, 0, None), -1, "no points")
+    refused(bwd(a, a, a, a, a, None, 1, 0, 1, 8, 4, 16, 0, 0, a, a, a, a, a, 0, None), -3, "bytes of scratch")
+    assert bwd(a, a, a, a, a, None, 1, 0, 1, 8, 4, 16, 0, 0, None, None, None, None, None, 0, None) == 0  # nothing wanted
 
     norm = lambda p: lib.cl3d_norm_residual_fwd(ctypes.byref(p), None)  # noqa: E731
     assert lib.cl3d_norm_residual_fwd(None, None) == -1
