@@ -41,19 +41,21 @@ inline size_t elem_bytes(int dtype) { return dtype == CL3D_F32 ? 4 : 2; }
 // ---- Philox 4x32 with ten rounds (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011): a
 // bijection of the 128-bit counter under a 64-bit key.  Block b of a draw is the counter (offset + b, 0); element i of a tensor
 // takes word i % 4 of block i / 4, so a mask is a pure function of (seed, offset, element) and is formed again in the backward
-// pass instead of being stored.  Twenty 32 x 32 -> 64 bit products per four elements.
+// pass instead of being stored.  Twenty 32 x 32 -> 64 bit products and as
+// many three-input exclusive ors per four elements.
 struct Words {
   unsigned w[4];
 };
+__device__ __forceinline__ unsigned xor3(unsigned a, unsigned b, unsigned c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
 __device__ __forceinline__ Words philox(unsigned long long counter, unsigned long long seed) {
   unsigned c0 = (unsigned)counter, c1 = (unsigned)(counter >> 32), c2 = 0u, c3 = 0u;
   unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const unsigned long long p0 = (unsigned long long)c0 * 0xD2511F53u, p1 = (unsigned long long)c2 * 0xCD9E8D57u;
-    c0 = (unsigned)(p1 >> 32) ^ c1 ^ k0;
+    c0 = xor3((unsigned)(p1 >> 32), c1, k0);
     c1 = (unsigned)p1;
-    c2 = (unsigned)(p0 >> 32) ^ c3 ^ k1;
+    c2 = xor3((unsigned)(p0 >> 32), c3, k1);
     c3 = (unsigned)p0;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;

@@ -272,35 +272,29 @@ __device__ __forceinline__ void product(f32x4 (&acc)[TI / 16][TJ / 16], const Pa
   barrier_lds();  // (another product may follow in the same tiles)
 }
 
-// ---- activations (CL3D_ACT_SILU / _GELU / _RELU): value and slope at g.  FAST: on the way to a 16-bit result, by the hardware's
-// exp2 and reciprocal (one step each) and the error function by Press et al., Numerical Recipes 6.2 (erfc to 1.2e-7 of itself
-// everywhere, so the tails keep their digits); otherwise by the math library.
-template <bool FAST> __device__ __forceinline__ void activate(int act, float g, float &value, float &slope) {
+// ---- activations (CL3D_ACT_SILU / _GELU / _RELU): value and slope at g.  exp2 and the reciprocal are the hardware's (one step
+// each), the error function is Press et al., Numerical Recipes 6.2: erfc to 1.2e-7 of itself everywhere, so the tails keep their
+// digits.  2 to 3e-7 of the value at |g| <= 10, below what the f32 sum in g carries.
+__device__ __forceinline__ void activate(int act, float g, float &value, float &slope) {
   if (act == CL3D_ACT_SILU) {
-    const float s = FAST ? __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g)) : 1.f / (1.f + expf(-g));
+    const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g));
     value = g * s;
     slope = s * __builtin_fmaf(g, 1.f - s, 1.f);
   } else if (act == CL3D_ACT_GELU) {
-    float c, e;
-    if (FAST) {
-      const float z = 0.70710678118654752f * fabsf(g), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.5f, z, 1.f));
-      float q = 0.17087277f;
-      q = __builtin_fmaf(q, t, -0.82215223f);
-      q = __builtin_fmaf(q, t, 1.48851587f);
-      q = __builtin_fmaf(q, t, -1.13520398f);
-      q = __builtin_fmaf(q, t, 0.27886807f);
-      q = __builtin_fmaf(q, t, -0.18628806f);
-      q = __builtin_fmaf(q, t, 0.09678418f);
-      q = __builtin_fmaf(q, t, 0.37409196f);
-      q = __builtin_fmaf(q, t, 1.00002368f);
-      q = __builtin_fmaf(q, t, -1.26551223f);
-      e = __builtin_amdgcn_exp2f(-1.4426950408889634f * z * z);
-      const float tail = 0.5f * t * e * __builtin_amdgcn_exp2f(1.4426950408889634f * q);
-      c = g < 0.f ? tail : 1.f - tail;
-    } else {
-      c = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-      e = expf(-0.5f * g * g);
-    }
+    const float z = 0.70710678118654752f * fabsf(g), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.5f, z, 1.f));
+    float q = 0.17087277f;
+    q = __builtin_fmaf(q, t, -0.82215223f);
+    q = __builtin_fmaf(q, t, 1.48851587f);
+    q = __builtin_fmaf(q, t, -1.13520398f);
+    q = __builtin_fmaf(q, t, 0.27886807f);
+    q = __builtin_fmaf(q, t, -0.18628806f);
+    q = __builtin_fmaf(q, t, 0.09678418f);
+    q = __builtin_fmaf(q, t, 0.37409196f);
+    q = __builtin_fmaf(q, t, 1.00002368f);
+    q = __builtin_fmaf(q, t, -1.26551223f);
+    const float e = __builtin_amdgcn_exp2f(-1.4426950408889634f * z * z);
+    const float tail = 0.5f * t * e * __builtin_amdgcn_exp2f(1.4426950408889634f * q);
+    const float c = g < 0.f ? tail : 1.f - tail;
     value = g * c;
     slope = __builtin_fmaf(g, 0.3989422804014327f * e, c);
   } else {  // relu; a NaN stays one, the slope at 0 is 0
@@ -452,7 +446,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void ffn_gemm_kernel(GemmArgs a) {
         for (int e = 0; e < 8; ++e) {
           const float gv = acc[2 * b + (e >> 2)][v][e & 3], uv = acc[TI / 32 + 2 * b + (e >> 2)][v][e & 3];
           float val, slope;
-          activate<!std::is_same<T, F32>::value>(a.act, gv, val, slope);
+          activate(a.act, gv, val, slope);
           h[e] = val * uv;
           if constexpr (KIND == GEMM_GATED_BWD) {
             float d = dh[2 * b + (e >> 2)][v][e & 3];
@@ -571,26 +565,41 @@ template <typename T, int V> __global__ __launch_bounds__(256) void ffn_slices_k
 
 // ---- operands that are not what the products read: another memory order, odd rows, f32 ---------------------------------
 // source element (b, r, c) at src + b sb + r sr + c sc, one of sr, sc being 1; out rows [(b, r)] of ld elements, zero behind C.
-// `planes` 3: the split of an f32 value; 1: one rounding to E (none when S is E).
-template <typename S, typename E>
-__global__ __launch_bounds__(256) void ffn_pack_kernel(const typename S::storage *__restrict__ src, long long sb, long long sr,
-                                                       long long sc, int Rb, int C, u16 *__restrict__ dst, int ld, long long plane,
-                                                       int planes) {
+// `planes` 3: the split of an f32 value; 1: one rounding to E (none when S is E).  All operands of a call in one launch: most are
+// weights, and a launch costs more than their copy.
+struct PackJob {
+  const void *src;
+  u16 *dst;
+  long long sb, sr, sc, plane;
+  int Rb, C, ld, tiles_c, tiles;  // tiles of 32 rows x 64 columns: of a batch's columns, of a batch
+  int first;                      // workgroup at which this job begins
+};
+constexpr int kPackJobs = 5;
+struct PackArgs {
+  PackJob job[kPackJobs];
+  int jobs, planes;
+};
+template <typename S, typename E> __global__ __launch_bounds__(256) void ffn_pack_kernel(PackArgs a) {
   __shared__ float tile[32][65];
-  const int b = blockIdx.z, r0 = blockIdx.x * 32, c0 = blockIdx.y * 64;
-  const int tid = threadIdx.x;
-  const typename S::storage *s = src + (long long)b * sb;
+  int which = 0;
+  while (which + 1 < a.jobs && (int)blockIdx.x >= a.job[which + 1].first) ++which;
+  const PackJob &j = a.job[which];
+  int id = blockIdx.x - j.first;
+  const int b = id / j.tiles;
+  id -= b * j.tiles;
+  const int r0 = id / j.tiles_c * 32, c0 = id % j.tiles_c * 64, tid = threadIdx.x;
+  const auto *s = static_cast<const typename S::storage *>(j.src) + (long long)b * j.sb;
   for (int e = tid; e < 32 * 64; e += 256) {
-    const int r = sc == 1 ? e >> 6 : e & 31, c = sc == 1 ? e & 63 : e >> 5;
-    tile[r][c] = r0 + r < Rb && c0 + c < C ? S::get(s[(r0 + r) * sr + (c0 + c) * sc]) : 0.f;
+    const int r = j.sc == 1 ? e >> 6 : e & 31, c = j.sc == 1 ? e & 63 : e >> 5;
+    tile[r][c] = r0 + r < j.Rb && c0 + c < j.C ? S::get(s[(r0 + r) * j.sr + (c0 + c) * j.sc]) : 0.f;
   }
   __syncthreads();
   const int r = tid >> 3, c = (tid & 7) * 8;  // 32 rows x 8 pieces of 8
-  if (r0 + r >= Rb || c0 + c >= ld) return;
+  if (r0 + r >= j.Rb || c0 + c >= j.ld) return;
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = tile[r][c + e];
-  put_internal<E, 8>(dst + ((long long)b * Rb + r0 + r) * ld + c0 + c, plane, planes, v);
+  put_internal<E, 8>(j.dst + ((long long)b * j.Rb + r0 + r) * j.ld + c0 + c, j.plane, a.planes, v);
 }
 
 // ---- few points: the weights are read once, straight into fragments -------------------------------------------------------
@@ -686,7 +695,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void ffn_rows_kernel(RowsArgs a) {
     o[e] = sum[0][e];
     if (GATED) {
       float slope;
-      activate<!std::is_same<T, F32>::value>(a.act, sum[0][e], o[e], slope);
+      activate(a.act, sum[0][e], o[e], slope);
       o[e] *= sum[M - 1][e];
     }
   }
@@ -708,31 +717,36 @@ struct FfnShape {
   bool convert() const { return dtype == CL3D_F32; }
 };
 
-template <typename S, typename E>
-static void pack_launch(const void *src, long long sb, long long sr, long long sc, int B, int Rb, int C, u16 *dst, int ld, long long plane,
-                        int planes, hipStream_t st) {
-  const dim3 grid(ceil_div(Rb, 32), ceil_div(ld, 64), B);
-  hipLaunchKernelGGL((ffn_pack_kernel<S, E>), grid, dim3(256), 0, st, static_cast<const typename S::storage *>(src), sb, sr, sc, Rb, C, dst,
-                     ld, plane, planes);
-}
+// the operands of one call: the caller's own memory where the products can read it, else a packed copy in the launch to come
+struct Operands {
+  const FfnShape &s;
+  Arena &ar;
+  PackArgs a{};
+  long long groups = 0;
+  Operands(const FfnShape &s_, Arena &ar_) : s(s_), ar(ar_) { a.planes = s.split ? 3 : 1; }
 
-// rows [(b, r)][C] as the products read them: the caller's own memory where it is already that, else a packed copy
-static Operand operand(Arena &ar, const FfnShape &s, const void *src, bool channel, int B, int Rb, int C, bool launch, hipStream_t st) {
-  const int ld = (C + 7) & ~7;
-  if (!s.convert() && !channel && C % 8 == 0) return {static_cast<const u16 *>(src), C, 0};
-  const long long plane = (long long)B * Rb * ld;
-  const int planes = s.split ? 3 : 1;
-  u16 *dst = static_cast<u16 *>(ar.take((size_t)plane * planes * 2));
-  if (launch) {
-    // rows that follow each other without regard to the cloud are one batch
-    const int b = channel ? B : 1, rb = channel ? Rb : B * Rb;
-    const long long sb = (long long)C * Rb, sr = channel ? 1 : C, sc = channel ? Rb : 1;
-    if (s.dtype == CL3D_F32) pack_launch<F32, Bf16>(src, sb, sr, sc, b, rb, C, dst, ld, plane, planes, st);
-    else if (s.dtype == CL3D_BF16) pack_launch<Bf16, Bf16>(src, sb, sr, sc, b, rb, C, dst, ld, plane, planes, st);
-    else pack_launch<F16, F16>(src, sb, sr, sc, b, rb, C, dst, ld, plane, planes, st);
+  // rows [(b, r)][C]
+  Operand take(const void *src, bool channel, int B, int Rb, int C) {
+    const int ld = (C + 7) & ~7;
+    if (!s.convert() && !channel && C % 8 == 0) return {static_cast<const u16 *>(src), C, 0};
+    const long long plane = (long long)B * Rb * ld;
+    u16 *dst = static_cast<u16 *>(ar.take((size_t)plane * a.planes * 2));
+    // (rows that follow each other without regard to the cloud are one batch)
+    const int b = channel ? B : 1, rb = channel ? Rb : B * Rb, tiles_c = ceil_div(ld, 64), tiles = tiles_c * ceil_div(rb, 32);
+    a.job[a.jobs++] = {src, dst, (long long)C * Rb, channel ? 1 : C, channel ? Rb : 1, plane, rb, C, ld, tiles_c, tiles, (int)groups};
+    groups += (long long)tiles * b;
+    return {dst, ld, plane};
   }
-  return {dst, ld, plane};
-}
+  int launch(hipStream_t st) {
+    if (a.jobs == 0) return CL3D_OK;
+    if (groups > 0x7fffffffll) return fail(CL3D_E_UNSUPPORTED, "gated_ffn: sizes outside what the kernels index");
+    const dim3 grid((unsigned)groups);
+    if (s.dtype == CL3D_F32) hipLaunchKernelGGL((ffn_pack_kernel<F32, Bf16>), grid, dim3(256), 0, st, a);
+    else if (s.dtype == CL3D_BF16) hipLaunchKernelGGL((ffn_pack_kernel<Bf16, Bf16>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((ffn_pack_kernel<F16, F16>), grid, dim3(256), 0, st, a);
+    return CL3D_OK;
+  }
+};
 
 template <int KIND, typename E, typename T, int NP, int BI, int BJ, int WI, int WJ, int BK, int TILES>
 static int gemm_as(const GemmArgs &a, int batches, hipStream_t st) {
@@ -852,15 +866,18 @@ static int ffn_forward(const FfnShape &s, const void *x, const void *wg, const v
     ffn_forward_rows(s, s.channel() ? xr : x, wg, wu, wd, yr, h, st);
     return s.channel() ? transposed(s.dtype, yr, s.B, s.N, out, y, st) : CL3D_OK;
   }
-  const Operand X = operand(ar, s, x, s.channel(), s.B, s.N, s.C, launch, st);
-  const Operand G = operand(ar, s, wg, false, 1, s.H, s.C, launch, st), U = operand(ar, s, wu, false, 1, s.H, s.C, launch, st);
+  Operands ops(s, ar);
+  const Operand X = ops.take(x, s.channel(), s.B, s.N, s.C);
+  const Operand G = ops.take(wg, false, 1, s.H, s.C), U = ops.take(wu, false, 1, s.H, s.C);
   Operand D, h;
   if (s.down) {
-    D = operand(ar, s, wd, false, 1, s.C, s.H, launch, st);
+    D = ops.take(wd, false, 1, s.C, s.H);
     h = {static_cast<u16 *>(hidden ? hidden : ar.take((size_t)R * hp * 2 * (s.split ? 3 : 1))), hp, (long long)R * hp};
   }
   void *rows = s.channel() ? ar.take((size_t)R * out * elem_bytes(s.dtype)) : y;
   if (!launch) return CL3D_OK;
+  int rc = ops.launch(st);
+  if (rc != CL3D_OK) return rc;
   GemmArgs a = gemm_args(s);
   a.P = G.p; a.P2 = U.p; a.Q = X.p;
   a.plane_p = G.plane; a.plane_q = X.plane;  // (wg and wu: one shape, one plane stride)
@@ -871,7 +888,7 @@ static int ffn_forward(const FfnShape &s, const void *x, const void *wg, const v
   } else {
     a.D = rows; a.ldd = s.H; a.vec = row_vec(s, rows, s.H);
   }
-  int rc = gemm<GEMM_GATED>(s, a, 1, st);
+  rc = gemm<GEMM_GATED>(s, a, 1, st);
   if (rc != CL3D_OK) return rc;
   if (s.down) {
     a = gemm_args(s);
@@ -890,13 +907,14 @@ static int ffn_backward(const FfnShape &s, const void *x, const void *wg, const 
                         const void *hidden, void *dx, void *dwg, void *dwu, void *dwd, unsigned wants, Arena &ar, bool launch, hipStream_t st) {
   const int R = (int)s.R(), hp = (s.H + 7) & ~7, planes = s.split ? 3 : 1;
   const bool want_x = wants & CL3D_FFN_DX, want_gu = wants & CL3D_FFN_DW_IN, want_d = s.down && (wants & CL3D_FFN_DW_DOWN);
-  const Operand X = operand(ar, s, x, s.channel(), s.B, s.N, s.C, launch, st);
-  const Operand G = operand(ar, s, wg, false, 1, s.H, s.C, launch, st), U = operand(ar, s, wu, false, 1, s.H, s.C, launch, st);
+  Operands ops(s, ar);
+  const Operand X = ops.take(x, s.channel(), s.B, s.N, s.C);
+  const Operand G = ops.take(wg, false, 1, s.H, s.C), U = ops.take(wu, false, 1, s.H, s.C);
   Operand D, dY, h;
   const void *dh_rows = dy;
   if (s.down) {
-    D = operand(ar, s, wd, false, 1, s.C, s.H, launch, st);
-    dY = operand(ar, s, dy, s.channel(), s.B, s.N, s.C, launch, st);
+    D = ops.take(wd, false, 1, s.C, s.H);
+    dY = ops.take(dy, s.channel(), s.B, s.N, s.C);
     if (want_d) h = {static_cast<const u16 *>(hidden ? hidden : ar.take((size_t)R * hp * 2 * planes)), hp, (long long)R * hp};
   } else if (s.channel()) {
     void *t = ar.take((size_t)R * s.H * elem_bytes(s.dtype));
@@ -913,7 +931,8 @@ static int ffn_backward(const FfnShape &s, const void *x, const void *wg, const 
   float *part_in = want_gu ? static_cast<float *>(ar.take((size_t)2 * slices_in * s.H * s.C * 4)) : nullptr;
   float *part_d = want_d ? static_cast<float *>(ar.take((size_t)slices_d * s.H * s.C * 4)) : nullptr;
   if (!launch) return CL3D_OK;
-
+  int rc = ops.launch(st);
+  if (rc != CL3D_OK) return rc;
   GemmArgs a = gemm_args(s);
   a.P = G.p; a.P2 = U.p; a.Q = X.p;
   a.plane_p = G.plane; a.plane_q = X.plane;
@@ -929,7 +948,7 @@ static int ffn_backward(const FfnShape &s, const void *x, const void *wg, const 
     a.dh = dh_rows; a.lddh = s.H;
   }
   a.dgu = dgu; a.plane_dgu = (long long)R * 2 * hp; a.ldh = hp;
-  int rc = gemm<GEMM_GATED_BWD>(s, a, 1, st);
+  rc = gemm<GEMM_GATED_BWD>(s, a, 1, st);
   if (rc != CL3D_OK) return rc;
   if (want_x) {
     a = gemm_args(s);

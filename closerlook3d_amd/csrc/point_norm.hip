@@ -30,8 +30,25 @@ struct NormArgs {
   int has_drop;
 };
 
-template <typename T> __device__ __forceinline__ float param(const void *p, long long i, int f32) {
-  return f32 ? static_cast<const float *>(p)[i] : T::get(static_cast<const typename T::storage *>(p)[i]);
+// V parameters from number i on, `none` where there are none; a workgroup loads them once
+template <typename T, int V> __device__ __forceinline__ void params(const void *p, long long i, int f32, float none, float *v) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = none;
+  } else if (V == 1) {
+    v[0] = f32 ? static_cast<const float *>(p)[i] : T::get(static_cast<const typename T::storage *>(p)[i]);
+  } else if (f32) {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+      const f32x4 t = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + i + 4 * q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * q + e] = t[e];
+    }
+  } else {
+    const auto t = *reinterpret_cast<const Vec16<T> *>(static_cast<const typename T::storage *>(p) + i);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = T::get(t.v[e % T::kVec]);
+  }
 }
 
 // v + v of the lane that the DPP control names (within 16 lanes)
@@ -100,55 +117,50 @@ template <typename T, int V> struct Raw {
   }
 };
 
-// 1 / (1 - p) or 0 for the V elements from `at` on (V > 1: at is a multiple of 4)
-template <int V> __device__ __forceinline__ void keep_v(const Drop &d, unsigned long long seed, unsigned long long offset, long long at, float *m) {
-  if (d.all) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) m[e] = 0.f;
-    return;
-  }
+// which of the V elements from `at` on stay (V > 1: at is a multiple of 4)
+template <int V> __device__ __forceinline__ void stay_v(const Drop &d, unsigned long long seed, unsigned long long offset, long long at, bool *m) {
   if constexpr (V == 1) {
     const Words w = philox(offset + (unsigned long long)(at >> 2), seed);
     const int e = (int)(at & 3);
     const unsigned word = e < 2 ? (e ? w.w[1] : w.w[0]) : (e == 2 ? w.w[2] : w.w[3]);
-    m[0] = word >= d.threshold ? d.scale : 0.f;
+    m[0] = !d.all && word >= d.threshold;
   } else {
 #pragma unroll
     for (int q = 0; q < V / 4; ++q) {
       const Words w = philox(offset + (unsigned long long)((at >> 2) + q), seed);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) m[4 * q + e] = w.w[e] >= d.threshold ? d.scale : 0.f;
+      for (int e = 0; e < 4; ++e) m[4 * q + e] = !d.all && w.w[e] >= d.threshold;
     }
   }
 }
 
-// mean and reciprocal deviation of a row held as v[NV][V]; `on`: which pieces exist
+// mean and reciprocal deviation of a row held as v[NV][V]; `on`: which pieces exist (the others hold zeros)
 template <int TPR, int NV, int V>
-__device__ __forceinline__ void row_stats(const float (&v)[NV][V], const bool (&on)[NV], int kind, float eps, int C, float *s_red, float &mean,
-                                          float &rinv) {
-  const float inv_c = 1.f / (float)C;
+__device__ __forceinline__ void row_stats(const float (&v)[NV][V], const bool (&on)[NV], int kind, float eps, float inv_c, float *s_red,
+                                          float &mean, float &rinv) {
   mean = 0.f;
   if (kind == CL3D_NORM_LAYER) {
     float a = 0.f, none = 0.f;
 #pragma unroll
     for (int q = 0; q < NV; ++q)
-      if (on[q])
 #pragma unroll
-        for (int e = 0; e < V; ++e) a += v[q][e];
+      for (int e = 0; e < V; ++e) a += v[q][e];
     row_sum<TPR>(a, none, s_red);
     mean = a * inv_c;
   }
   float a = 0.f, none = 0.f;
 #pragma unroll
-  for (int q = 0; q < NV; ++q)
-    if (on[q])
+  for (int q = 0; q < NV; ++q) {
+    float t = 0.f;
 #pragma unroll
-      for (int e = 0; e < V; ++e) a = __builtin_fmaf(v[q][e] - mean, v[q][e] - mean, a);
+    for (int e = 0; e < V; ++e) t = __builtin_fmaf(v[q][e] - mean, v[q][e] - mean, t);
+    a += on[q] ? t : 0.f;
+  }
   row_sum<TPR>(a, none, s_red);
   rinv = 1.f / sqrtf(a * inv_c + eps);
 }
 
-template <typename T, int TPR, int NV, int V>
+template <typename T, int TPR, int NV, int V, bool DROP>
 __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
   __shared__ float s_red[8];
   const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
@@ -156,6 +168,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
   const long long first = (long long)b * a.N + (long long)chunk * a.per;
   long long last = first + a.per, end = (long long)(b + 1) * a.N;
   if (last > end) last = end;
+  const float inv_c = 1.f / (float)a.C;
   bool on[NV];
   int col[NV];
   float w1[NV][V], b1[NV][V], gate[NV][V], w2[NV][V], b2[NV][V];
@@ -163,18 +176,15 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
   for (int q = 0; q < NV; ++q) {
     col[q] = (q * TPR + lane) * V;
     on[q] = col[q] < a.C;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int c = on[q] ? col[q] + e : 0;
-      w1[q][e] = a.w1 ? param<T>(a.w1, c, a.param_f32) : 1.f;
-      b1[q][e] = a.b1 ? param<T>(a.b1, c, a.param_f32) : 0.f;
-      gate[q][e] = a.gate ? param<T>(a.gate, a.gate_cloud ? (long long)b * a.C + c : c, a.param_f32) : 1.f;
-      w2[q][e] = a.w2 ? param<T>(a.w2, c, a.param_f32) : 1.f;
-      b2[q][e] = a.b2 ? param<T>(a.b2, c, a.param_f32) : 0.f;
-    }
+    const int c = on[q] ? col[q] : 0;
+    params<T, V>(a.w1, c, a.param_f32, 1.f, w1[q]);
+    params<T, V>(a.b1, c, a.param_f32, 0.f, b1[q]);
+    params<T, V>(a.gate, (a.gate_cloud ? (long long)b * a.C : 0) + c, a.param_f32, 1.f, gate[q]);
+    params<T, V>(a.w2, c, a.param_f32, 1.f, w2[q]);
+    params<T, V>(a.b2, c, a.param_f32, 0.f, b2[q]);
   }
   unsigned long long seed = 0, offset = 0;
-  if (a.has_drop) { seed = a.drop.state[0]; offset = a.drop.state[1]; }
+  if (DROP) { seed = a.drop.state[0]; offset = a.drop.state[1]; }
   // every lane walks the same number of rows (row_sum's barriers): a group behind the last row works on the last one, unstored.
   // The next rows are on their way while these are worked on: a wave's time is the latency of its row, and few rows fit a CU
   constexpr int kStep = 256 / TPR;
@@ -192,49 +202,56 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a) {
   for (long long r0 = first; r0 < last; r0 += kStep) {
     const bool live = r0 + group < last;
     const long long r = live ? r0 + group : last - 1;
+    // (a lane without a piece works on zeros: the arithmetic below runs in all lanes, the memory does not)
     float v[NV][V], y[NV][V];
 #pragma unroll
-    for (int q = 0; q < NV; ++q)
+    for (int q = 0; q < NV; ++q) {
       if (on[q]) {
         nx[q].get(v[q]);
         if (a.exit) ny[q].get(y[q]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[q][e] = y[q][e] = 0.f;
       }
+    }
     if (r0 + kStep < last) fetch(r0 + kStep + group);
     if (a.exit) {
       float mean = 0.f, rinv = 1.f;
-      if (a.kind1 != CL3D_NORM_NONE) row_stats<TPR, NV, V>(y, on, a.kind1, a.eps1, a.C, s_red, mean, rinv);
+      if (a.kind1 != CL3D_NORM_NONE) row_stats<TPR, NV, V>(y, on, a.kind1, a.eps1, inv_c, s_red, mean, rinv);
       if (a.stats && live && lane == 0) *reinterpret_cast<float2 *>(a.stats + 4 * r) = make_float2(mean, rinv);
 #pragma unroll
       for (int q = 0; q < NV; ++q) {
-        if (!on[q]) continue;
-        float m[V];
-        if (a.has_drop) keep_v<V>(a.drop, seed, offset, r * a.C + col[q], m);
+        bool m[V];
+        if (DROP) stay_v<V>(a.drop, seed, offset, r * a.C + col[q], m);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           float n = __builtin_fmaf((y[q][e] - mean) * rinv, w1[q][e], b1[q][e]);
-          if (a.has_drop) n = m[e] == 0.f ? 0.f : n * m[e];
+          if (DROP) n = m[e] ? n * a.drop.scale : 0.f;
           v[q][e] = __builtin_fmaf(a.alpha, v[q][e], gate[q][e] * n);
         }
-        if (live) store_v<T, V>(a.o, r * a.C + col[q], v[q]);
+        if (live && on[q]) store_v<T, V>(a.o, r * a.C + col[q], v[q]);
+        if (!on[q]) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[q][e] = 0.f;
+        }
       }
     }
     if (a.next) {
       float mean = 0.f, rinv = 1.f;
-      row_stats<TPR, NV, V>(v, on, a.kind2, a.eps2, a.C, s_red, mean, rinv);
+      row_stats<TPR, NV, V>(v, on, a.kind2, a.eps2, inv_c, s_red, mean, rinv);
       if (a.stats && live && lane == 0) *reinterpret_cast<float2 *>(a.stats + 4 * r + 2) = make_float2(mean, rinv);
 #pragma unroll
       for (int q = 0; q < NV; ++q) {
-        if (!on[q]) continue;
 #pragma unroll
         for (int e = 0; e < V; ++e) v[q][e] = __builtin_fmaf((v[q][e] - mean) * rinv, w2[q][e], b2[q][e]);
-        if (live) store_v<T, V>(a.h, r * a.C + col[q], v[q]);
+        if (live && on[q]) store_v<T, V>(a.h, r * a.C + col[q], v[q]);
       }
     }
   }
 }
 
 // d of norm: dhat -> d = rinv (dhat - hat mean(dhat hat) - [layer] mean(dhat))
-template <typename T, int TPR, int NV, int V>
+template <typename T, int TPR, int NV, int V, bool DROP, bool BIAS>
 __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
   __shared__ float s_red[8];
   __shared__ float s_sum[TPR < 256 ? 256 / TPR : 1][TPR < 256 ? TPR * NV * V : 1];
@@ -252,18 +269,18 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
   for (int q = 0; q < NV; ++q) {
     col[q] = (q * TPR + lane) * V;
     on[q] = col[q] < a.C;
+    const int c = on[q] ? col[q] : 0;
+    params<T, V>(a.w1, c, a.param_f32, 1.f, w1[q]);
+    params<T, V>(BIAS ? a.b1 : nullptr, c, a.param_f32, 0.f, b1[q]);
+    params<T, V>(a.gate, (a.gate_cloud ? (long long)b * a.C : 0) + c, a.param_f32, 1.f, gate[q]);
+    params<T, V>(a.w2, c, a.param_f32, 1.f, w2[q]);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int c = on[q] ? col[q] + e : 0;
-      w1[q][e] = a.w1 ? param<T>(a.w1, c, a.param_f32) : 1.f;
-      b1[q][e] = a.b1 ? param<T>(a.b1, c, a.param_f32) : 0.f;
-      gate[q][e] = a.gate ? param<T>(a.gate, a.gate_cloud ? (long long)b * a.C + c : c, a.param_f32) : 1.f;
-      w2[q][e] = a.w2 ? param<T>(a.w2, c, a.param_f32) : 1.f;
       s_w1[q][e] = s_b1[q][e] = s_gate[q][e] = s_w2[q][e] = s_b2[q][e] = 0.f;
     }
   }
   unsigned long long seed = 0, offset = 0;
-  if (a.has_drop) { seed = a.drop.state[0]; offset = a.drop.state[1]; }
+  if (DROP) { seed = a.drop.state[0]; offset = a.drop.state[1]; }
   constexpr int kStep = 256 / TPR;
   Raw<T, V> nx[NV], ny[NV], nd[NV], nh[NV];
   f32x4 ns;
@@ -286,31 +303,35 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
     const bool live = r0 + group < last;
     const long long r = live ? r0 + group : last - 1;
     const f32x4 st = ns;
-    float hat1[NV][V], keep[NV][V], d[NV][V], hat[NV][V], dh[NV][V];
+    // a lane without a piece works on zeros, a group behind the last row on zero gradients: only memory is guarded below
+    float hat1[NV][V], d[NV][V], hat[NV][V], dh[NV][V];
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) d[q][e] = 0.f;
-      if (!on[q]) continue;
-      if (a.exit) ny[q].get(hat1[q]);
-      if (a.dout) nd[q].get(d[q]);
-      if (a.dnext) {
-        nx[q].get(hat[q]);
-        nh[q].get(dh[q]);
+      for (int e = 0; e < V; ++e) hat1[q][e] = d[q][e] = hat[q][e] = dh[q][e] = 0.f;
+      if (on[q]) {
+        if (a.exit) ny[q].get(hat1[q]);
+        if (a.dnext) nx[q].get(hat[q]);
+        if (live) {
+          if (a.dout) nd[q].get(d[q]);
+          if (a.dnext) nh[q].get(dh[q]);
+        }
       }
     }
     if (r0 + kStep < last) fetch(r0 + kStep + group);
     // the exit once more, from x and y: out as the forward pass had it before it was rounded costs no more traffic than the
-    // rounded one, and the y hats are needed below anyway.  keep: 1 / (1 - p) or 0; hat1, n: of y
+    // rounded one, and the y hats are needed below anyway.  nk: what was left of the norm of y
+    bool stays[NV][V];
+    float nk[NV][V];
     if (a.exit) {
 #pragma unroll
       for (int q = 0; q < NV; ++q) {
-        if (!on[q]) continue;
-        if (a.has_drop) keep_v<V>(a.drop, seed, offset, r * a.C + col[q], keep[q]);
+        if (DROP) stay_v<V>(a.drop, seed, offset, r * a.C + col[q], stays[q]);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           hat1[q][e] = (hat1[q][e] - st[0]) * st[1];
-          if (!a.has_drop) keep[q][e] = 1.f;
+          nk[q][e] = __builtin_fmaf(hat1[q][e], w1[q][e], b1[q][e]);
+          if (DROP) nk[q][e] = stays[q][e] ? nk[q][e] * a.drop.scale : 0.f;
         }
       }
     }
@@ -318,31 +339,27 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
       float p1 = 0.f, p2 = 0.f;
 #pragma unroll
       for (int q = 0; q < NV; ++q) {
-        if (!on[q]) continue;
+        float t1 = 0.f, t2 = 0.f;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          if (a.exit) {
-            const float n = keep[q][e] == 0.f ? 0.f : __builtin_fmaf(hat1[q][e], w1[q][e], b1[q][e]) * keep[q][e];
-            hat[q][e] = __builtin_fmaf(a.alpha, hat[q][e], gate[q][e] * n);
-          }
+          if (a.exit) hat[q][e] = __builtin_fmaf(a.alpha, hat[q][e], gate[q][e] * nk[q][e]);
           hat[q][e] = (hat[q][e] - st[2]) * st[3];
-          if (live) {
-            s_w2[q][e] = __builtin_fmaf(dh[q][e], hat[q][e], s_w2[q][e]);
-            s_b2[q][e] += dh[q][e];
-          }
+          s_w2[q][e] = __builtin_fmaf(dh[q][e], hat[q][e], s_w2[q][e]);
+          if (BIAS) s_b2[q][e] += dh[q][e];
           dh[q][e] *= w2[q][e];
-          p1 = __builtin_fmaf(dh[q][e], hat[q][e], p1);
-          p2 += dh[q][e];
+          t1 = __builtin_fmaf(dh[q][e], hat[q][e], t1);
+          t2 += dh[q][e];
         }
+        p1 += on[q] ? t1 : 0.f;
+        p2 += on[q] ? t2 : 0.f;
       }
       row_sum<TPR>(p1, p2, s_red);
       p1 *= inv_c;
       p2 = a.kind2 == CL3D_NORM_LAYER ? p2 * inv_c : 0.f;
 #pragma unroll
       for (int q = 0; q < NV; ++q)
-        if (on[q])
 #pragma unroll
-          for (int e = 0; e < V; ++e) d[q][e] += st[3] * (dh[q][e] - __builtin_fmaf(hat[q][e], p1, p2));
+        for (int e = 0; e < V; ++e) d[q][e] = __builtin_fmaf(st[3], dh[q][e] - __builtin_fmaf(hat[q][e], p1, p2), d[q][e]);
     }
     if (a.dx && live) {
 #pragma unroll
@@ -358,22 +375,22 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
       float p1 = 0.f, p2 = 0.f;
 #pragma unroll
       for (int q = 0; q < NV; ++q) {
-        if (!on[q]) continue;
+        float t1 = 0.f, t2 = 0.f;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          float dm = keep[q][e] == 0.f ? 0.f : d[q][e] * keep[q][e];
-          if (live && keep[q][e] != 0.f)  // (a dropped element: n is not looked at)
-            s_gate[q][e] = __builtin_fmaf(dm, __builtin_fmaf(hat1[q][e], w1[q][e], b1[q][e]), s_gate[q][e]);
+          float dm = live ? d[q][e] : 0.f;
+          s_gate[q][e] = __builtin_fmaf(dm, nk[q][e], s_gate[q][e]);
+          if (DROP) dm = stays[q][e] ? dm * a.drop.scale : 0.f;
           dm *= gate[q][e];
-          if (live) {
-            s_w1[q][e] = __builtin_fmaf(dm, hat1[q][e], s_w1[q][e]);
-            s_b1[q][e] += dm;
-          }
+          s_w1[q][e] = __builtin_fmaf(dm, hat1[q][e], s_w1[q][e]);
+          if (BIAS) s_b1[q][e] += dm;
           dm *= w1[q][e];
-          p1 = __builtin_fmaf(dm, hat1[q][e], p1);
-          p2 += dm;
+          t1 = __builtin_fmaf(dm, hat1[q][e], t1);
+          t2 += dm;
           d[q][e] = dm;
         }
+        p1 += on[q] ? t1 : 0.f;
+        p2 += on[q] ? t2 : 0.f;
       }
       if (a.dy) {
         if (a.kind1 != CL3D_NORM_NONE) {
@@ -422,11 +439,11 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
   };
   if (a.exit) {
     if (a.w1) flush(s_w1, 0);
-    if (a.b1) flush(s_b1, 1);
+    if (BIAS && a.b1) flush(s_b1, 1);
     if (a.gate) flush(s_gate, 2);
   }
   if (a.w2) flush(s_w2, 3);
-  if (a.b2) flush(s_b2, 4);
+  if (BIAS && a.b2) flush(s_b2, 4);
 }
 
 // sums of the partial rows [row][which][C]: 16 columns a workgroup, 64 runs of rows side by side, joined in order
@@ -460,9 +477,9 @@ __global__ __launch_bounds__(1024) void norm_sums_kernel(NormSums a) {
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------
-constexpr int kNormMaxC = 8192;
+constexpr int kNormMaxC = 4096;
 
-// workgroups of a cloud and rows of each: about 8 workgroups a CU forward, 4 backward (each leaves a partial row behind)
+// workgroups of a cloud and rows of each
 static void norm_grid(NormArgs &a, int rows_per_pass, int target) {
   long long want = ((long long)target + a.B - 1) / a.B;
   const long long passes = (a.N + rows_per_pass - 1) / rows_per_pass;
@@ -487,15 +504,23 @@ static NormMap norm_map(int dtype, int C, bool aligned) {
   if (v > 1 && pieces <= 32) return {32, 1, v};
   if (pieces <= 64) return {64, 1, v};
   if (need <= 2) return {256, need, v};
-  if (need <= 4) return {256, 4, v};
-  if (v == 1) return {256, need <= 10 ? 10 : 32, v};
-  return {256, 8, v};
+  if (v > 1 || need <= 4) return {256, 4, v};
+  return {256, need <= 10 ? 10 : 16, v};
 }
 
 template <typename T, int TPR, int NV, int V> static void norm_run(bool backward, const NormArgs &a, hipStream_t st) {
   const dim3 grid((unsigned)((long long)a.B * a.chunks));
-  if (backward) hipLaunchKernelGGL((norm_bwd_kernel<T, TPR, NV, V>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((norm_fwd_kernel<T, TPR, NV, V>), grid, dim3(256), 0, st, a);
+  const bool bias = V == 1 || a.b1 || a.b2;  // (single elements: one variant)
+  if (!backward) {
+    if (a.has_drop) hipLaunchKernelGGL((norm_fwd_kernel<T, TPR, NV, V, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((norm_fwd_kernel<T, TPR, NV, V, false>), grid, dim3(256), 0, st, a);
+  } else if (bias) {
+    if (a.has_drop) hipLaunchKernelGGL((norm_bwd_kernel<T, TPR, NV, V, true, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((norm_bwd_kernel<T, TPR, NV, V, false, true>), grid, dim3(256), 0, st, a);
+  } else if constexpr (V > 1) {
+    if (a.has_drop) hipLaunchKernelGGL((norm_bwd_kernel<T, TPR, NV, V, true, false>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((norm_bwd_kernel<T, TPR, NV, V, false, false>), grid, dim3(256), 0, st, a);
+  }
 }
 template <typename T> static void norm_pick(const NormMap &m, bool backward, const NormArgs &a, hipStream_t st) {
   constexpr int V = T::kVec;
@@ -505,15 +530,14 @@ template <typename T> static void norm_pick(const NormMap &m, bool backward, con
     if (m.nv == 2) return norm_run<T, 256, 2, 1>(backward, a, st);
     if (m.nv == 4) return norm_run<T, 256, 4, 1>(backward, a, st);
     if (m.nv == 10) return norm_run<T, 256, 10, 1>(backward, a, st);
-    return norm_run<T, 256, 32, 1>(backward, a, st);
+    return norm_run<T, 256, 16, 1>(backward, a, st);
   }
   if (m.tpr == 16) return norm_run<T, 16, 1, V>(backward, a, st);
   if (m.tpr == 32) return norm_run<T, 32, 1, V>(backward, a, st);
   if (m.tpr == 64) return norm_run<T, 64, 1, V>(backward, a, st);
   if (m.nv == 1) return norm_run<T, 256, 1, V>(backward, a, st);
   if (m.nv == 2) return norm_run<T, 256, 2, V>(backward, a, st);
-  if (m.nv == 4) return norm_run<T, 256, 4, V>(backward, a, st);
-  if constexpr (V == 4) norm_run<T, 256, 8, V>(backward, a, st);
+  if constexpr (V == 4) norm_run<T, 256, 4, V>(backward, a, st);  // (16-bit: two pieces hold kNormMaxC)
 }
 static void norm_launch(int dtype, const NormMap &m, bool backward, const NormArgs &a, hipStream_t st) {
   if (dtype == CL3D_F32) norm_pick<F32>(m, backward, a, st);
@@ -550,7 +574,13 @@ static void norm_args(NormArgs &a, const cl3d_norm_residual *p) {
   a.has_drop = p->p > 0.0;
 }
 
-constexpr int kNormBwdGroups = 1024;
+// workgroups: as many as are resident with the registers of the 16-bit variants (four a CU forward, three backward); more would
+// load their parameters again, one round too few leaves CUs idle (backward 81 920 x 288: 512 156 us, 768 125, 1024 167)
+constexpr int kNormFwdGroups = 1024, kNormBwdGroups = 768;
+
+static bool params_aligned(const cl3d_norm_residual *p) {
+  return aligned16(p->weight) && aligned16(p->bias) && aligned16(p->gate) && aligned16(p->next_weight) && aligned16(p->next_bias);
+}
 
 // point-major copies of channel-major tensors, and back
 struct NormCopies {
@@ -605,8 +635,8 @@ extern "C" int cl3d_norm_residual_fwd(const cl3d_norm_residual *p, cl3d_stream_t
   a.x = c.in(p->x); a.y = c.in(p->y);
   a.o = c.out(p->out); a.h = c.out(p->next);
   if (c.rc != CL3D_OK) return c.rc;
-  const NormMap m = norm_map(p->dtype, p->C, aligned16(a.x) && aligned16(a.y) && aligned16(a.o) && aligned16(a.h));
-  norm_grid(a, 256 / m.tpr, 2048);
+  const NormMap m = norm_map(p->dtype, p->C, aligned16(a.x) && aligned16(a.y) && aligned16(a.o) && aligned16(a.h) && params_aligned(p));
+  norm_grid(a, 256 / m.tpr, kNormFwdGroups);
   norm_launch(p->dtype, m, false, a, st);
   c.back(a.o, p->out), c.back(a.h, p->next);
   return c.rc != CL3D_OK ? c.rc : check_launch("cl3d_norm_residual_fwd");
@@ -629,8 +659,8 @@ extern "C" int cl3d_norm_residual_bwd(const cl3d_norm_residual *p, cl3d_stream_t
   const void *x = p->dnext ? p->x : nullptr;  // (without the entry's gradient x is not looked at)
   NormCopies need(p, nullptr, st), c(p, p->ws, st);
   need.in(x), need.in(p->y), need.in(p->dout), need.in(p->dnext), need.out(p->dx), need.out(p->dy);
-  const NormMap m = norm_map(p->dtype, p->C, need.copies || (aligned16(x) && aligned16(p->y) && aligned16(p->dout) && aligned16(p->dnext) &&
-                                                             aligned16(p->dx) && aligned16(p->dy)));
+  const NormMap m = norm_map(p->dtype, p->C, params_aligned(p) && (need.copies || (aligned16(x) && aligned16(p->y) && aligned16(p->dout) && aligned16(p->dnext) &&
+                                                             aligned16(p->dx) && aligned16(p->dy))));
   norm_grid(a, 256 / m.tpr, kNormBwdGroups);
   const size_t partial_bytes = sums ? (size_t)a.B * a.chunks * 5 * a.C * sizeof(float) : 0;
   if (sums) need.ar.take(partial_bytes);

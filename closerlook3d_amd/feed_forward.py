@@ -34,7 +34,7 @@ _ACTIVATIONS = {'silu': 0, 'gelu': 1, 'relu': 2}
 _NORMS = {'none': 0, 'rms': 1, 'layer': 2}
 _PRECISIONS = {'f32': 0, 'bf16': 1}
 _OP_GATED_FFN, _OP_POINT_NORM = 17, 18
-_MAX_NORM_CHANNELS = 8192
+_MAX_NORM_CHANNELS = 4096
 
 
 def _p(t):

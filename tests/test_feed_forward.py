@@ -49,7 +49,7 @@ def fake(*shape, dtype=torch.float32):
     (lambda: ff.point_norm(fake(4, 8), kind='none'), ValueError, "a norm is one of"),
     (lambda: ff.point_norm(fake(4, 8), eps=-1.0), ValueError, "eps"),
     (lambda: ff.point_norm(fake(4, 8), eps=float('nan')), ValueError, "eps"),
-    (lambda: ff.point_norm(fake(4, 8193)), ValueError, "channels"),
+    (lambda: ff.point_norm(fake(4, 4097)), ValueError, "channels"),
     (lambda: ff.point_norm(fake(4, 8), fake(7)), ValueError, "weight has the shape"),
     (lambda: ff.point_norm(fake(4, 8), fake(8, dtype=torch.float16)), TypeError, "weight is torch.float16"),
     (lambda: ff.norm_gate_residual(fake(4, 8), fake(4, 9)), ValueError, "one shape"),
@@ -113,7 +113,7 @@ def test_c_entries_return_codes_and_say_why():
     refused(norm(_block(kind=3, x=a, y=a, out=a)), -1, "unknown norm")
     refused(norm(_block(x=a)), -1, "neither a block")
     refused(norm(_block(x=a, next_kind=1, gate=a, next=a)), -1, "not there")
-    refused(norm(_block(C=8193, x=a, y=a, out=a)), -4, "channels")
+    refused(norm(_block(C=4097, x=a, y=a, out=a)), -4, "channels")
     refused(norm(_block(p=0.5, x=a, y=a, out=a)), -1, "generator state")
     refused(norm(_block(p=-0.5, rng=a, x=a, y=a, out=a)), -1, "probability")
     refused(norm(_block(x=a, y=a)), -1, "null pointer")
