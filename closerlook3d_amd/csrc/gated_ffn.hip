@@ -702,6 +702,155 @@ __global__ __launch_bounds__(64 * kRowsWaves) void ffn_rows_kernel(RowsArgs a) {
   put_row<T, 4>(static_cast<S *>(a.D) + (long long)j * a.ldd + c0, a.I - c0, a.vec_out, o);
 }
 
+// ---- narrow points, many of them: the whole forward pass in one kernel -----------------------------------------------------------
+// Up to 224 channels a wave keeps its 16 NJ points in registers -- their x as fragments, their y as accumulators -- and the workgroup
+// walks the hidden channels, 32 at a time: G and U of a chunk, h = act(G) U, y += Wd h.  The accumulators of G and U are laid out so
+// that a lane's eight values of h (channels 8 g .. 8 g + 7 of one point) are what the last product wants as its second operand, so h
+// passes from one product to the next without leaving the lane.  Only the weights travel: a chunk's rows of Wg and Wu and columns
+// of Wd, by way of LDS, the next chunk in flight; x is read and y written once, h is written only if the caller keeps it.
+// CF: 32-channel fragments of x, odd (a row of 64 CF bytes then starts at a quarter of its own of the 64 banks).
+// Measured against the two kernels it replaces (us, bf16): 65 536 x 144 x 576 60 (83), 131 072 x 72 x 288 41 (63), 32 768 x 144 x
+// 576 39 (42), 65 536 x 200 x 800 91 (121); 16 384 x 144 x 576 37 (25): below 32 768 points there are fewer than 256 workgroups of
+// 128, one for each CU.  Bound: per chunk a wave waits for its weights, reads each fragment for one or two products and then is in
+// the activation; the two workgroups of a CU cover each other's waits in part.
+constexpr int kFusedMostC = 224, kFusedFewest = 32768;
+struct FusedArgs {
+  const u16 *G, *U, *D, *X;  // G, U: rows of ldw, D: rows of ldd, X: rows of ldx
+  void *Y;
+  u16 *h;                    // nullable: rows of hp
+  int J, C, H, hp, ldw, ldd, ldx, ldy, act, vec;
+};
+template <typename E, typename T, int CF, int NJ, int NW>
+__global__ __launch_bounds__(64 * NW) void ffn_fused_kernel(FusedArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  constexpr int kPart = 2048 * CF, kTile = 3 * kPart;  // 32 rows of 64 CF bytes; 32 CF rows of 64 bytes
+  constexpr int kAll = 6 * CF, kPer = (kAll + NW - 1) / NW;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, m = lane & 15, cp = (a.C + 7) & ~7;
+  const int j0 = (xcd_order(blockIdx.x, gridDim.x) * NW + wave) * NJ * 16;
+
+  unsigned off[kPer];
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    const int n0 = wave * kPer + q, n = n0 < kAll ? n0 : n0 - kAll, part = n / (2 * CF), slot = (n - part * 2 * CF) * 64 + lane;
+    if (part < 2) {
+      const int row = slot / (4 * CF), piece = slot - row * 4 * CF, chunk = (piece & ~3) | ((piece & 3) ^ ((row >> 3) & 3));
+      off[q] = chunk * 8 < cp ? (unsigned)(row * a.ldw + chunk * 8) * 2u : 0x80000000u;
+    } else {
+      const int row = slot >> 2, chunk = (slot & 3) ^ ((row >> 3) & 3);
+      off[q] = (unsigned)(row * a.ldd + chunk * 8) * 2u;
+    }
+  }
+  auto issue = [&](int h0, int place) {
+    const int rows = a.H - h0 < 32 ? a.H - h0 : 32, cols = a.hp - h0 < 32 ? a.hp - h0 : 32;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+      const int n0 = wave * kPer + q, n = n0 < kAll ? n0 : n0 - kAll, part = n / (2 * CF);
+      const u16 *base = part == 0 ? a.G + (long long)h0 * a.ldw : part == 1 ? a.U + (long long)h0 * a.ldw : a.D + h0;
+      const unsigned bytes = part < 2 ? (unsigned)((rows - 1) * a.ldw + cp) * 2u : (unsigned)((a.C - 1) * a.ldd + cols) * 2u;
+      unsigned o = off[q];
+      if (part == 2 && cols < 32) {  // the last columns of Wd: what follows them in memory is the next row
+        const int slot = (n - 4 * CF) * 64 + lane, chunk = (slot & 3) ^ (((slot >> 2) >> 3) & 3);
+        o = chunk * 8 < cols ? o : 0x80000000u;
+      }
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, bytes, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, CL3D_LDS(void, smem + place * kTile + n * 1024), 16, o, 0, 0, 0);
+    }
+  };
+  issue(0, 0);
+
+  s16x8 x[CF][NJ];
+#pragma unroll
+  for (int t = 0; t < NJ; ++t) {
+    const int j = j0 + t * 16 + m;
+    const u16 *row = a.X + (long long)(j < a.J ? j : a.J - 1) * a.ldx;
+#pragma unroll
+    for (int kk = 0; kk < CF; ++kk) {
+      const int k = kk * 32 + 8 * g;
+      x[kk][t] = k < cp ? *reinterpret_cast<const s16x8 *>(row + k) : (s16x8){0, 0, 0, 0, 0, 0, 0, 0};
+    }
+  }
+  f32x4 y[2 * CF][NJ];
+#pragma unroll
+  for (int u = 0; u < 2 * CF; ++u)
+#pragma unroll
+    for (int t = 0; t < NJ; ++t) y[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+  f32x4 s[4][NJ];
+  auto project = [&](const char *lds) {  // G and U of a chunk
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int t = 0; t < NJ; ++t) s[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < CF; ++kk) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {  // gate, gate, up, up
+        const int row = 8 * (m >> 2) + 4 * (u & 1) + (m & 3);
+        const s16x8 p = *reinterpret_cast<const s16x8 *>(lds + (u >> 1) * kPart + row * (64 * CF) + ((kk * 4 + (g ^ ((row >> 3) & 3))) << 4));
+#pragma unroll
+        for (int t = 0; t < NJ; ++t) s[u][t] = mfma16<E>(p, x[kk][t], s[u][t]);
+      }
+    }
+  };
+  auto finish = [&](const char *lds, int h0) {  // h of the chunk, and what it adds to y
+    s16x8 h[NJ];
+#pragma unroll
+    for (int t = 0; t < NJ; ++t) {
+      u16 o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float v, slope;
+        activate(a.act, s[e >> 2][t][e & 3], v, slope);
+        o[e] = E::put(v * s[2 + (e >> 2)][t][e & 3]);
+      }
+      if (h0 + 32 > a.H) {  // behind the last channel: zero, whatever 0 x inf made
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (h0 + 8 * g + e >= a.H) o[e] = 0;
+      }
+      h[t] = *reinterpret_cast<s16x8 *>(o);
+      const int j = j0 + t * 16 + m;
+      if (a.h != nullptr && j < a.J && h0 + 8 * g < a.hp) *reinterpret_cast<s16x8 *>(a.h + (long long)j * a.hp + h0 + 8 * g) = h[t];
+    }
+#pragma unroll
+    for (int u = 0; u < 2 * CF; ++u) {
+      const int row = (u >> 1) * 32 + 8 * (m >> 2) + 4 * (u & 1) + (m & 3);
+      const s16x8 p = *reinterpret_cast<const s16x8 *>(lds + 2 * kPart + row * 64 + ((g ^ ((row >> 3) & 3)) << 4));
+#pragma unroll
+      for (int t = 0; t < NJ; ++t) y[u][t] = mfma16<E>(p, h[t], y[u][t]);
+    }
+  };
+  int place = 0;
+  // a chunk's weights are older than the NJ stores of the chunk before, if every lane made them: those need not be waited for
+  const bool all_store = a.h != nullptr && j0 + NJ * 16 <= a.J;
+  for (int h0 = 0; h0 < a.hp; h0 += 32) {
+    if (all_store && h0 > 0) wait_vm<NJ>();  // (the chunk before was a whole one)
+    else wait_vm<0>();
+    barrier_lds();
+    if (h0 + 32 < a.hp) issue(h0 + 32, place ^ 1);
+    const char *lds = smem + place * kTile;
+    place ^= 1;
+    project(lds);
+    finish(lds, h0);
+  }
+  auto *Y = static_cast<typename T::storage *>(a.Y);
+#pragma unroll
+  for (int t = 0; t < NJ; ++t) {
+    const int j = j0 + t * 16 + m;
+    if (j >= a.J) continue;
+#pragma unroll
+    for (int b = 0; b < CF; ++b) {
+      const int c0 = b * 32 + 8 * g;
+      if (c0 >= a.C) continue;
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = y[2 * b + (e >> 2)][t][e & 3];
+      put_row<T, 8>(Y + (long long)j * a.ldy + c0, a.C - c0, a.vec, o);
+    }
+  }
+}
+
 // ---- host side -----------------------------------------------------------------------------------------------------
 struct Operand {
   const u16 *p = nullptr;
@@ -852,6 +1001,32 @@ static void ffn_forward_rows(const FfnShape &s, const void *x, const void *wg, c
   if (s.down) rows<false>(s.dtype, {wd, nullptr, h, y, s.C, R, s.H, s.H, hp, s.C, s.act, s.C % quad == 0}, st);
 }
 
+template <typename E, typename T, int CF, int NJ, int NW> static int fused_as(const FusedArgs &a, hipStream_t st) {
+  const auto kernel = ffn_fused_kernel<E, T, CF, NJ, NW>;
+  constexpr int kLds = 2 * 3 * 2048 * CF;
+  static std::atomic<unsigned long long> granted{0};
+  if (kLds > 65536) {
+    const int rc = lds_opt_in(granted, reinterpret_cast<const void *>(kernel), kLds, "gated_ffn");
+    if (rc != CL3D_OK) return rc;
+  }
+  hipLaunchKernelGGL(kernel, dim3(ceil_div(a.J, NW * NJ * 16)), dim3(64 * NW), kLds, st, a);
+  return CL3D_OK;
+}
+// Eight waves of 16 points: two workgroups a CU (65 536 x 144: 60 us; of 32 points, one a CU: 59, but 53 against 39 at half the
+// points).  At 7 fragments only one fits either way, and 32 points read each weight half as often (65 536 x 200: 91, 125).
+template <typename E, typename T, int CF> static int fused_width(const FusedArgs &a, hipStream_t st) {
+  if constexpr (CF == 7)
+    if (a.J >= 65536) return fused_as<E, T, CF, 2, 8>(a, st);
+  return fused_as<E, T, CF, 1, 8>(a, st);
+}
+template <typename E, typename T> static int fused(const FusedArgs &a, hipStream_t st) {
+  const int cf = (a.C + 31) / 32;
+  if (cf <= 1) return fused_width<E, T, 1>(a, st);
+  if (cf <= 3) return fused_width<E, T, 3>(a, st);
+  if (cf <= 5) return fused_width<E, T, 5>(a, st);
+  return fused_width<E, T, 7>(a, st);
+}
+
 // x in the layout of `s`, its rows of C
 static int ffn_forward(const FfnShape &s, const void *x, const void *wg, const void *wu, const void *wd, void *y, void *hidden, Arena &ar,
                        bool launch, hipStream_t st) {
@@ -870,14 +1045,23 @@ static int ffn_forward(const FfnShape &s, const void *x, const void *wg, const v
   const Operand X = ops.take(x, s.channel(), s.B, s.N, s.C);
   const Operand G = ops.take(wg, false, 1, s.H, s.C), U = ops.take(wu, false, 1, s.H, s.C);
   Operand D, h;
+  const bool whole = s.down && !s.split && s.C <= kFusedMostC && R >= kFusedFewest;
   if (s.down) {
     D = ops.take(wd, false, 1, s.C, s.H);
-    h = {static_cast<u16 *>(hidden ? hidden : ar.take((size_t)R * hp * 2 * (s.split ? 3 : 1))), hp, (long long)R * hp};
+    if (!whole) h = {static_cast<u16 *>(hidden ? hidden : ar.take((size_t)R * hp * 2 * (s.split ? 3 : 1))), hp, (long long)R * hp};
   }
   void *rows = s.channel() ? ar.take((size_t)R * out * elem_bytes(s.dtype)) : y;
   if (!launch) return CL3D_OK;
   int rc = ops.launch(st);
   if (rc != CL3D_OK) return rc;
+  if (whole) {
+    const FusedArgs f{G.p, U.p, D.p, X.p, rows, static_cast<u16 *>(hidden), R, s.C, s.H, hp, G.ld, D.ld, X.ld, s.C, s.act, row_vec(s, rows, s.C)};
+    if (s.dtype == CL3D_F32) rc = fused<Bf16, F32>(f, st);
+    else if (s.dtype == CL3D_BF16) rc = fused<Bf16, Bf16>(f, st);
+    else rc = fused<F16, F16>(f, st);
+    if (rc != CL3D_OK) return rc;
+    return s.channel() ? transposed(s.dtype, rows, s.B, s.N, out, y, st) : CL3D_OK;
+  }
   GemmArgs a = gemm_args(s);
   a.P = G.p; a.P2 = U.p; a.Q = X.p;
   a.plane_p = G.plane; a.plane_q = X.plane;  // (wg and wu: one shape, one plane stride)

@@ -67,6 +67,19 @@ def test_feed_forward_matches_its_formula(size, kind):
     ffn_check(x, ws, ["silu", "gelu", "relu"][(C + N) % 3], dtype, features(g, B, C, N, dtype, order), order, tag=(size, kind))
 
 
+# many narrow points: the forward pass in one kernel, at the widths and point counts where it changes its shape
+@pytest.mark.parametrize("size", [(1, 24, 32768, 40), (1, 33, 32775, 47), (2, 144, 16385, 96), (1, 160, 33000, 33), (1, 72, 65537, 64),
+                                  (1, 200, 32769, 100), (1, 224, 65540, 70), (1, 217, 65536, 31), (1, 225, 32768, 32)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_feed_forward_of_many_narrow_points(size):
+    B, C, N, H = size
+    for kind, precision in (("bf16", "f32"), ("f16", "f32"), ("f32", "bf16")):
+        dtype, g = TYPES[kind], gen(16)
+        order = "channel" if C % 3 == 0 and kind != "f16" else "point"
+        x, ws = ffn_inputs(g, B, C, N, H, dtype, order)
+        ffn_check(x, ws, "gelu" if C % 2 else "silu", dtype, features(g, B, C, N, dtype, order), order, precision, tag=(size, kind))
+
+
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
 def test_gated_projections_without_the_last_product(kind, act):
@@ -175,7 +188,7 @@ def test_what_is_not_finite_stays_in_its_point(kind):
     """A NaN or an infinity reaches its own point only, and of the weights' gradients what the formula says; the infinity of an f32
     value stays one (its split is not inf - inf)."""
     dtype, g = TYPES[kind], gen(7)
-    for R, C, H in ((40, 24, 40), (300, 21, 35)):
+    for R, C, H in ((40, 24, 40), (300, 21, 35), (32800, 40, 45)):
         x, ws = ffn_inputs(g, 1, C, R, H, dtype)
         x = x.transpose(1, 2)[0].contiguous()
         clean = ff.gated_feed_forward(x, *ws)
