@@ -8,6 +8,7 @@ Layout (only what the hot path needs):
   pt_utils.py                   the reference's grouping API (MaskedQueryAndGroup, ...)
   local_aggregation_operators   LocalAggregation / PosPool / AdaptiveWeight / PointWiseMLP / PseudoGrid
   fused.py                      fused-operator entry points
+  feed_forward.py               gated feed-forward, norms around a block, dropout from a counter
   backbones.py                  ResNet / Bottleneck / SceneSegHeadResNet callers (integration, bench)
   dp.py                         one-process-per-GPU sharding + RCCL gradient all-reduce
 """

@@ -42,9 +42,13 @@ template <> __device__ __forceinline__ f32x4 mfma16<F16>(s16x8 a, s16x8 b, f32x4
 
 #define CL3D_LDS(T, p) ((__attribute__((address_space(3))) T *)(p))
 
-// s_waitcnt vmcnt(n), the other counters left alone
+// s_waitcnt vmcnt(n), the other counters left alone; no memory operation moves across it (the count is of those issued before)
 template <int N> __device__ __forceinline__ void wait_vm() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
   __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
 }
 __device__ __forceinline__ void barrier_lds() {
   asm volatile("" ::: "memory");
@@ -589,9 +593,16 @@ template <typename S, typename E> __global__ __launch_bounds__(256) void ffn_pac
   id -= b * j.tiles;
   const int r0 = id / j.tiles_c * 32, c0 = id % j.tiles_c * 64, tid = threadIdx.x;
   const auto *s = static_cast<const typename S::storage *>(j.src) + (long long)b * j.sb;
-  for (int e = tid; e < 32 * 64; e += 256) {
-    const int r = j.sc == 1 ? e >> 6 : e & 31, c = j.sc == 1 ? e & 63 : e >> 5;
-    tile[r][c] = r0 + r < j.Rb && c0 + c < j.C ? S::get(s[(r0 + r) * j.sr + (c0 + c) * j.sc]) : 0.f;
+  float in[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {  // (all eight on their way before the first is put down)
+    const int e = q * 256 + tid, r = j.sc == 1 ? e >> 6 : e & 31, c = j.sc == 1 ? e & 63 : e >> 5;
+    in[q] = r0 + r < j.Rb && c0 + c < j.C ? S::get(s[(r0 + r) * j.sr + (c0 + c) * j.sc]) : 0.f;
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const int e = q * 256 + tid;
+    tile[j.sc == 1 ? e >> 6 : e & 31][j.sc == 1 ? e & 63 : e >> 5] = in[q];
   }
   __syncthreads();
   const int r = tid >> 3, c = (tid & 7) * 8;  // 32 rows x 8 pieces of 8
@@ -640,7 +651,7 @@ constexpr int kRowsWaves = 8, kRowsMost = CL3D_FFN_FEW;  // points of a call tha
 template <bool GATED, typename T, int JT, bool VEC>
 __global__ __launch_bounds__(64 * kRowsWaves) void ffn_rows_kernel(RowsArgs a) {
   using S = typename T::storage;
-  constexpr int M = GATED ? 2 : 1, U = JT == 1 ? 8 : 4, V = T::kVec;
+  constexpr int M = GATED ? 2 : 1, U = JT == 4 ? 2 : 4, V = T::kVec;
   __shared__ f32x4 s_acc[kRowsWaves][M][JT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
   const int i0 = blockIdx.x * 16;
@@ -655,23 +666,35 @@ __global__ __launch_bounds__(64 * kRowsWaves) void ffn_rows_kernel(RowsArgs a) {
 #pragma unroll
     for (int m = 0; m < M; ++m) acc[m][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  for (int k0 = wave * U * 4 * V; k0 < a.K; k0 += kRowsWaves * U * 4 * V) {
-    Piece<T, VEC> p[U], p2[GATED ? U : 1], q[JT][U];
+  // two sets of pieces: one on its way while the other is multiplied
+  Piece<T, VEC> p[2][U], p2[2][GATED ? U : 1], q[2][JT][U];
+  constexpr int kTurn = kRowsWaves * U * 4 * V;
+  auto fetch = [&](int set, int k0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = k0 + (u * 4 + g) * V;
-      p[u].load(P, k, a.K);
-      if (GATED) p2[u].load(P2, k, a.K);
+      p[set][u].load(P, k, a.K);
+      if (GATED) p2[set][u].load(P2, k, a.K);
 #pragma unroll
-      for (int t = 0; t < JT; ++t) q[t][u].load(Q[t], k, a.K);
+      for (int t = 0; t < JT; ++t) q[set][t][u].load(Q[t], k, a.K);
     }
+  };
+  auto multiply = [&](int set) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int t = 0; t < JT; ++t) {
-        acc[0][t] = mul_piece<T, VEC>(p[u], q[t][u], acc[0][t]);
-        if (GATED) acc[M - 1][t] = mul_piece<T, VEC>(p2[u], q[t][u], acc[M - 1][t]);
+        acc[0][t] = mul_piece<T, VEC>(p[set][u], q[set][t][u], acc[0][t]);
+        if (GATED) acc[M - 1][t] = mul_piece<T, VEC>(p2[set][u], q[set][t][u], acc[M - 1][t]);
       }
+  };
+  const int k0 = wave * U * 4 * V;
+  if (k0 < a.K) fetch(0, k0);
+  for (int k = k0; k < a.K; k += 2 * kTurn) {
+    if (k + kTurn < a.K) fetch(1, k + kTurn);
+    multiply(0);
+    if (k + 2 * kTurn < a.K) fetch(0, k + 2 * kTurn);
+    if (k + kTurn < a.K) multiply(1);
   }
 #pragma unroll
   for (int m = 0; m < M; ++m)
@@ -912,21 +935,25 @@ static int gemm_as(const GemmArgs &a, int batches, hipStream_t st) {
   return CL3D_OK;
 }
 
+static bool pads_less_by_96(int I) { return ceil_div(I, 96) * 96 < ceil_div(I, 128) * 128; }
+
 // The tile of a product.  Measured at 16 384 x 288 x 1152 in bf16 and 16 384 x 144 x 576 in f32 (us):
 //   * dX and Y: rows of tiles of 96 results where they pad the width less than 128 do (widths 144, 288, 576 fit 96), 64 points a
 //     tile, so that three workgroups share a CU and 768 of them come out even: dX 34 (96 x 128: 39, 128 x 128: 42), Y 22 (23, 24);
-//     split: 96 x 128 by eight waves 62, 27 (128 x 128: 67, 30);
+//     split: dX in 64 x 64, three workgroups a CU, 50 (96 x 128 by eight waves: 62), Y in 96 x 128 26 (64 x 64: 29, 128 x 128: 30);
 //   * projections, forward and backward: 64 channels of both x 128 points by eight waves, 43 and 73 (four waves: 50, 86); split:
 //     64 points by four waves, two workgroups a CU: 70, 119 (128 points: 72, 131);
-//   * weight gradients: 128 x 128 by eight waves, 34 (four: 39).
+//   * weight gradients: 128 x 128 (or 96) by eight waves, 34 (32; four waves: 39); split: 64 x 128, two workgroups a CU, 43 (58).
 // Two tiles of k in LDS: a third one costs a workgroup of the CU (dX 44 -> 64).
 template <int KIND, typename E, typename T, int NP> static int gemm_tile(const GemmArgs &a, int batches, hipStream_t st) {
-  const bool by96 = ceil_div(a.I, 96) * 96 < ceil_div(a.I, 128) * 128;
+  [[maybe_unused]] const bool by96 = pads_less_by_96(a.I);
   if constexpr (KIND == GEMM_NT || KIND == GEMM_NN) {
-    if constexpr (NP == 3) return by96 ? gemm_as<KIND, E, T, 3, 96, 128, 2, 4, 32, 2>(a, batches, st) : gemm_as<KIND, E, T, 3, 128, 128, 2, 4, 32, 2>(a, batches, st);
+    if constexpr (NP == 3 && KIND == GEMM_NN) return gemm_as<KIND, E, T, 3, 64, 64, 2, 2, 32, 2>(a, batches, st);
+    else if constexpr (NP == 3) return by96 ? gemm_as<KIND, E, T, 3, 96, 128, 2, 4, 32, 2>(a, batches, st) : gemm_as<KIND, E, T, 3, 128, 128, 2, 4, 32, 2>(a, batches, st);
     else return by96 ? gemm_as<KIND, E, T, 1, 96, 64, 2, 2, 64, 2>(a, batches, st) : gemm_as<KIND, E, T, 1, 128, 64, 2, 2, 64, 2>(a, batches, st);
   } else if constexpr (KIND == GEMM_TN) {
-    return gemm_as<KIND, E, T, NP, 128, 128, 2, 4, NP == 1 ? 64 : 32, 2>(a, batches, st);
+    if constexpr (NP == 3) return gemm_as<KIND, E, T, 3, 64, 128, 2, 4, 32, 2>(a, batches, st);
+    else return by96 ? gemm_as<KIND, E, T, 1, 96, 128, 2, 4, 64, 2>(a, batches, st) : gemm_as<KIND, E, T, 1, 128, 128, 2, 4, 64, 2>(a, batches, st);
   } else {
     if constexpr (NP == 3) return gemm_as<KIND, E, T, 3, 128, 64, 2, 2, 32, 2>(a, batches, st);
     else return gemm_as<KIND, E, T, 1, 128, 128, 2, 4, 64, 2>(a, batches, st);
@@ -943,13 +970,13 @@ template <int KIND> static int gemm(const FfnShape &s, const GemmArgs &a, int ba
 
 static bool row_vec(const FfnShape &s, const void *D, int ldd) { return aligned16(D) && ldd % (s.dtype == CL3D_F32 ? 4 : 8) == 0; }
 
-// pieces of k in a weight gradient: as many workgroups as the chip holds at once (two on a CU, split products one), not one more
+// pieces of k in a weight gradient: as many workgroups as the chip holds at once (two on a CU), not one more
 // -- a few workgroups of a second round would take as long as the whole first one (540 on 512 places: 49 us, 486: 30) --, four
 // tiles of k in each at least
 static int weight_slices(const FfnShape &s, int I, int J, int batches) {
-  const long long tiles = (long long)ceil_div(I, 128) * ceil_div(J, 128) * batches;
+  const long long tiles = (long long)ceil_div(I, s.split ? 64 : pads_less_by_96(I) ? 96 : 128) * ceil_div(J, 128) * batches;
   const long long steps = (s.R() + 63) / 64;
-  long long n = (s.split ? 256 : 512) / tiles;
+  long long n = 512 / tiles;
   if (n > steps / 4) n = steps / 4;
   return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
 }

@@ -627,6 +627,7 @@ extern "C" int cl3d_norm_residual_fwd(const cl3d_norm_residual *p, cl3d_stream_t
   if (rc != CL3D_OK) return rc;
   if (p->B == 0 || p->N == 0) return CL3D_OK;
   CL3D_REQUIRE(p->x && (!a.exit || p->out) && (!a.next || p->next), "norm_residual_fwd: null pointer");
+  CL3D_REQUIRE(aligned16(p->stats) && aligned16(p->ws), "norm_residual_fwd: stats and scratch start on 16 bytes");
   const hipStream_t st = (hipStream_t)stream;
   NormCopies need(p, nullptr, st), c(p, p->ws, st);
   need.in(p->x), need.in(p->y), need.out(p->out), need.out(p->next);
@@ -666,7 +667,7 @@ extern "C" int cl3d_norm_residual_bwd(const cl3d_norm_residual *p, cl3d_stream_t
   if (sums) need.ar.take(partial_bytes);
   if (need.ar.used && (!p->ws || p->ws_bytes < need.ar.used))
     return fail(CL3D_E_WORKSPACE, "norm_residual_bwd: %zu bytes of scratch, %zu needed", p->ws_bytes, need.ar.used);
-  CL3D_REQUIRE(aligned16(p->ws), "norm_residual_bwd: scratch starts on 16 bytes");
+  CL3D_REQUIRE(aligned16(p->stats) && aligned16(p->ws), "norm_residual_bwd: stats and scratch start on 16 bytes");
   a.x = c.in(x); a.y = c.in(p->y); a.dout = c.in(p->dout); a.dnext = c.in(p->dnext);
   a.dx = c.out(p->dx); a.dy = c.out(p->dy);
   if (sums) a.partial = static_cast<float *>(c.ar.take(partial_bytes));

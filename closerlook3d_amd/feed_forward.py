@@ -62,6 +62,8 @@ def _check_param(t, shape, x, who, name, optional=True, f32=True):
         if optional:
             return
         raise TypeError(f"{who}: {name} is missing")
+    if isinstance(t, torch.Tensor) and t.shape == shape and t.dtype == x.dtype and t.device == x.device:
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{who}: {name} is a tensor, got {type(t).__name__}")
     if tuple(t.shape) != tuple(shape):
@@ -301,9 +303,13 @@ def _norm_forward(x, y, weight, bias, gate, next_weight, next_bias, rng, opts, n
     x, order = _order(x)
     y = None if y is None else _as_order(y, order)
     params = (weight, bias, gate, next_weight, next_bias)
-    f32 = any(t is not None and t.dtype == torch.float32 for t in params)
-    # (one type for all of them: a mixture goes to f32)
-    held = [None if t is None else (t.float() if f32 else t).contiguous() for t in params]
+    held, f32 = [], False
+    for t in params:
+        f32 = f32 or (t is not None and t.dtype == torch.float32)
+    for t in params:  # (one type for all of them: a mixture goes to f32)
+        if t is not None:
+            t = (t if not f32 or t.dtype == torch.float32 else t.float()).contiguous()
+        held.append(t)
     out = _empty(shape, order, dtype, device) if y is not None else None
     nxt = _empty(shape, order, dtype, device) if next_kind else None
     stats = torch.empty((B * N, 4), dtype=torch.float32, device=device) if need_grad else None
@@ -521,7 +527,8 @@ class _Draws:
 
 
 class CounterDropout(nn.Module):
-    """nn.Dropout by dropout(): no mask in memory.  Every call in training mode is a draw of its own."""
+    """nn.Dropout by dropout(): no mask in memory.  Every call in training mode is a draw of its own; the generator's state is not
+    part of the state dict."""
 
     def __init__(self, p=0.5, seed=None):
         super().__init__()
@@ -559,7 +566,8 @@ class FeedForwardBlock(nn.Module):
     """features -> residual_scale * features + gate * dropout(post_norm(gated_feed_forward(pre_norm(features)))).
 
     pre_norm and post_norm: 'rms', 'layer', or for post_norm 'none' (the default).  gate: a learned number per channel, from
-    `gate_init`; None: none.  (B, C, N) features in either memory order; the result is channel-major when they are."""
+    `gate_init`; None: none.  (B, C, N) features in either memory order, of the parameters' type; the result is channel-major when
+    they are.  The state of the dropout's generator is not part of the state dict."""
 
     def __init__(self, channels, hidden, activation='silu', pre_norm='rms', post_norm='none', eps=1e-6, gate_init=1.0,
                  residual_scale=1.0, dropout=0.0, precision='f32', seed=None):

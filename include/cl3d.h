@@ -580,12 +580,13 @@ int cl3d_transpose16(const void *src, int B, int R, int C, void *dst, cl3d_strea
  * y NULL: there is no block to leave, next = next_norm(x) next_weight + next_bias.  next_kind CL3D_NORM_NONE: no entry.
  * rms: v / sqrt(mean v^2 + eps); layer: (v - mean) / sqrt(var + eps), over the channels of a point.  weight, bias, gate,
  * next_weight, next_bias: [C] (gate [B,C] with gate_cloud), NULL: 1, 0, 1, 1, 0; of the tensors' type, or f32 with param_f32.
- * p, rng: as in cl3d_dropout, element (b, n, c) being number (b N + n) C + c.  stats [B,N,4]: what the backward pass needs of
- * the forward pass, besides its inputs (NULL: no backward pass follows).
- * Backward (x, y and the parameters as in the forward pass, out and next not read): dout, dnext are the gradients of out and next (either may be NULL: zero); dx, dy and the parameters' gradients
- * (shapes and types of what they belong to) NULL where not wanted.  ws, 16-byte aligned: cl3d_workspace_bytes(CL3D_OP_POINT_NORM,
- * B, N, 0, flags, C), copies being the number of feature tensors that the call is given, sums whether a parameter's gradient is
- * wanted.  Sums over the points are taken in a fixed order: bit-identical run to run. */
+ * p, rng: as in cl3d_dropout, element (b, n, c) being number (b N + n) C + c.  stats [B,N,4], 16-byte aligned: what the
+ * backward pass needs of the forward pass, besides its inputs (NULL: no backward pass follows).
+ * Backward (x, y and the parameters as in the forward pass, out and next not read): dout, dnext are the gradients of out and
+ * next (either may be NULL: zero); dx, dy and the parameters' gradients (shapes and types of what they belong to) NULL where not
+ * wanted.  ws, 16-byte aligned: cl3d_workspace_bytes(CL3D_OP_POINT_NORM, B, N, 0, flags, C), copies being the number of feature
+ * tensors that the call is given, sums whether a parameter's gradient is wanted.  Sums over the points are taken in a fixed
+ * order: bit-identical run to run. */
 #define CL3D_NORM_NONE 0
 #define CL3D_NORM_RMS 1
 #define CL3D_NORM_LAYER 2

@@ -118,6 +118,7 @@ def test_c_entries_return_codes_and_say_why():
     refused(norm(_block(p=-0.5, rng=a, x=a, y=a, out=a)), -1, "probability")
     refused(norm(_block(x=a, y=a)), -1, "null pointer")
     refused(norm(_block(B=70000, gate_cloud=1, gate=a, x=a, y=a, out=a)), -4, "65535 clouds")
+    refused(norm(_block(x=a, y=a, out=a, stats=a + 8)), -1, "16 bytes")
     nb = lambda p: lib.cl3d_norm_residual_bwd(ctypes.byref(p), None)  # noqa: E731
     refused(nb(_block(x=a, y=a, stats=a)), -1, "null pointer")
     refused(nb(_block(x=a, y=a, stats=a, dnext=a)), -1, "was not formed")
