@@ -5,9 +5,9 @@
 //     dh = dY Wd;  dG = dh U act'(G);  dU = dh act(G);   dX = dG Wg + dU Wu;   dWg = dG^T X, dWu = dU^T X, dWd = dY^T h
 // Three products of 2 R C H operations forward and six backward.  G and U never reach memory: the forward kernel keeps both
 // accumulators of an element in one lane and writes h, the backward kernel forms G, U and dh together (two products more) and
-// writes dG, dU (h is kept from the forward pass where the caller has room for it, or formed again).  Against storing G and U that is 8 R H bytes less traffic for 4 R C H operations more -- at 5.1 TB/s and
-// 1.28 PFLOP/s (a large copy, a large product) it pays below C = 500 -- and dG, dU come from f32 values of G, U, dh: one
-// rounding in front of the last products instead of two.
+// writes dG, dU (h is kept from the forward pass where the caller has room for it, or formed again).  Against storing G and U that
+// is 8 R H bytes less traffic for 4 R C H operations more -- at 5.1 TB/s and 1.28 PFLOP/s (a large copy, a large product) it pays
+// below C = 500 -- and dG, dU come from f32 values of G, U, dh: one rounding in front of the last products instead of two.
 //
 // One kernel template.  D[j][i] = sum_k P(i, k) Q(j, k), i contiguous in the result; P is the first MFMA operand, so a lane of
 // v_mfma_f32_16x16x32 holds four consecutive i of one j.
@@ -16,8 +16,6 @@
 //   * two LDS tiles of 64 k each (projections: 32): the next one is in flight while this one is multiplied; a third tile would cost
 //     a workgroup of the CU, and what bounds these short sums is what one workgroup cannot overlap with itself: its start, its
 //     barriers, its stores (of the backward twin's 68 us, 27 are left without any product, 50 without the stores).
-// Measured at 16 384 x 288 x 1152 in bf16: projections 37 us (590 TFLOP/s), their backward twin 68 (480), Y 19 (570), dX 35 (620),
-// the three weight gradients 61 (535); 16 384 x 144 x 576 in f32, counting f32 operations: 66 (82), 107 (76), 27 (100), 53 (103), 81 (100).
 //   * an operand whose k is contiguous lies in LDS as [row][64 k], 16-byte pieces XORed with the row, read by ds_read_b128; one
 //     whose row index is contiguous (Wd in dh, Wg / Wu in dX, all operands of the weight gradients) lies as [64 k][row] and is
 //     read by ds_read_b64_tr_b16, which hands a lane four k of its row: no operand is transposed in memory;
@@ -27,6 +25,8 @@
 // left out is below 2^-23 of |x||y|, as much as the rounding of an f32 product.  Six passes at the bf16 rate outrun the f32 MFMA
 // (1/16 of it).  A tile holds the three planes of 32 k, so each fragment is read once for its two or three products.  A value
 // that is not finite takes part in the product of the leading planes only, so an infinity stays one (not_finite below).
+// Measured at 16 384 x 288 x 1152 in bf16: projections 37 us (590 TFLOP/s), their backward twin 68 (480), Y 19 (570), dX 35 (620),
+// the three weight gradients 61 (535); 16 384 x 144 x 576 in f32, counting f32 operations: 66 (82), 107 (76), 27 (100), 53 (103), 81 (100).
 #include "ff_common.h"
 #include <type_traits>
 

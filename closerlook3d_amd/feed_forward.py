@@ -155,11 +155,13 @@ class _Reorder(Function):
     @staticmethod
     def forward(ctx, x, order):
         ctx.back = _order(x)[1]
+        _track(ctx, x)
         return _as_order(x, order).view_as(x)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
+        _check_capture(ctx, g.device)
         return _as_order(g, ctx.back), None
 
 
@@ -511,24 +513,28 @@ class CounterRng:
 
 # ---------------------------------------------------------------------------------------------------------- modules
 class _Draws:
-    """A module's generator: made on the device of its first input, from `seed` or, when that is None, from torch's CPU generator."""
+    """A module's generators, one for each device it has seen, made on the first input there: from `seed` or, when that is None,
+    from torch's CPU generator."""
 
     def __init__(self, seed):
-        self.seed, self.rng = seed, None
+        self.seed, self.rng, self.rngs = seed, None, {}  # rng: that of the last draw
 
     def take(self, x):
-        if self.rng is None or self.rng.state.device != x.device:
-            if torch.cuda.is_current_stream_capturing():
+        rng = self.rngs.get(x.device)
+        if rng is None:
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("dropout: run the module once before its step is captured (its generator is made on first use)")
             if self.seed is None:
                 self.seed = int(torch.randint(0, 2 ** 62, (1,)).item())
-            self.rng = CounterRng(self.seed, x.device)
-        return self.rng.take(x.numel())
+            rng = self.rngs[x.device] = CounterRng(self.seed, x.device)
+        self.rng = rng
+        return rng.take(x.numel())
 
 
 class CounterDropout(nn.Module):
-    """nn.Dropout by dropout(): no mask in memory.  Every call in training mode is a draw of its own; the generator's state is not
-    part of the state dict."""
+    """nn.Dropout by dropout(): no mask in memory.  Every call in training mode is a draw of its own, also one that activation
+    checkpointing makes a second time (draw outside of what is run twice and call dropout() there).  The generator's state is not part
+    of the state dict."""
 
     def __init__(self, p=0.5, seed=None):
         super().__init__()
@@ -567,7 +573,7 @@ class FeedForwardBlock(nn.Module):
 
     pre_norm and post_norm: 'rms', 'layer', or for post_norm 'none' (the default).  gate: a learned number per channel, from
     `gate_init`; None: none.  (B, C, N) features in either memory order, of the parameters' type; the result is channel-major when
-    they are.  The state of the dropout's generator is not part of the state dict."""
+    they are.  The dropout draws as CounterDropout does."""
 
     def __init__(self, channels, hidden, activation='silu', pre_norm='rms', post_norm='none', eps=1e-6, gate_init=1.0,
                  residual_scale=1.0, dropout=0.0, precision='f32', seed=None):
@@ -583,7 +589,7 @@ class FeedForwardBlock(nn.Module):
 
         self.pre_weight, self.pre_bias = vector(1.0, True), vector(0.0, pre_norm == 'layer')
         self.post_weight, self.post_bias = vector(1.0, post_norm != 'none'), vector(0.0, post_norm == 'layer')
-        self.gate = vector(gate_init, gate_init is not None) if gate_init is not None else None
+        self.gate = vector(0.0 if gate_init is None else gate_init, gate_init is not None)
         self.feed_forward = GatedFeedForward(channels, hidden, activation, precision)
 
     def forward(self, features):

@@ -232,3 +232,22 @@ def test_gradients_of_the_references_against_differences():
         want = float((grads[name][0] * v).sum())
         # the error of d2 is a third of d1 - d2 (fourth order aside); 1e-9 for the cancellation
         assert abs(d2 - want) <= abs(d1 - d2) * 0.5 + 1e-9 * max(1.0, abs(want)), (name, d1, d2, want)
+
+
+def test_a_module_keeps_its_generator_of_each_device(monkeypatch):
+    """Going back to a device goes on with its numbers."""
+    made = []
+
+    class Rng:
+        def __init__(self, seed, device):
+            made.append((seed, device))
+
+        def take(self, n):
+            return made, n
+
+    monkeypatch.setattr(ff, "CounterRng", Rng)
+    draws = ff._Draws(5)
+    here, there = torch.empty(3), torch.empty(4, device="meta")
+    for x in (here, there, here, there):
+        assert draws.take(x)[1] == x.numel()
+    assert made == [(5, here.device), (5, there.device)]
