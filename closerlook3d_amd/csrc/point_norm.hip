@@ -447,6 +447,284 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
   if (BIAS && a.b2) flush(s_b2, 4);
 }
 
+// ---- channel-major features [B][C][N] of up to 256 channels, a multiple of 4: no transposed copies.  A workgroup has 64 points of a
+// cloud, a lane one of them; wave w has the channels 4 (w + W i) .. + 3, i < QN, of the W waves (fours: one block of the generator).
+// A channel is read and written 64 elements in a row, the values stay in registers, sums over channels go through LDS: a buffer for
+// each, so that a barrier each is enough.  Parameter gradients: 64 points by lane_sum, one partial row per workgroup.
+// @@CM@@
+constexpr int kCmMaxC = 256, kCmWaves = 16;
+
+template <typename T> struct CmParams {
+  float v[5][kCmMaxC];  // w, b, gate, w2, b2
+  __device__ __forceinline__ void load(const NormArgs &a, int b) {
+    for (int c = threadIdx.x; c < a.C; c += blockDim.x) {
+      params<T, 1>(a.w1, c, a.param_f32, 1.f, &v[0][c]);
+      params<T, 1>(a.b1, c, a.param_f32, 0.f, &v[1][c]);
+      params<T, 1>(a.gate, (a.gate_cloud ? (long long)b * a.C : 0) + c, a.param_f32, 1.f, &v[2][c]);
+      params<T, 1>(a.w2, c, a.param_f32, 1.f, &v[3][c]);
+      params<T, 1>(a.b2, c, a.param_f32, 0.f, &v[4][c]);
+    }
+  }
+};
+using CmSums = float[kCmWaves][64];
+
+// a point's elements of QN quads of channels; what a lane does not have is 0
+template <typename S, int QN>
+__device__ __forceinline__ void cm_fetch(const void *p, bool wanted, const long long (&at)[QN], const bool (&on)[QN], long long N, S (&raw)[QN][4]) {
+#pragma unroll
+  for (int q = 0; q < QN; ++q)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) raw[q][e] = 0;
+  if (!wanted) return;
+#pragma unroll
+  for (int q = 0; q < QN; ++q)
+    if (on[q]) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) raw[q][e] = static_cast<const S *>(p)[at[q] + e * N];
+    }
+}
+
+// the waves' values of a lane, added in their order
+__device__ __forceinline__ float wave_sum(float v, CmSums &s, int wave, int lane, int waves) {
+  s[wave][lane] = v;
+  __syncthreads();
+  float t = 0.f;
+  for (int w = 0; w < waves; ++w) t += s[w][lane];
+  return t;
+}
+// mean and reciprocal deviation of a point held as v[QN][4] by the waves of a workgroup
+template <int QN>
+__device__ __forceinline__ void cm_stats(const float (&v)[QN][4], const bool (&on)[QN], int kind, float eps, float inv_c, CmSums &s0, CmSums &s1,
+                                         int wave, int lane, int waves, float &mean, float &rinv) {
+  mean = 0.f;
+  float t = 0.f;
+  if (kind == CL3D_NORM_LAYER) {
+#pragma unroll
+    for (int q = 0; q < QN; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t += on[q] ? v[q][e] : 0.f;
+    mean = wave_sum(t, s0, wave, lane, waves) * inv_c;
+  }
+  t = 0.f;
+#pragma unroll
+  for (int q = 0; q < QN; ++q)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t = on[q] ? __builtin_fmaf(v[q][e] - mean, v[q][e] - mean, t) : t;
+  rinv = 1.f / sqrtf(wave_sum(t, s1, wave, lane, waves) * inv_c + eps);
+}
+
+template <typename T, int QN, bool DROP>
+__global__ __launch_bounds__(64 * kCmWaves) void norm_cm_fwd_kernel(NormArgs a) {
+  using S = typename T::storage;
+  __shared__ CmSums s[4];
+  __shared__ CmParams<T> par;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int b = blockIdx.x / a.chunks, tile = blockIdx.x % a.chunks;
+  const long long n0 = (long long)tile * 64 + lane;
+  const bool live = n0 < a.N;
+  const long long n = live ? n0 : a.N - 1, r = (long long)b * a.N + n;  // (a lane behind the last point works on it, unstored)
+  const float inv_c = 1.f / (float)a.C;
+  bool on[QN];
+  int c0[QN];
+  long long at[QN];
+  S rx[QN][4], ry[QN][4];
+  float v[QN][4], y[QN][4];
+#pragma unroll
+  for (int q = 0; q < QN; ++q) {
+    c0[q] = 4 * (wave + waves * q);
+    on[q] = c0[q] < a.C;
+    at[q] = ((long long)b * a.C + c0[q]) * a.N + n;
+  }
+  cm_fetch<S, QN>(a.x, true, at, on, a.N, rx);
+  cm_fetch<S, QN>(a.y, a.exit, at, on, a.N, ry);
+  par.load(a, b);
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < QN; ++q)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[q][e] = T::get(rx[q][e]);
+      y[q][e] = T::get(ry[q][e]);
+    }
+  if (a.exit) {
+    float mean = 0.f, rinv = 1.f;
+    if (a.kind1 != CL3D_NORM_NONE) cm_stats<QN>(y, on, a.kind1, a.eps1, inv_c, s[0], s[1], wave, lane, waves, mean, rinv);
+    if (a.stats && live && wave == 0) *reinterpret_cast<float2 *>(a.stats + 4 * r) = make_float2(mean, rinv);
+    unsigned long long seed = 0, offset = 0;
+    if (DROP) { seed = a.drop.state[0]; offset = a.drop.state[1]; }
+#pragma unroll
+    for (int q = 0; q < QN; ++q) {
+      if (!on[q]) continue;
+      bool m[4];
+      if (DROP) stay_v<4>(a.drop, seed, offset, r * a.C + c0[q], m);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float k = __builtin_fmaf((y[q][e] - mean) * rinv, par.v[0][c0[q] + e], par.v[1][c0[q] + e]);
+        if (DROP) k = m[e] ? k * a.drop.scale : 0.f;
+        v[q][e] = __builtin_fmaf(a.alpha, v[q][e], par.v[2][c0[q] + e] * k);
+        if (live) static_cast<S *>(a.o)[at[q] + e * a.N] = T::put(v[q][e]);
+      }
+    }
+  }
+  if (a.next) {
+    float mean, rinv;
+    cm_stats<QN>(v, on, a.kind2, a.eps2, inv_c, s[2], s[3], wave, lane, waves, mean, rinv);
+    if (a.stats && live && wave == 0) *reinterpret_cast<float2 *>(a.stats + 4 * r + 2) = make_float2(mean, rinv);
+#pragma unroll
+    for (int q = 0; q < QN; ++q) {
+      if (!on[q] || !live) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        static_cast<S *>(a.h)[at[q] + e * a.N] =
+            T::put(__builtin_fmaf((v[q][e] - mean) * rinv, par.v[3][c0[q] + e], par.v[4][c0[q] + e]));
+    }
+  }
+}
+
+template <typename T, int QN, bool DROP>
+__global__ __launch_bounds__(64 * kCmWaves) void norm_cm_bwd_kernel(NormArgs a) {
+  using S = typename T::storage;
+  __shared__ CmSums s[4];
+  __shared__ CmParams<T> par;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int b = blockIdx.x / a.chunks, tile = blockIdx.x % a.chunks;
+  const long long n0 = (long long)tile * 64 + lane;
+  const bool live = n0 < a.N;
+  const long long n = live ? n0 : a.N - 1, r = (long long)b * a.N + n;
+  const float inv_c = 1.f / (float)a.C;
+  const f32x4 st = *reinterpret_cast<const f32x4 *>(a.stats + 4 * r);
+  bool on[QN];
+  int c0[QN];
+  long long at[QN];
+  S ry[QN][4], rd[QN][4], rx[QN][4], rh[QN][4];
+  float hat1[QN][4], d[QN][4], hat[QN][4], dh[QN][4], nk[QN][4];
+  bool stays[QN][4];
+#pragma unroll
+  for (int q = 0; q < QN; ++q) {
+    c0[q] = 4 * (wave + waves * q);
+    on[q] = c0[q] < a.C;
+    at[q] = ((long long)b * a.C + c0[q]) * a.N + n;
+  }
+  cm_fetch<S, QN>(a.y, a.exit, at, on, a.N, ry);
+  cm_fetch<S, QN>(a.dout, a.dout != nullptr, at, on, a.N, rd);
+  cm_fetch<S, QN>(a.x, a.dnext != nullptr, at, on, a.N, rx);
+  cm_fetch<S, QN>(a.dnext, a.dnext != nullptr, at, on, a.N, rh);
+  par.load(a, b);
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < QN; ++q)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      hat1[q][e] = T::get(ry[q][e]);
+      d[q][e] = live ? T::get(rd[q][e]) : 0.f;  // (a lane behind the last point: zero gradients)
+      hat[q][e] = T::get(rx[q][e]);
+      dh[q][e] = live ? T::get(rh[q][e]) : 0.f;
+      nk[q][e] = 0.f;
+    }
+  float *partial = a.partial ? a.partial + (long long)blockIdx.x * 5 * a.C : nullptr;
+  // a wave's sums over its 64 points of a quad's four columns
+  auto flush = [&](int which, int c, float v0, float v1, float v2, float v3) {
+    const f32x4 t = {lane_sum<64>(v0), lane_sum<64>(v1), lane_sum<64>(v2), lane_sum<64>(v3)};
+    if (lane == 0) *reinterpret_cast<f32x4 *>(partial + (long long)which * a.C + c) = t;
+  };
+  if (a.exit) {  // (as in norm_bwd_kernel: the exit once more)
+    unsigned long long seed = 0, offset = 0;
+    if (DROP) { seed = a.drop.state[0]; offset = a.drop.state[1]; }
+#pragma unroll
+    for (int q = 0; q < QN; ++q) {
+      if (!on[q]) continue;
+      if (DROP) stay_v<4>(a.drop, seed, offset, r * a.C + c0[q], stays[q]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        hat1[q][e] = (hat1[q][e] - st[0]) * st[1];
+        nk[q][e] = __builtin_fmaf(hat1[q][e], par.v[0][c0[q] + e], par.v[1][c0[q] + e]);
+        if (DROP) nk[q][e] = stays[q][e] ? nk[q][e] * a.drop.scale : 0.f;
+      }
+    }
+  }
+  if (a.dnext) {
+    float p1 = 0.f, p2 = 0.f;
+#pragma unroll
+    for (int q = 0; q < QN; ++q) {
+      if (!on[q]) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (a.exit) hat[q][e] = __builtin_fmaf(a.alpha, hat[q][e], par.v[2][c0[q] + e] * nk[q][e]);
+        hat[q][e] = (hat[q][e] - st[2]) * st[3];
+      }
+      if (partial) {
+        if (a.w2) flush(3, c0[q], dh[q][0] * hat[q][0], dh[q][1] * hat[q][1], dh[q][2] * hat[q][2], dh[q][3] * hat[q][3]);
+        if (a.b2) flush(4, c0[q], dh[q][0], dh[q][1], dh[q][2], dh[q][3]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        dh[q][e] *= par.v[3][c0[q] + e];
+        p1 = __builtin_fmaf(dh[q][e], hat[q][e], p1);
+        p2 += dh[q][e];
+      }
+    }
+    p1 = wave_sum(p1, s[0], wave, lane, waves) * inv_c;
+    p2 = a.kind2 == CL3D_NORM_LAYER ? wave_sum(p2, s[1], wave, lane, waves) * inv_c : 0.f;
+#pragma unroll
+    for (int q = 0; q < QN; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[q][e] = __builtin_fmaf(st[3], dh[q][e] - __builtin_fmaf(hat[q][e], p1, p2), d[q][e]);
+  } else if (partial && a.next) {  // (the next norm's result was not used)
+#pragma unroll
+    for (int q = 0; q < QN; ++q) {
+      if (!on[q]) continue;
+      if (a.w2) flush(3, c0[q], 0.f, 0.f, 0.f, 0.f);
+      if (a.b2) flush(4, c0[q], 0.f, 0.f, 0.f, 0.f);
+    }
+  }
+  if (a.dx && live) {
+#pragma unroll
+    for (int q = 0; q < QN; ++q) {
+      if (!on[q]) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) static_cast<S *>(a.dx)[at[q] + e * a.N] = T::put(a.exit ? a.alpha * d[q][e] : d[q][e]);
+    }
+  }
+  if (!a.exit) return;
+  float p1 = 0.f, p2 = 0.f;
+#pragma unroll
+  for (int q = 0; q < QN; ++q) {
+    if (!on[q]) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) d[q][e] = live ? d[q][e] : 0.f;
+    if (partial && a.gate) flush(2, c0[q], d[q][0] * nk[q][0], d[q][1] * nk[q][1], d[q][2] * nk[q][2], d[q][3] * nk[q][3]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (DROP) d[q][e] = stays[q][e] ? d[q][e] * a.drop.scale : 0.f;
+      d[q][e] *= par.v[2][c0[q] + e];
+    }
+    if (partial && a.w1)
+      flush(0, c0[q], d[q][0] * hat1[q][0], d[q][1] * hat1[q][1], d[q][2] * hat1[q][2], d[q][3] * hat1[q][3]);
+    if (partial && a.b1) flush(1, c0[q], d[q][0], d[q][1], d[q][2], d[q][3]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      d[q][e] *= par.v[0][c0[q] + e];
+      p1 = __builtin_fmaf(d[q][e], hat1[q][e], p1);
+      p2 += d[q][e];
+    }
+  }
+  if (!a.dy) return;
+  if (a.kind1 == CL3D_NORM_NONE) {
+    p1 = p2 = 0.f;
+  } else {
+    p1 = wave_sum(p1, s[2], wave, lane, waves) * inv_c;
+    p2 = a.kind1 == CL3D_NORM_LAYER ? wave_sum(p2, s[3], wave, lane, waves) * inv_c : 0.f;
+  }
+  if (!live) return;
+#pragma unroll
+  for (int q = 0; q < QN; ++q) {
+    if (!on[q]) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      static_cast<S *>(a.dy)[at[q] + e * a.N] = T::put(st[1] * (d[q][e] - __builtin_fmaf(hat1[q][e], p1, p2)));
+  }
+}
+
 // sums of the partial rows [row][which][C]: 16 columns a workgroup, 64 runs of rows side by side, joined in order
 struct NormSums {
   const float *partial;
@@ -546,6 +824,33 @@ static void norm_launch(int dtype, const NormMap &m, bool backward, const NormAr
   else norm_pick<F16>(m, backward, a, st);
 }
 
+// (as few channels a wave as sixteen waves allow)
+static int cm_quads(int C) { return C <= 8 * kCmWaves ? 2 : 4; }
+static bool norm_cm(int order, int B, int N, int C) {
+  if (order != CL3D_CHANNEL_MAJOR || N <= 1 || C % 4 != 0 || C > kCmMaxC) return false;
+  return (long long)B * ceil_div(N, 64) * 64 * ceil_div(C / 4, cm_quads(C)) <= 0xffffffffll;  // (threads that a grid counts)
+}
+
+template <typename T, int QN> static void norm_cm_run(bool backward, const NormArgs &a, hipStream_t st) {
+  const dim3 grid((unsigned)((long long)a.B * a.chunks)), block(64 * ceil_div(a.C / 4, QN));
+  if (backward) {
+    if (a.has_drop) hipLaunchKernelGGL((norm_cm_bwd_kernel<T, QN, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((norm_cm_bwd_kernel<T, QN, false>), grid, block, 0, st, a);
+  } else {
+    if (a.has_drop) hipLaunchKernelGGL((norm_cm_fwd_kernel<T, QN, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((norm_cm_fwd_kernel<T, QN, false>), grid, block, 0, st, a);
+  }
+}
+template <typename T> static void norm_cm_pick(bool backward, const NormArgs &a, hipStream_t st) {
+  if (cm_quads(a.C) == 2) norm_cm_run<T, 2>(backward, a, st);
+  else norm_cm_run<T, 4>(backward, a, st);
+}
+static void norm_cm_launch(int dtype, bool backward, const NormArgs &a, hipStream_t st) {
+  if (dtype == CL3D_F32) norm_cm_pick<F32>(backward, a, st);
+  else if (dtype == CL3D_BF16) norm_cm_pick<Bf16>(backward, a, st);
+  else norm_cm_pick<F16>(backward, a, st);
+}
+
 static int norm_checks(const cl3d_norm_residual *p, bool backward, const char *who) {
   CL3D_REQUIRE(p != nullptr, "%s: null argument block", who);
   CL3D_REQUIRE(p->dtype == CL3D_F32 || p->dtype == CL3D_BF16 || p->dtype == CL3D_F16, "%s: unknown element type %d", who, p->dtype);
@@ -567,7 +872,8 @@ static void norm_args(NormArgs &a, const cl3d_norm_residual *p) {
   a.w1 = p->weight; a.b1 = p->bias; a.gate = p->gate; a.w2 = p->next_weight; a.b2 = p->next_bias;
   a.stats = p->stats;
   a.N = p->N; a.B = p->B; a.C = p->C;
-  if (!p->gate_cloud) { a.N *= a.B; a.B = 1; }  // nothing differs from cloud to cloud: one run of rows
+  if (norm_cm(p->order, p->B, p->N, p->C)) a.chunks = ceil_div(a.N, 64);
+  else if (!p->gate_cloud) { a.N *= a.B; a.B = 1; }  // nothing differs from cloud to cloud: one run of rows
   a.kind1 = p->kind; a.kind2 = p->next_kind;
   a.exit = p->y != nullptr; a.next = p->next_kind != CL3D_NORM_NONE;
   a.gate_cloud = p->gate_cloud; a.param_f32 = p->param_f32 || p->dtype == CL3D_F32;
@@ -591,7 +897,7 @@ struct NormCopies {
   bool copies;
   int rc = CL3D_OK;
   NormCopies(const cl3d_norm_residual *p_, void *ws, hipStream_t st_)
-      : p(p_), ar(ws), st(st_), copies(p_->order == CL3D_CHANNEL_MAJOR && p_->N > 1 && p_->C > 1) {}
+      : p(p_), ar(ws), st(st_), copies(p_->order == CL3D_CHANNEL_MAJOR && p_->N > 1 && p_->C > 1 && !norm_cm(p_->order, p_->B, p_->N, p_->C)) {}
   void *place() { return ar.take((size_t)p->B * p->N * p->C * elem_bytes(p->dtype)); }
   const void *in(const void *t) {
     if (!copies || !t) return t;
@@ -609,7 +915,9 @@ size_t point_norm_workspace(int B, int N, int C, int flags) {
   // flags: element type | memory order << 2 | tensors to copy << 3 | parameter gradients << 8
   if (B <= 0 || N <= 0 || C <= 0) return 0;
   Arena ar(nullptr);
-  if (((flags >> 2) & 1) == CL3D_CHANNEL_MAJOR && N > 1 && C > 1)
+  const int order = (flags >> 2) & 1;
+  if (norm_cm(order, B, N, C)) return (flags >> 8) & 1 ? (size_t)B * ceil_div(N, 64) * 5 * (size_t)C * sizeof(float) : 0;
+  if (order == CL3D_CHANNEL_MAJOR && N > 1 && C > 1)
     for (int q = 0; q < ((flags >> 3) & 31); ++q) ar.take((size_t)B * N * C * elem_bytes(flags & 3));
   // partial rows of the backward pass: at most kNormBwdGroups + B workgroups
   if ((flags >> 8) & 1) ar.take(((size_t)kNormBwdGroups + B) * 5 * (size_t)C * sizeof(float));
@@ -637,6 +945,10 @@ extern "C" int cl3d_norm_residual_fwd(const cl3d_norm_residual *p, cl3d_stream_t
   a.x = c.in(p->x); a.y = c.in(p->y);
   a.o = c.out(p->out); a.h = c.out(p->next);
   if (c.rc != CL3D_OK) return c.rc;
+  if (norm_cm(p->order, p->B, p->N, p->C)) {
+    norm_cm_launch(p->dtype, false, a, st);
+    return check_launch("cl3d_norm_residual_fwd");
+  }
   const NormMap m = norm_map(p->dtype, p->C, aligned16(a.x) && aligned16(a.y) && aligned16(a.o) && aligned16(a.h) && params_aligned(p));
   norm_grid(a, 256 / m.tpr, kNormFwdGroups);
   norm_launch(p->dtype, m, false, a, st);
@@ -663,7 +975,8 @@ extern "C" int cl3d_norm_residual_bwd(const cl3d_norm_residual *p, cl3d_stream_t
   need.in(x), need.in(p->y), need.in(p->dout), need.in(p->dnext), need.out(p->dx), need.out(p->dy);
   const NormMap m = norm_map(p->dtype, p->C, params_aligned(p) && (need.copies || (aligned16(x) && aligned16(p->y) && aligned16(p->dout) && aligned16(p->dnext) &&
                                                              aligned16(p->dx) && aligned16(p->dy))));
-  norm_grid(a, 256 / m.tpr, kNormBwdGroups);
+  const bool cm = norm_cm(p->order, p->B, p->N, p->C);
+  if (!cm) norm_grid(a, 256 / m.tpr, kNormBwdGroups);
   const size_t partial_bytes = sums ? (size_t)a.B * a.chunks * 5 * a.C * sizeof(float) : 0;
   if (sums) need.ar.take(partial_bytes);
   if (need.ar.used && (!p->ws || p->ws_bytes < need.ar.used))
@@ -673,7 +986,8 @@ extern "C" int cl3d_norm_residual_bwd(const cl3d_norm_residual *p, cl3d_stream_t
   a.dx = c.out(p->dx); a.dy = c.out(p->dy);
   if (sums) a.partial = static_cast<float *>(c.ar.take(partial_bytes));
   if (c.rc != CL3D_OK) return c.rc;
-  norm_launch(p->dtype, m, true, a, st);
+  if (cm) norm_cm_launch(p->dtype, true, a, st);
+  else norm_launch(p->dtype, m, true, a, st);
   c.back(a.dx, p->dx), c.back(a.dy, p->dy);
   if (c.rc != CL3D_OK) return c.rc;
   if (sums) {

@@ -112,7 +112,7 @@ def _workspace(op, B, N, M, K, C, device):
         if len(_WORKSPACE) > 4096:
             _WORKSPACE.clear()
         nbytes = _WORKSPACE[key] = _lib.lib().cl3d_workspace_bytes(*key)
-    return torch.empty(nbytes or 1, dtype=torch.uint8, device=device), nbytes
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None, nbytes
 
 
 def _empty(shape, order, dtype, device):
