@@ -447,26 +447,26 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
   if (BIAS && a.b2) flush(s_b2, 4);
 }
 
-// ---- channel-major features [B][C][N] of up to 256 channels, a multiple of 4: no transposed copies.  A workgroup has 64 points of a
-// cloud, a lane one of them; wave w has the channels 4 (w + W i) .. + 3, i < QN, of the W waves (fours: one block of the generator).
-// A channel is read and written 64 elements in a row, the values stay in registers, sums over channels go through LDS: a buffer for
-// each, so that a barrier each is enough.  Parameter gradients: 64 points by lane_sum, one partial row per workgroup.
-// @@CM@@
-constexpr int kCmMaxC = 256, kCmWaves = 16;
+// ---- channel-major features [B][C][N] of up to 1024 channels, a multiple of 4: no transposed copies.  A workgroup has P = 64, 32 or
+// 16 points of a cloud, a lane one of them; the 64 / P lane groups of its W waves have the channels 4 (g + G i) .. + 3, i < QN, of
+// G = W 64 / P (fours: one block of the generator).  A channel is read and written P elements in a row, the values stay in registers,
+// sums over channels go through LDS: a buffer for each, so that a barrier each is enough.  Parameter gradients: P points by
+// lane_sum, one partial row per workgroup.
+// Measured: 16 x 144 x 4096 bf16, exit and next norm, 19 us (4.0 TB/s; by transposed copies 91), with the gradients 75 (250); 4 x 72 x
+// 10 000 f32, exit with dropout and its gradients 29 (72).
+constexpr int kCmMaxC = 1024, kCmWaves = 16;
 
-template <typename T> struct CmParams {
-  float v[5][kCmMaxC];  // w, b, gate, w2, b2
-  __device__ __forceinline__ void load(const NormArgs &a, int b) {
-    for (int c = threadIdx.x; c < a.C; c += blockDim.x) {
-      params<T, 1>(a.w1, c, a.param_f32, 1.f, &v[0][c]);
-      params<T, 1>(a.b1, c, a.param_f32, 0.f, &v[1][c]);
-      params<T, 1>(a.gate, (a.gate_cloud ? (long long)b * a.C : 0) + c, a.param_f32, 1.f, &v[2][c]);
-      params<T, 1>(a.w2, c, a.param_f32, 1.f, &v[3][c]);
-      params<T, 1>(a.b2, c, a.param_f32, 0.f, &v[4][c]);
-    }
+// LDS of a workgroup: four buffers of a float per lane, then w, b, gate, w2, b2 [C] each
+static size_t cm_lds_bytes(int waves, int C) { return (4 * 64 * (size_t)waves + 5 * (size_t)C) * sizeof(float); }
+template <typename T> __device__ __forceinline__ void cm_params(const NormArgs &a, int b, float *par) {
+  for (int c = threadIdx.x; c < a.C; c += blockDim.x) {
+    params<T, 1>(a.w1, c, a.param_f32, 1.f, par + c);
+    params<T, 1>(a.b1, c, a.param_f32, 0.f, par + a.C + c);
+    params<T, 1>(a.gate, (a.gate_cloud ? (long long)b * a.C : 0) + c, a.param_f32, 1.f, par + 2 * a.C + c);
+    params<T, 1>(a.w2, c, a.param_f32, 1.f, par + 3 * a.C + c);
+    params<T, 1>(a.b2, c, a.param_f32, 0.f, par + 4 * a.C + c);
   }
-};
-using CmSums = float[kCmWaves][64];
+}
 
 // a point's elements of QN quads of channels; what a lane does not have is 0
 template <typename S, int QN>
@@ -484,17 +484,25 @@ __device__ __forceinline__ void cm_fetch(const void *p, bool wanted, const long 
     }
 }
 
-// the waves' values of a lane, added in their order
-__device__ __forceinline__ float wave_sum(float v, CmSums &s, int wave, int lane, int waves) {
-  s[wave][lane] = v;
+// the lane groups' values of a point, added in one order
+template <int P> __device__ __forceinline__ float wave_sum(float v, float *s, int wave, int lane, int waves) {
+  if (P < 32) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  if (P < 64) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  s[wave * 64 + lane] = v;
   __syncthreads();
   float t = 0.f;
-  for (int w = 0; w < waves; ++w) t += s[w][lane];
+  for (int w = 0; w < waves; ++w) t += s[w * 64 + lane];
   return t;
 }
-// mean and reciprocal deviation of a point held as v[QN][4] by the waves of a workgroup
-template <int QN>
-__device__ __forceinline__ void cm_stats(const float (&v)[QN][4], const bool (&on)[QN], int kind, float eps, float inv_c, CmSums &s0, CmSums &s1,
+// mean and reciprocal deviation of a point held as v[QN][4] by the lane groups of a workgroup
+template <int P, int QN>
+__device__ __forceinline__ void cm_stats(const float (&v)[QN][4], const bool (&on)[QN], int kind, float eps, float inv_c, float *s0, float *s1,
                                          int wave, int lane, int waves, float &mean, float &rinv) {
   mean = 0.f;
   float t = 0.f;
@@ -503,24 +511,29 @@ __device__ __forceinline__ void cm_stats(const float (&v)[QN][4], const bool (&o
     for (int q = 0; q < QN; ++q)
 #pragma unroll
       for (int e = 0; e < 4; ++e) t += on[q] ? v[q][e] : 0.f;
-    mean = wave_sum(t, s0, wave, lane, waves) * inv_c;
+    mean = wave_sum<P>(t, s0, wave, lane, waves) * inv_c;
   }
   t = 0.f;
 #pragma unroll
   for (int q = 0; q < QN; ++q)
 #pragma unroll
     for (int e = 0; e < 4; ++e) t = on[q] ? __builtin_fmaf(v[q][e] - mean, v[q][e] - mean, t) : t;
-  rinv = 1.f / sqrtf(wave_sum(t, s1, wave, lane, waves) * inv_c + eps);
+  rinv = 1.f / sqrtf(wave_sum<P>(t, s1, wave, lane, waves) * inv_c + eps);
 }
 
-template <typename T, int QN, bool DROP>
+template <typename T, int P, int QN, bool DROP>
 __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_fwd_kernel(NormArgs a) {
   using S = typename T::storage;
-  __shared__ CmSums s[4];
-  __shared__ CmParams<T> par;
+  extern __shared__ float s_cm[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int group = wave * (64 / P) + lane / P, groups = waves * (64 / P);
+  float *s[4], *par[5];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) s[k] = s_cm + k * 64 * waves;
+#pragma unroll
+  for (int k = 0; k < 5; ++k) par[k] = s_cm + 4 * 64 * waves + k * a.C;
   const int b = blockIdx.x / a.chunks, tile = blockIdx.x % a.chunks;
-  const long long n0 = (long long)tile * 64 + lane;
+  const long long n0 = (long long)tile * P + lane % P;
   const bool live = n0 < a.N;
   const long long n = live ? n0 : a.N - 1, r = (long long)b * a.N + n;  // (a lane behind the last point works on it, unstored)
   const float inv_c = 1.f / (float)a.C;
@@ -531,13 +544,13 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_fwd_kernel(NormArgs a) 
   float v[QN][4], y[QN][4];
 #pragma unroll
   for (int q = 0; q < QN; ++q) {
-    c0[q] = 4 * (wave + waves * q);
+    c0[q] = 4 * (group + groups * q);
     on[q] = c0[q] < a.C;
     at[q] = ((long long)b * a.C + c0[q]) * a.N + n;
   }
   cm_fetch<S, QN>(a.x, true, at, on, a.N, rx);
   cm_fetch<S, QN>(a.y, a.exit, at, on, a.N, ry);
-  par.load(a, b);
+  cm_params<T>(a, b, par[0]);
   __syncthreads();
 #pragma unroll
   for (int q = 0; q < QN; ++q)
@@ -548,8 +561,8 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_fwd_kernel(NormArgs a) 
     }
   if (a.exit) {
     float mean = 0.f, rinv = 1.f;
-    if (a.kind1 != CL3D_NORM_NONE) cm_stats<QN>(y, on, a.kind1, a.eps1, inv_c, s[0], s[1], wave, lane, waves, mean, rinv);
-    if (a.stats && live && wave == 0) *reinterpret_cast<float2 *>(a.stats + 4 * r) = make_float2(mean, rinv);
+    if (a.kind1 != CL3D_NORM_NONE) cm_stats<P, QN>(y, on, a.kind1, a.eps1, inv_c, s[0], s[1], wave, lane, waves, mean, rinv);
+    if (a.stats && live && group == 0) *reinterpret_cast<float2 *>(a.stats + 4 * r) = make_float2(mean, rinv);
     unsigned long long seed = 0, offset = 0;
     if (DROP) { seed = a.drop.state[0]; offset = a.drop.state[1]; }
 #pragma unroll
@@ -559,36 +572,41 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_fwd_kernel(NormArgs a) 
       if (DROP) stay_v<4>(a.drop, seed, offset, r * a.C + c0[q], m);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float k = __builtin_fmaf((y[q][e] - mean) * rinv, par.v[0][c0[q] + e], par.v[1][c0[q] + e]);
+        float k = __builtin_fmaf((y[q][e] - mean) * rinv, par[0][c0[q] + e], par[1][c0[q] + e]);
         if (DROP) k = m[e] ? k * a.drop.scale : 0.f;
-        v[q][e] = __builtin_fmaf(a.alpha, v[q][e], par.v[2][c0[q] + e] * k);
+        v[q][e] = __builtin_fmaf(a.alpha, v[q][e], par[2][c0[q] + e] * k);
         if (live) static_cast<S *>(a.o)[at[q] + e * a.N] = T::put(v[q][e]);
       }
     }
   }
   if (a.next) {
     float mean, rinv;
-    cm_stats<QN>(v, on, a.kind2, a.eps2, inv_c, s[2], s[3], wave, lane, waves, mean, rinv);
-    if (a.stats && live && wave == 0) *reinterpret_cast<float2 *>(a.stats + 4 * r + 2) = make_float2(mean, rinv);
+    cm_stats<P, QN>(v, on, a.kind2, a.eps2, inv_c, s[2], s[3], wave, lane, waves, mean, rinv);
+    if (a.stats && live && group == 0) *reinterpret_cast<float2 *>(a.stats + 4 * r + 2) = make_float2(mean, rinv);
 #pragma unroll
     for (int q = 0; q < QN; ++q) {
       if (!on[q] || !live) continue;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         static_cast<S *>(a.h)[at[q] + e * a.N] =
-            T::put(__builtin_fmaf((v[q][e] - mean) * rinv, par.v[3][c0[q] + e], par.v[4][c0[q] + e]));
+            T::put(__builtin_fmaf((v[q][e] - mean) * rinv, par[3][c0[q] + e], par[4][c0[q] + e]));
     }
   }
 }
 
-template <typename T, int QN, bool DROP>
+template <typename T, int P, int QN, bool DROP>
 __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_bwd_kernel(NormArgs a) {
   using S = typename T::storage;
-  __shared__ CmSums s[4];
-  __shared__ CmParams<T> par;
+  extern __shared__ float s_cm[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int group = wave * (64 / P) + lane / P, groups = waves * (64 / P);
+  float *s[4], *par[5];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) s[k] = s_cm + k * 64 * waves;
+#pragma unroll
+  for (int k = 0; k < 5; ++k) par[k] = s_cm + 4 * 64 * waves + k * a.C;
   const int b = blockIdx.x / a.chunks, tile = blockIdx.x % a.chunks;
-  const long long n0 = (long long)tile * 64 + lane;
+  const long long n0 = (long long)tile * P + lane % P;
   const bool live = n0 < a.N;
   const long long n = live ? n0 : a.N - 1, r = (long long)b * a.N + n;
   const float inv_c = 1.f / (float)a.C;
@@ -601,7 +619,7 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_bwd_kernel(NormArgs a) 
   bool stays[QN][4];
 #pragma unroll
   for (int q = 0; q < QN; ++q) {
-    c0[q] = 4 * (wave + waves * q);
+    c0[q] = 4 * (group + groups * q);
     on[q] = c0[q] < a.C;
     at[q] = ((long long)b * a.C + c0[q]) * a.N + n;
   }
@@ -609,7 +627,7 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_bwd_kernel(NormArgs a) 
   cm_fetch<S, QN>(a.dout, a.dout != nullptr, at, on, a.N, rd);
   cm_fetch<S, QN>(a.x, a.dnext != nullptr, at, on, a.N, rx);
   cm_fetch<S, QN>(a.dnext, a.dnext != nullptr, at, on, a.N, rh);
-  par.load(a, b);
+  cm_params<T>(a, b, par[0]);
   __syncthreads();
 #pragma unroll
   for (int q = 0; q < QN; ++q)
@@ -622,10 +640,10 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_bwd_kernel(NormArgs a) 
       nk[q][e] = 0.f;
     }
   float *partial = a.partial ? a.partial + (long long)blockIdx.x * 5 * a.C : nullptr;
-  // a wave's sums over its 64 points of a quad's four columns
+  // a lane group's sums over its points of a quad's four columns
   auto flush = [&](int which, int c, float v0, float v1, float v2, float v3) {
-    const f32x4 t = {lane_sum<64>(v0), lane_sum<64>(v1), lane_sum<64>(v2), lane_sum<64>(v3)};
-    if (lane == 0) *reinterpret_cast<f32x4 *>(partial + (long long)which * a.C + c) = t;
+    const f32x4 t = {lane_sum<P>(v0), lane_sum<P>(v1), lane_sum<P>(v2), lane_sum<P>(v3)};
+    if (lane % P == 0) *reinterpret_cast<f32x4 *>(partial + (long long)which * a.C + c) = t;
   };
   if (a.exit) {  // (as in norm_bwd_kernel: the exit once more)
     unsigned long long seed = 0, offset = 0;
@@ -637,7 +655,7 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_bwd_kernel(NormArgs a) 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         hat1[q][e] = (hat1[q][e] - st[0]) * st[1];
-        nk[q][e] = __builtin_fmaf(hat1[q][e], par.v[0][c0[q] + e], par.v[1][c0[q] + e]);
+        nk[q][e] = __builtin_fmaf(hat1[q][e], par[0][c0[q] + e], par[1][c0[q] + e]);
         if (DROP) nk[q][e] = stays[q][e] ? nk[q][e] * a.drop.scale : 0.f;
       }
     }
@@ -649,7 +667,7 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_bwd_kernel(NormArgs a) 
       if (!on[q]) continue;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (a.exit) hat[q][e] = __builtin_fmaf(a.alpha, hat[q][e], par.v[2][c0[q] + e] * nk[q][e]);
+        if (a.exit) hat[q][e] = __builtin_fmaf(a.alpha, hat[q][e], par[2][c0[q] + e] * nk[q][e]);
         hat[q][e] = (hat[q][e] - st[2]) * st[3];
       }
       if (partial) {
@@ -658,13 +676,13 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_bwd_kernel(NormArgs a) 
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        dh[q][e] *= par.v[3][c0[q] + e];
+        dh[q][e] *= par[3][c0[q] + e];
         p1 = __builtin_fmaf(dh[q][e], hat[q][e], p1);
         p2 += dh[q][e];
       }
     }
-    p1 = wave_sum(p1, s[0], wave, lane, waves) * inv_c;
-    p2 = a.kind2 == CL3D_NORM_LAYER ? wave_sum(p2, s[1], wave, lane, waves) * inv_c : 0.f;
+    p1 = wave_sum<P>(p1, s[0], wave, lane, waves) * inv_c;
+    p2 = a.kind2 == CL3D_NORM_LAYER ? wave_sum<P>(p2, s[1], wave, lane, waves) * inv_c : 0.f;
 #pragma unroll
     for (int q = 0; q < QN; ++q)
 #pragma unroll
@@ -696,14 +714,14 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_bwd_kernel(NormArgs a) 
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (DROP) d[q][e] = stays[q][e] ? d[q][e] * a.drop.scale : 0.f;
-      d[q][e] *= par.v[2][c0[q] + e];
+      d[q][e] *= par[2][c0[q] + e];
     }
     if (partial && a.w1)
       flush(0, c0[q], d[q][0] * hat1[q][0], d[q][1] * hat1[q][1], d[q][2] * hat1[q][2], d[q][3] * hat1[q][3]);
     if (partial && a.b1) flush(1, c0[q], d[q][0], d[q][1], d[q][2], d[q][3]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      d[q][e] *= par.v[0][c0[q] + e];
+      d[q][e] *= par[0][c0[q] + e];
       p1 = __builtin_fmaf(d[q][e], hat1[q][e], p1);
       p2 += d[q][e];
     }
@@ -712,8 +730,8 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_bwd_kernel(NormArgs a) 
   if (a.kind1 == CL3D_NORM_NONE) {
     p1 = p2 = 0.f;
   } else {
-    p1 = wave_sum(p1, s[2], wave, lane, waves) * inv_c;
-    p2 = a.kind1 == CL3D_NORM_LAYER ? wave_sum(p2, s[3], wave, lane, waves) * inv_c : 0.f;
+    p1 = wave_sum<P>(p1, s[2], wave, lane, waves) * inv_c;
+    p2 = a.kind1 == CL3D_NORM_LAYER ? wave_sum<P>(p2, s[3], wave, lane, waves) * inv_c : 0.f;
   }
   if (!live) return;
 #pragma unroll
@@ -824,26 +842,40 @@ static void norm_launch(int dtype, const NormMap &m, bool backward, const NormAr
   else norm_pick<F16>(m, backward, a, st);
 }
 
-// (as few channels a wave as sixteen waves allow)
-static int cm_quads(int C) { return C <= 8 * kCmWaves ? 2 : 4; }
+struct CmMap {
+  int points, quads;  // P, QN
+};
+// points of a workgroup: as many as leave the channels to sixteen waves, fewer where the clouds would not fill the chip with
+// workgroups or have no more points.  Exit with dropout and its gradients, 64 / 16 points: 16 x 144 x 16 f32 16 / 11 us, 1 x 72 x 2500
+// 12.1 / 11.4, 2000 x 64 x 8 37 / 19, but 4 x 72 x 10 000 29 / 41, 16 x 144 x 1024 bf16 21 / 28 (short runs of a channel)
+static CmMap cm_map(int B, int N, int C) {
+  int p = C <= 256 ? 64 : C <= 512 ? 32 : 16;
+  while (p > 16 && (p / 2 >= N || (long long)B * ceil_div(N, p) < 256)) p /= 2;
+  return {p, C <= 2 * 4 * kCmWaves * 64 / p ? 2 : 4};  // (as few channels a lane as sixteen waves allow)
+}
+static int cm_waves(const CmMap &m, int C) { return ceil_div(ceil_div(C / 4, m.quads), 64 / m.points); }
 static bool norm_cm(int order, int B, int N, int C) {
   if (order != CL3D_CHANNEL_MAJOR || N <= 1 || C % 4 != 0 || C > kCmMaxC) return false;
-  return (long long)B * ceil_div(N, 64) * 64 * ceil_div(C / 4, cm_quads(C)) <= 0xffffffffll;  // (threads that a grid counts)
+  const CmMap m = cm_map(B, N, C);
+  return (long long)B * ceil_div(N, m.points) * 64 * cm_waves(m, C) <= 0xffffffffll;  // (threads that a grid counts)
 }
 
-template <typename T, int QN> static void norm_cm_run(bool backward, const NormArgs &a, hipStream_t st) {
-  const dim3 grid((unsigned)((long long)a.B * a.chunks)), block(64 * ceil_div(a.C / 4, QN));
+template <typename T, int P, int QN> static void norm_cm_run(bool backward, const NormArgs &a, const CmMap &m, hipStream_t st) {
+  const dim3 grid((unsigned)((long long)a.B * a.chunks)), block(64 * cm_waves(m, a.C));
+  const size_t lds = cm_lds_bytes(cm_waves(m, a.C), a.C);
   if (backward) {
-    if (a.has_drop) hipLaunchKernelGGL((norm_cm_bwd_kernel<T, QN, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((norm_cm_bwd_kernel<T, QN, false>), grid, block, 0, st, a);
+    if (a.has_drop) hipLaunchKernelGGL((norm_cm_bwd_kernel<T, P, QN, true>), grid, block, lds, st, a);
+    else hipLaunchKernelGGL((norm_cm_bwd_kernel<T, P, QN, false>), grid, block, lds, st, a);
   } else {
-    if (a.has_drop) hipLaunchKernelGGL((norm_cm_fwd_kernel<T, QN, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((norm_cm_fwd_kernel<T, QN, false>), grid, block, 0, st, a);
+    if (a.has_drop) hipLaunchKernelGGL((norm_cm_fwd_kernel<T, P, QN, true>), grid, block, lds, st, a);
+    else hipLaunchKernelGGL((norm_cm_fwd_kernel<T, P, QN, false>), grid, block, lds, st, a);
   }
 }
 template <typename T> static void norm_cm_pick(bool backward, const NormArgs &a, hipStream_t st) {
-  if (cm_quads(a.C) == 2) norm_cm_run<T, 2>(backward, a, st);
-  else norm_cm_run<T, 4>(backward, a, st);
+  const CmMap m = cm_map(a.B, (int)a.N, a.C);
+  if (m.points == 64) return m.quads == 2 ? norm_cm_run<T, 64, 2>(backward, a, m, st) : norm_cm_run<T, 64, 4>(backward, a, m, st);
+  if (m.points == 32) return m.quads == 2 ? norm_cm_run<T, 32, 2>(backward, a, m, st) : norm_cm_run<T, 32, 4>(backward, a, m, st);
+  return m.quads == 2 ? norm_cm_run<T, 16, 2>(backward, a, m, st) : norm_cm_run<T, 16, 4>(backward, a, m, st);
 }
 static void norm_cm_launch(int dtype, bool backward, const NormArgs &a, hipStream_t st) {
   if (dtype == CL3D_F32) norm_cm_pick<F32>(backward, a, st);
@@ -872,7 +904,7 @@ static void norm_args(NormArgs &a, const cl3d_norm_residual *p) {
   a.w1 = p->weight; a.b1 = p->bias; a.gate = p->gate; a.w2 = p->next_weight; a.b2 = p->next_bias;
   a.stats = p->stats;
   a.N = p->N; a.B = p->B; a.C = p->C;
-  if (norm_cm(p->order, p->B, p->N, p->C)) a.chunks = ceil_div(a.N, 64);
+  if (norm_cm(p->order, p->B, p->N, p->C)) a.chunks = ceil_div(a.N, cm_map(p->B, p->N, p->C).points);
   else if (!p->gate_cloud) { a.N *= a.B; a.B = 1; }  // nothing differs from cloud to cloud: one run of rows
   a.kind1 = p->kind; a.kind2 = p->next_kind;
   a.exit = p->y != nullptr; a.next = p->next_kind != CL3D_NORM_NONE;
@@ -916,7 +948,7 @@ size_t point_norm_workspace(int B, int N, int C, int flags) {
   if (B <= 0 || N <= 0 || C <= 0) return 0;
   Arena ar(nullptr);
   const int order = (flags >> 2) & 1;
-  if (norm_cm(order, B, N, C)) return (flags >> 8) & 1 ? (size_t)B * ceil_div(N, 64) * 5 * (size_t)C * sizeof(float) : 0;
+  if (norm_cm(order, B, N, C)) return (flags >> 8) & 1 ? (size_t)B * ceil_div(N, cm_map(B, N, C).points) * 5 * (size_t)C * sizeof(float) : 0;
   if (order == CL3D_CHANNEL_MAJOR && N > 1 && C > 1)
     for (int q = 0; q < ((flags >> 3) & 31); ++q) ar.take((size_t)B * N * C * elem_bytes(flags & 3));
   // partial rows of the backward pass: at most kNormBwdGroups + B workgroups

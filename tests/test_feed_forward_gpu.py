@@ -307,13 +307,14 @@ def test_every_form_of_the_exit(norm, next_norm, gate):
 
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("size", [(1, 4, 2), (5, 8, 64), (3, 72, 65), (2, 128, 63), (1, 132, 130), (2, 144, 77), (2, 256, 200), (70000, 4, 3),
-                                  (2, 260, 70), (2, 126, 70)], ids=lambda s: "x".join(map(str, s)))
+                                  (2, 260, 70), (2, 126, 70), (70, 288, 300), (9, 512, 40), (3, 772, 33), (2, 1024, 17), (1, 1028, 20), (300, 36, 70),
+                                  (300, 200, 70)], ids=lambda s: "x".join(map(str, s)))
 def test_channel_major_features_match_their_formula(size, kind):
     """Up to 256 channels, a multiple of four: read as they lie; others by transposed copies."""
     k = (size[1] // 4 + len(kind)) % 3
     norm_check(size, kind, ["rms", "layer", "none"][k], [None, "rms", "layer"][k], ["channel", "none", "channel"][k], [0.0, 0.3, 0.1][k], "channel",
                kind, offset=2 ** 32 - 5, bias=k != 0)
-    if size[0] <= 5:
+    if size[0] <= 300:
         norm_check(size, kind, "layer", "rms", "cloud", 0.3, "channel", "f32", bias=k == 0)
 
 
