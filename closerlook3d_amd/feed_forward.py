@@ -78,7 +78,10 @@ def _point_major(t):
     if t.dim() == 2:
         return t.is_contiguous()
     (_, C, N), s = t.shape, t.stride()
-    return (s[1] == 1 and s[2] == C and s[0] == C * N) or t.transpose(1, 2).is_contiguous()
+    if s[1] == 1:
+        return (s[2] == C and s[0] == C * N) or t.transpose(1, 2).is_contiguous()
+    # (a stride other than 1 counts where there is more than one channel)
+    return (C == 1 or t.numel() == 0) and t.transpose(1, 2).is_contiguous()
 
 
 def _aligned(t):
@@ -90,9 +93,7 @@ def _order(t):
     """(dense tensor, its memory order)."""
     if _point_major(t):
         return _aligned(t), _POINT
-    if t.dim() == 2:
-        return _aligned(t.contiguous()), _POINT
-    return _aligned(t.contiguous()), _CHANNEL
+    return _aligned(t if t.is_contiguous() else t.contiguous()), _POINT if t.dim() == 2 else _CHANNEL
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # (torch.cuda.current_stream() builds an object: 3.5 us a call)
@@ -120,10 +121,6 @@ def _empty(shape, order, dtype, device):
         B, C, N = shape
         return torch.empty_strided(shape, (N * C, 1, C), dtype=dtype, device=device)
     return torch.empty(shape, dtype=dtype, device=device)
-
-
-def _zeros(shape, order, dtype, device):
-    return _empty(shape, order, dtype, device).zero_()
 
 
 def _swap(src, B, R, C, dst):
@@ -220,7 +217,8 @@ def _ffn_forward(x, w_gate, w_up, w_down, activation, precision, keep_hidden):
     w_gate, w_up = _aligned(w_gate.contiguous()), _aligned(w_up.contiguous())
     w_down = None if w_down is None else _aligned(w_down.contiguous())
     H = w_gate.shape[0]
-    y = _empty((shape[0], C if w_down is not None else H) + tuple(shape[2:]), order, x.dtype, device)
+    # (empty_like: a dense tensor's memory order, at a third of the host time)
+    y = torch.empty_like(x) if w_down is not None else _empty((shape[0], H) + tuple(shape[2:]), order, x.dtype, device)
     hidden = None
     if keep_hidden and w_down is not None and B * N > _FEW_POINTS:
         hidden = torch.empty((3 if dtype == 0 and precision == 0 else 1, B * N, (H + 7) // 8 * 8), dtype=torch.int16, device=device)
@@ -252,7 +250,7 @@ class _GatedFeedForward(Function):
         order, B, C, N, H, activation, precision = ctx.args
         need = ctx.needs_input_grad
         new = torch.empty_like if B * N else torch.zeros_like
-        dx = _empty(x.shape, order, x.dtype, x.device) if need[0] else None
+        dx = torch.empty_like(x) if need[0] else None
         dwg = new(w_gate) if need[1] else None
         dwu = new(w_up) if need[2] else None
         dwd = new(w_down) if w_down is not None and need[3] else None
@@ -300,7 +298,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down=None, activation='silu', precisio
 def _norm_forward(x, y, weight, bias, gate, next_weight, next_bias, rng, opts, need_grad):
     """(out, next) in x's memory order, and what a backward pass needs."""
     kind, next_kind, eps, next_eps, scale, p = opts
-    shape, dtype, device = x.shape, x.dtype, x.device
+    dtype, device = x.dtype, x.device
     B, C, N = _sizes(x)
     x, order = _order(x)
     y = None if y is None else _as_order(y, order)
@@ -312,8 +310,8 @@ def _norm_forward(x, y, weight, bias, gate, next_weight, next_bias, rng, opts, n
         if t is not None:
             t = (t if not f32 or t.dtype == torch.float32 else t.float()).contiguous()
         held.append(t)
-    out = _empty(shape, order, dtype, device) if y is not None else None
-    nxt = _empty(shape, order, dtype, device) if next_kind else None
+    out = torch.empty_like(x) if y is not None else None
+    nxt = torch.empty_like(x) if next_kind else None
     stats = torch.empty((B * N, 4), dtype=torch.float32, device=device) if need_grad else None
     sizes = (B, N, C, _DTYPES[dtype], f32, kind, next_kind, gate is not None and gate.dim() == 2, scale, eps, next_eps, order, p)
     if B * N:
@@ -326,7 +324,8 @@ def _norm_forward(x, y, weight, bias, gate, next_weight, next_bias, rng, opts, n
         with _lib.on_device(device):
             _lib.check(_lib.lib().cl3d_norm_residual_fwd(ctypes.byref(block), _stream(device)))
     # (an exit alone: x is not looked at again)
-    return out, nxt, (x if next_kind else None, y, *held, rng, stats), (order, shape, dtype, sizes, [None if t is None else t.dtype for t in params])
+    kept = (x if next_kind else None, y, *held, rng, stats)
+    return out, nxt, kept, (order, sizes, [None if t is None else t.dtype for t in params])
 
 
 class _NormResidual(Function):
@@ -344,7 +343,7 @@ class _NormResidual(Function):
     @once_differentiable
     def backward(ctx, dout, dnext):
         x, y, weight, bias, gate, next_weight, next_bias, rng, stats = ctx.saved_tensors
-        order, shape, dtype, sizes, types = ctx.args
+        order, sizes, types = ctx.args
         B, N, C = sizes[:3]
         need, device = ctx.needs_input_grad, stats.device
         _check_capture(ctx, device)
@@ -352,8 +351,9 @@ class _NormResidual(Function):
             return (None,) * 9
         dout = None if dout is None else _as_order(dout, order)
         dnext = None if dnext is None else _as_order(dnext, order)
-        dx = _empty(shape, order, dtype, device) if need[0] else None
-        dy = _empty(shape, order, dtype, device) if y is not None and need[1] else None
+        like = x if y is None else y  # (one of them was kept, in this memory order)
+        dx = torch.empty_like(like) if need[0] else None
+        dy = torch.empty_like(like) if y is not None and need[1] else None
         new = torch.empty_like if B * N else torch.zeros_like
         grads = [new(t) if t is not None and n else None for t, n in zip((weight, bias, gate, next_weight, next_bias), need[2:7])]
         if B * N:
