@@ -124,20 +124,46 @@ static void tile_shape(int R, int C, int *tr, int *tc) {
   *tc = TC;
 }
 
-// [b][R][C] -> [b][C][R], 16-bit elements: a 64 x 64 tile through LDS, rows of 66 elements (33 banks: conflict-free both ways)
+// [b][R][C] -> [b][C][R], 16-bit elements.  R and C multiples of 8, pointers on 16 bytes: a wave has a tile of 64 x 64, a lane 8 x 8
+// of it, in registers from eight 16-byte loads to eight 16-byte stores; eight lanes side by side store 128 bytes of a column.
+// Measured: 16 x 144 x 4096 (38 MB read and written) 7 us, 5.3 TB/s; through LDS two bytes at a time 17.
+__global__ __launch_bounds__(256) void transpose16x8_kernel(const unsigned short *__restrict__ src, int R, int C, unsigned short *__restrict__ dst) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long long r = (long long)blockIdx.y * 64 + 8 * (lane & 7), c = ((long long)blockIdx.x * 4 + wave) * 64 + 8 * (lane >> 3);
+  if (r >= R || c >= C) return;
+  src += (long long)blockIdx.z * R * C + r * C + c;
+  dst += (long long)blockIdx.z * R * C + c * R + r;
+  union { uint4 v; unsigned d[4]; } in[8], out;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) in[u].v = *reinterpret_cast<const uint4 *>(src + (long long)u * C);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)  // the u & 1 halves of two rows, the even row's in the low half
+      out.d[k] = __builtin_amdgcn_perm(in[2 * k + 1].d[u >> 1], in[2 * k].d[u >> 1], u & 1 ? 0x07060302u : 0x05040100u);
+    *reinterpret_cast<uint4 *>(dst + (long long)u * R) = out.v;
+  }
+}
+
+// other sizes: a 64 x 64 tile through LDS, rows of 66 elements (33 banks: conflict-free both ways)
 __global__ __launch_bounds__(256) void transpose16_kernel(const unsigned short *__restrict__ src, int R, int C, unsigned short *__restrict__ dst) {
   __shared__ unsigned short tile[64][66];
-  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
   src += (long long)blockIdx.z * R * C;
   dst += (long long)blockIdx.z * R * C;
-  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-    const int r = e >> 6, c = e & 63;
-    if (r0 + r < R && c0 + c < C) tile[r][c] = src[(long long)(r0 + r) * C + c0 + c];
+  unsigned short v[16];
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {  // all 16 loads of the thread in flight
+    const int r = r0 + ty + 4 * u, c = c0 + tx;
+    v[u] = src[(long long)(r < R ? r : R - 1) * C + (c < C ? c : C - 1)];
   }
+#pragma unroll
+  for (int u = 0; u < 16; ++u) tile[ty + 4 * u][tx] = v[u];
   __syncthreads();
-  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-    const int r = e & 63, c = e >> 6;
-    if (r0 + r < R && c0 + c < C) dst[(long long)(c0 + c) * R + r0 + r] = tile[r][c];
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    const int c = c0 + ty + 4 * u, r = r0 + tx;
+    if (c < C && r < R) dst[(long long)c * R + r] = tile[tx][ty + 4 * u];
   }
 }
 
@@ -186,7 +212,10 @@ extern "C" int cl3d_transpose16(const void *src, int B, int R, int C, void *dst,
   if (B == 0 || R == 0 || C == 0) return CL3D_OK;
   CL3D_REQUIRE(src && dst, "transpose16: null pointer");
   if (B > 65535 || R > 65535 * 64) return fail(CL3D_E_UNSUPPORTED, "transpose16: more than 65535 clouds or 4194240 rows");
-  hipLaunchKernelGGL(transpose16_kernel, dim3(ceil_div(C, 64), ceil_div(R, 64), B), dim3(256), 0, (hipStream_t)stream,
-                     static_cast<const unsigned short *>(src), R, C, static_cast<unsigned short *>(dst));
+  const auto *s = static_cast<const unsigned short *>(src);
+  auto *d = static_cast<unsigned short *>(dst);
+  const bool vec = ((R | C) & 7) == 0 && ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 15u) == 0;
+  if (vec) hipLaunchKernelGGL(transpose16x8_kernel, dim3(ceil_div(C, 256), ceil_div(R, 64), B), dim3(256), 0, (hipStream_t)stream, s, R, C, d);
+  else hipLaunchKernelGGL(transpose16_kernel, dim3(ceil_div(C, 64), ceil_div(R, 64), B), dim3(256), 0, (hipStream_t)stream, s, R, C, d);
   return check_launch("cl3d_transpose16");
 }

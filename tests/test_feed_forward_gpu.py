@@ -16,6 +16,19 @@ def gen(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("size", [(1, 8, 8), (3, 16, 264), (2, 72, 520), (2, 144, 70), (1, 201, 65), (2, 2, 300), (70, 64, 1000)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_memory_orders_there_and_back(size, kind):
+    x = torch.randn(size, device="cuda", generator=gen(1)).to(TYPES[kind])
+    y = ff.to_point_major(x)
+    assert ff._point_major(y) and torch.equal(y, x)
+    z = ff.to_channel_major(y)
+    assert z.is_contiguous() and torch.equal(z, x)
+    off = torch.zeros((x.numel() + 1,), dtype=x.dtype, device="cuda")[1:].view(size).copy_(x)  # (starts off 16 bytes)
+    assert torch.equal(ff.to_point_major(off), x)
+
+
 def features(g, B, C, N, dtype, order="point", scale=1.0):
     rows = (torch.randn((B, N, C), device="cuda", generator=g) * scale).to(dtype)
     return rows.transpose(1, 2) if order == "point" else rows.transpose(1, 2).contiguous()
