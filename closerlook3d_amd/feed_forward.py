@@ -10,9 +10,9 @@ configuration asks for it).
 
 Tensors are features (B, C, N), as everywhere in this package, or rows (R, C): pooled vectors, the input of nn.Linear.  (B, C, N)
 features may lie channel-major (dense) or point-major (a transposed view of dense (B, N, C) rows); results lie as the first
-input does.  The kernels work on point-major rows: of channel-major features they take and leave a transposed copy, so a chain
-of these operators is best kept point-major (to_point_major, once, at its beginning; FeedForwardBlock does).  Types: float32,
-bfloat16, float16.  Everything is formed in f32 and rounded once, to the type of the result.
+input does.  The norms read channel-major features as they lie (up to 1024 channels, a multiple of four); otherwise the kernels work
+on point-major rows and take and leave a transposed copy, so a chain of these operators is best kept point-major (to_point_major,
+once, at its beginning; FeedForwardBlock does).  Types: float32, bfloat16, float16.  Everything is formed in f32 and rounded once, to the type of the result.
 
 Points are independent of each other (only parameter gradients sum over them); padding points are computed like the others.  The
 results of a point depend on no other point, and every gradient is summed in a fixed order: bit-identical run to run.  There is no

@@ -575,7 +575,8 @@ int cl3d_gated_ffn_bwd(const void *x, const void *w_gate, const void *w_up, cons
 /* [B,R,C] -> [B,C,R] of 16-bit elements (cl3d_transpose: f32) */
 int cl3d_transpose16(const void *src, int B, int R, int C, void *dst, cl3d_stream_t stream);
 
-/* Exit of a block and entry of the next, one pass over the points (channel-major tensors: by way of transposed copies in ws):
+/* Exit of a block and entry of the next, one pass over the points (channel-major tensors of more than 1024 channels, or not a
+ * multiple of 4: by way of transposed copies in ws):
  *     n = norm(y) weight + bias;  out = residual_scale x + gate * drop(n);  next = next_norm(out) next_weight + next_bias
  * y NULL: there is no block to leave, next = next_norm(x) next_weight + next_bias.  next_kind CL3D_NORM_NONE: no entry.
  * rms: v / sqrt(mean v^2 + eps); layer: (v - mean) / sqrt(var + eps), over the channels of a point.  weight, bias, gate,
