@@ -16,14 +16,15 @@ once, at its beginning; FeedForwardBlock does).  Types: float32, bfloat16, float
 
 Points are independent of each other (only parameter gradients sum over them); padding points are computed like the others.  The
 results of a point depend on no other point, and every gradient is summed in a fixed order: bit-identical run to run.  There is no
-CPU fallback.  The operators can be captured into HIP graphs, forward and backward.
+CPU fallback.  The operators can be captured into HIP graphs, forward and backward.  A forward-mode tangent, a derivative of a
+gradient and a torch.jit.trace are refused.
 """
 import ctypes
 import weakref
 
 import torch
 import torch.nn as nn
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -41,7 +42,17 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+_is_tracing = torch._C._is_tracing
+
+
+def _check_trace(who):
+    # (a trace holds the allocations of a call and nothing of what the launches put there)
+    if _is_tracing():
+        raise RuntimeError(f"{who}: cannot be traced by torch.jit.trace (capture a HIP graph instead)")
+
+
 def _check_features(x, who, name='x'):
+    _check_trace(who)
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{who}: {name} is a tensor, got {type(x).__name__}")
     if not x.is_cuda:
@@ -174,8 +185,11 @@ def to_channel_major(features):
     return features if features.is_contiguous() else _Reorder.apply(features, _CHANNEL)
 
 
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _recorded(*tensors):
+    """Whether a call goes through its autograd function: a gradient is wanted, or a forward-mode level is open (the function refuses
+    a tangent; the launches alone would lose it).  Other calls do without the node, which costs as much host time as the rest of a
+    small call."""
+    return forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
 
 
 # Autograd runs a leaf's gradient on the stream that was current when the leaf's node was made, and keeps that node while any
@@ -291,7 +305,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down=None, activation='silu', precisio
         raise ValueError(f"{who}: precision is one of {sorted(_PRECISIONS)}, got {precision!r}")
     args = (x, w_gate, w_up, w_down, _ACTIVATIONS[activation], _PRECISIONS[precision])
     # (without a gradient: no autograd node)
-    return _GatedFeedForward.apply(*args) if _wants_grad(x, w_gate, w_up, w_down) else _ffn_forward(*args, False)[0]
+    return _GatedFeedForward.apply(*args) if _recorded(x, w_gate, w_up, w_down) else _ffn_forward(*args, False)[0]
 
 
 # ---------------------------------------------------------------------------------------------- norms around a block
@@ -391,7 +405,7 @@ def point_norm(x, weight=None, bias=None, kind='rms', eps=1e-6):
     _check_param(weight, (C,), x, who, 'weight')
     _check_param(bias, (C,), x, who, 'bias')
     args = (x, None, None, None, None, weight, bias, None, (0, _NORMS[kind], 0.0, float(eps), 1.0, 0.0))
-    return (_NormResidual.apply(*args) if _wants_grad(x, weight, bias) else _norm_forward(*args, False))[1]
+    return (_NormResidual.apply(*args) if _recorded(x, weight, bias) else _norm_forward(*args, False))[1]
 
 
 def norm_gate_residual(x, y, weight=None, bias=None, gate=None, residual_scale=1.0, kind='rms', eps=1e-6, p=0.0, rng=None,
@@ -426,7 +440,7 @@ def norm_gate_residual(x, y, weight=None, bias=None, gate=None, residual_scale=1
         _check_rng(rng, x, who)
     args = (x, y, weight, bias, gate, next_weight, next_bias, rng if p > 0 else None,
             (_NORMS[kind], _NORMS[next_kind], float(eps), float(eps if next_eps is None else next_eps), float(residual_scale), p))
-    need = _wants_grad(x, y, weight, bias, gate, next_weight, next_bias)
+    need = _recorded(x, y, weight, bias, gate, next_weight, next_bias)
     out, nxt = _NormResidual.apply(*args) if need else _norm_forward(*args, False)[:2]
     return out if next_kind == 'none' else (out, nxt)
 
@@ -477,6 +491,7 @@ def dropout(x, p, rng):
     the device, by the backward pass too: they must not be changed in between (autograd notices).  A dropped element is 0 whatever
     it was.  p = 0 returns x, p = 1 zeros.  x: any shape; float32, bfloat16 or float16."""
     who = 'dropout'
+    _check_trace(who)
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{who}: x is a tensor, got {type(x).__name__}")
     if not x.is_cuda:
@@ -487,7 +502,7 @@ def dropout(x, p, rng):
     if p == 0.0:
         return x
     _check_rng(rng, x, who)
-    return _Dropout.apply(x, p, rng) if _wants_grad(x) else _drop(x, p, rng)
+    return _Dropout.apply(x, p, rng) if _recorded(x) else _drop(x, p, rng)
 
 
 class CounterRng:
@@ -505,6 +520,7 @@ class CounterRng:
     def take(self, n):
         if n < 0:
             raise ValueError(f"CounterRng.take: {n} elements")
+        _check_trace('CounterRng.take')
         out = torch.empty_like(self.state)
         with _lib.on_device(out.device):
             _lib.check(_lib.lib().cl3d_rng_take(_p(self.state), (n + 3) // 4, _p(out), _stream(out.device)))
