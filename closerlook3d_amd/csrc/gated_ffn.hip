@@ -20,11 +20,12 @@
 //     whose row index is contiguous (Wd in dh, Wg / Wu in dX, all operands of the weight gradients) lies as [64 k][row] and is
 //     read by ds_read_b64_tr_b16, which hands a lane four k of its row: no operand is transposed in memory;
 //   * workgroups are numbered so that neighbours in i, which share the rows of Q, run on one XCD and share its L2.
-// f32 tensors: an f32 value is the exact sum of three bf16 values (8 significant bits each, by truncation: planes 0, 1, 2); a
-// product takes the six largest of the nine partial products on the bf16 units, smallest first, into one f32 accumulator.  What is
-// left out is below 2^-23 of |x||y|, as much as the rounding of an f32 product.  Six passes at the bf16 rate outrun the f32 MFMA
-// (1/16 of it).  A tile holds the three planes of 32 k, so each fragment is read once for its two or three products.  A value
-// that is not finite takes part in the product of the leading planes only, so an infinity stays one (not_finite below).
+// f32 tensors: an f32 value is the exact sum of three bf16 values (planes 0, 1, 2, each what is left rounded to nearest); a product
+// takes the six largest of the nine partial products on the bf16 units, smallest first, into one f32 accumulator.  Plane 1 is at most
+// 2^-8 of the value and plane 2 2^-17, so what is left out is below 2^-24 of |x||y|, of either sign: less than the rounding of an
+// f32 product.  Six passes at the bf16 rate outrun the f32 MFMA (1/16 of it).  A tile holds the three planes of 32 k, so each
+// fragment is read once for its two or three products.  A value that is not finite takes part in the product of the leading planes
+// only, so an infinity stays one (not_finite below).
 // Measured at 16 384 x 288 x 1152 in bf16: projections 37 us (590 TFLOP/s), their backward twin 68 (480), Y 19 (570), dX 35 (620),
 // the three weight gradients 61 (535); 16 384 x 144 x 576 in f32, counting f32 operations: 66 (82), 107 (76), 27 (100), 53 (103), 81 (100).
 #include "ff_common.h"
@@ -304,23 +305,26 @@ __device__ __forceinline__ void activate(int act, float g, float &value, float &
   }
 }
 
-// an f32 value as the exact sum of three bf16 values by truncation (not finite: the leading one alone)
+// an f32 value as the exact sum of three bf16 values, each rounded to nearest (8, 8 and the last 8 of 24 bits; truncated, the products
+// left out would be up to 2^-21 of |x||y| and all of its sign).  Where rounding would make an infinity of a finite value the leading
+// one is truncated; what is not finite is the leading one alone.
 struct Split {
   u16 p[3];
 };
 __device__ __forceinline__ Split split3(float x) {
-  const unsigned b = __float_as_uint(x), hi = b & 0xffff0000u;
+  const unsigned b = __float_as_uint(x);
   Split s;
-  s.p[0] = (u16)(hi >> 16);
   if ((b & 0x7f800000u) == 0x7f800000u) {
+    s.p[0] = (u16)(b >> 16);
     if (b & 0x007fffffu) s.p[0] |= 0x40;  // a NaN whose payload sits in the low half stays a NaN
     s.p[1] = s.p[2] = 0;
     return s;
   }
-  const float r = x - __uint_as_float(hi);
-  const unsigned mid = __float_as_uint(r) & 0xffff0000u;
-  s.p[1] = (u16)(mid >> 16);
-  s.p[2] = (u16)(__float_as_uint(r - __uint_as_float(mid)) >> 16);
+  s.p[0] = Bf16::put(x);
+  if ((s.p[0] & 0x7f80u) == 0x7f80u) s.p[0] = (u16)(b >> 16);
+  const float r = x - Bf16::get(s.p[0]);
+  s.p[1] = Bf16::put(r);
+  s.p[2] = Bf16::put(r - Bf16::get(s.p[1]));
   return s;
 }
 

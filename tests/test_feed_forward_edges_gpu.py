@@ -54,3 +54,40 @@ def test_a_trace_is_refused(name):
         with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="traced"):
             torch.jit.trace(calls[name], (x.clone().requires_grad_(grad),), check_trace=False)
     assert rng.state.tolist() == [5, 0]
+
+
+# --------------------------------------------------------------------------------------------------------- f32 at f32 accuracy
+def test_an_f32_product_is_as_good_as_one():
+    """One product of two f32 values, in h = relu(a b) * 1 (the other terms of every sum are zero), against 64 bits.
+
+    The kernel forms six of the nine products of two values of three planes.  What it leaves out is at most 2^-24 of |a b|: a plane
+    holds 8 bits and is rounded to nearest, so the second is at most 2^-8 of the value and the third 2^-17, and the products left
+    out are second by third (twice) and third by third.  Six additions in f32, the largest last: at most a step (2^-23) of the
+    result for the last one, whichever way it rounds, and of its 2^-7 th part for the five before.  The sum is below 1.6 x 2^-23."""
+    g = gen(4)
+    R, H = 96, 512
+    a, b = torch.randn((R,), device="cuda", generator=g).abs() + 0.25, torch.randn((H,), device="cuda", generator=g).abs() + 0.25
+    worst = torch.tensor([0x3f80ffff, 0x3f81ffff, 0x3fffffff, 0x3f807fff, 0x3f808000, 0x3fff8000, 0x3f800001], dtype=torch.int32, device="cuda")
+    a[:7] = b[:7] = worst.view(torch.float32)
+    x = torch.stack([a, torch.ones_like(a)], 1)
+    w_gate, w_up = torch.stack([b, torch.zeros_like(b)], 1), torch.stack([torch.zeros_like(b), torch.ones_like(b)], 1)
+    h = ff.gated_feed_forward(x, w_gate, w_up, activation='relu').double()
+    want = a.double()[:, None] * b.double()[None]
+    off = ((h - want) / want).abs() * 2.0 ** 23
+    assert float(off.max()) <= 1.6, float(off.max())
+
+
+def test_f32_values_at_the_ends_of_their_range():
+    """The largest finite values (a leading plane that rounded up would be an infinity) and the smallest normal ones, each through a
+    product by one: the value itself."""
+    ends = ["0x1.fffffep127", "0x1.ff0002p127", "0x1.fep127", "0x1p-126", "0x1.8p-126", "0x1.00fffep0", "0x1.fffffep-100"]
+    v = torch.tensor([float.fromhex(s) for s in ends], device="cuda")
+    n = len(ends)
+    x = torch.zeros((80, n + 1), device="cuda")
+    x[:n, :n] = torch.diag(v)
+    x[:, n] = 1.0  # for the second projection
+    w_gate, w_up = torch.zeros((n, n + 1), device="cuda"), torch.zeros((n, n + 1), device="cuda")
+    w_gate[:, :n] = torch.eye(n, device="cuda")
+    w_up[:, n] = 1.0
+    h = ff.gated_feed_forward(x, w_gate, w_up, activation='relu')
+    assert torch.equal(h[:n], torch.diag(v)) and not h[n:].any()
