@@ -333,6 +333,7 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
           hat1[q][e] = (hat1[q][e] - st[0]) * st[1];
           nk[q][e] = __builtin_fmaf(hat1[q][e], w1[q][e], b1[q][e]);
           if (DROP) nk[q][e] = stays[q][e] ? nk[q][e] * a.drop.scale : 0.f;
+          if (!live) hat1[q][e] = nk[q][e] = 0.f;  // (its gradients are zeros, but 0 x inf is a NaN)
         }
       }
     }
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           if (a.exit) hat[q][e] = __builtin_fmaf(a.alpha, hat[q][e], gate[q][e] * nk[q][e]);
-          hat[q][e] = (hat[q][e] - st[2]) * st[3];
+          hat[q][e] = live ? (hat[q][e] - st[2]) * st[3] : 0.f;
           s_w2[q][e] = __builtin_fmaf(dh[q][e], hat[q][e], s_w2[q][e]);
           if (BIAS) s_b2[q][e] += dh[q][e];
           dh[q][e] *= w2[q][e];
@@ -383,7 +384,7 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
           s_gate[q][e] = __builtin_fmaf(dm, nk[q][e], s_gate[q][e]);
           if (DROP) dm = stays[q][e] ? dm * a.drop.scale : 0.f;
           dm *= gate[q][e];
-          s_w1[q][e] = __builtin_fmaf(dm, hat1[q][e], s_w1[q][e]);
+          s_w1[q][e] = __builtin_fmaf(dm, DROP && !stays[q][e] ? 0.f : hat1[q][e], s_w1[q][e]);  // (dropped: nothing, whatever y is)
           if (BIAS) s_b1[q][e] += dm;
           dm *= w1[q][e];
           t1 = __builtin_fmaf(dm, hat1[q][e], t1);
@@ -398,8 +399,12 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
           row_sum<TPR>(p1, p2, s_red);
           p1 *= inv_c;
           p2 = a.kind1 == CL3D_NORM_LAYER ? p2 * inv_c : 0.f;
-        } else {
+        } else {  // (y does not enter its own gradient, whatever it is)
           p1 = p2 = 0.f;
+#pragma unroll
+          for (int q = 0; q < NV; ++q)
+#pragma unroll
+            for (int e = 0; e < V; ++e) hat1[q][e] = 0.f;
         }
         if (live)
 #pragma unroll
@@ -657,6 +662,7 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_bwd_kernel(NormArgs a) 
         hat1[q][e] = (hat1[q][e] - st[0]) * st[1];
         nk[q][e] = __builtin_fmaf(hat1[q][e], par[0][c0[q] + e], par[1][c0[q] + e]);
         if (DROP) nk[q][e] = stays[q][e] ? nk[q][e] * a.drop.scale : 0.f;
+        if (!live) hat1[q][e] = nk[q][e] = 0.f;  // (its gradients are zeros, but 0 x inf is a NaN)
       }
     }
   }
@@ -668,7 +674,7 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_bwd_kernel(NormArgs a) 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (a.exit) hat[q][e] = __builtin_fmaf(a.alpha, hat[q][e], par[2][c0[q] + e] * nk[q][e]);
-        hat[q][e] = (hat[q][e] - st[2]) * st[3];
+        hat[q][e] = live ? (hat[q][e] - st[2]) * st[3] : 0.f;
       }
       if (partial) {
         if (a.w2) flush(3, c0[q], dh[q][0] * hat[q][0], dh[q][1] * hat[q][1], dh[q][2] * hat[q][2], dh[q][3] * hat[q][3]);
@@ -716,8 +722,12 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_bwd_kernel(NormArgs a) 
       if (DROP) d[q][e] = stays[q][e] ? d[q][e] * a.drop.scale : 0.f;
       d[q][e] *= par[2][c0[q] + e];
     }
-    if (partial && a.w1)
-      flush(0, c0[q], d[q][0] * hat1[q][0], d[q][1] * hat1[q][1], d[q][2] * hat1[q][2], d[q][3] * hat1[q][3]);
+    if (partial && a.w1) {
+      float t[4];  // (dropped: nothing, whatever y is)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] = DROP && !stays[q][e] ? 0.f : d[q][e] * hat1[q][e];
+      flush(0, c0[q], t[0], t[1], t[2], t[3]);
+    }
     if (partial && a.b1) flush(1, c0[q], d[q][0], d[q][1], d[q][2], d[q][3]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -727,8 +737,12 @@ __global__ __launch_bounds__(64 * kCmWaves) void norm_cm_bwd_kernel(NormArgs a) 
     }
   }
   if (!a.dy) return;
-  if (a.kind1 == CL3D_NORM_NONE) {
+  if (a.kind1 == CL3D_NORM_NONE) {  // (y does not enter its own gradient, whatever it is)
     p1 = p2 = 0.f;
+#pragma unroll
+    for (int q = 0; q < QN; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) hat1[q][e] = 0.f;
   } else {
     p1 = wave_sum<P>(p1, s[2], wave, lane, waves) * inv_c;
     p2 = a.kind1 == CL3D_NORM_LAYER ? wave_sum<P>(p2, s[3], wave, lane, waves) * inv_c : 0.f;

@@ -91,3 +91,43 @@ def test_f32_values_at_the_ends_of_their_range():
     w_up[:, n] = 1.0
     h = ff.gated_feed_forward(x, w_gate, w_up, activation='relu')
     assert torch.equal(h[:n], torch.diag(v)) and not h[n:].any()
+
+
+# -------------------------------------------------------------------------------------------- what is not finite, without a norm
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("order", ["point", "channel"])
+@pytest.mark.parametrize("size", [(1, 40, 70), (2, 33, 21), (1, 1024, 19), (3, 8, 5)], ids=lambda s: "x".join(map(str, s)))
+def test_gradients_around_what_is_not_finite(size, order, kind):
+    """kind 'none': the gradient of y does not depend on y, whatever y is; a dropped element adds nothing to a parameter's gradient;
+    an infinity that stays makes its column's gradient an infinity of the right sign, also in the last point (where idle lanes
+    work on the same point)."""
+    B, C, N = size
+    dtype, g = TYPES[kind], gen(5)
+    rng = torch.tensor([11, 7], device="cuda")
+    x, y = features(g, B, C, N, dtype, order), features(g, B, C, N, dtype, order)
+    bad = y.clone(memory_format=torch.preserve_format)
+    places = [(B - 1, 3, N - 1, float('inf')), (B - 1, 5, N - 1, float('-inf')), (0, 6, 1, float('inf')), (0, 7, 2, float('nan'))]
+    for b, c, n, value in places:
+        bad[b, c, n] = value
+        y[b, c, n] = 0.0
+    w, gate = vector(g, C, dtype=dtype, mean=2.0), vector(g, C, dtype=dtype, mean=2.0)
+    given = features(g, B, C, N, dtype, order)
+    mask = ref.keep(11, 7, 0.5, (B * N, C)).reshape(B, N, C)
+    for p in (0.0, 0.5):
+        def grads(y):
+            leaves = [t.detach().requires_grad_(True) for t in (x, y, w, gate)]
+            o = ff.norm_gate_residual(leaves[0], leaves[1], leaves[2], gate=leaves[3], kind='none', p=p, rng=rng)
+            return torch.autograd.grad(o, leaves, given)
+        want, got = grads(y), grads(bad)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        sums = {}
+        for b, c, n, value in places:
+            if p == 0 or bool(mask[b, n, c]):
+                sums[c] = value
+        other = [c for c in range(C) if c not in sums]
+        for k, coefficient in ((2, gate), (3, w)):
+            assert torch.equal(got[k][other], want[k][other]), (p, k)
+            for c, value in sums.items():
+                b, n = next((b, n) for b, cc, n, _ in places if cc == c)
+                sign = float(given[b, c, n]) * float(coefficient[c])
+                assert float(got[k][c].float()) == sign * value or value != value and bool(got[k][c].isnan()), (p, k, c)
