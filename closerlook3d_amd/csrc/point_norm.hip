@@ -1014,6 +1014,9 @@ extern "C" int cl3d_norm_residual_bwd(const cl3d_norm_residual *p, cl3d_stream_t
   CL3D_REQUIRE(p->stats && (p->dout || p->dnext), "norm_residual_bwd: null pointer");
   CL3D_REQUIRE(!p->dnext || (a.next && p->x), "norm_residual_bwd: a gradient of a norm that was not formed");
   CL3D_REQUIRE(!p->dout || a.exit, "norm_residual_bwd: a gradient of a sum that was not formed");
+  CL3D_REQUIRE((!p->dweight || p->weight) && (!p->dbias || p->bias) && (!p->dgate || p->gate) &&
+                   (!p->dnext_weight || (a.next && p->next_weight)) && (!p->dnext_bias || (a.next && p->next_bias)),
+               "norm_residual_bwd: a gradient of a parameter that is not there");
   const hipStream_t st = (hipStream_t)stream;
   const bool sums = p->dweight || p->dbias || p->dgate || p->dnext_weight || p->dnext_bias;
   const void *x = p->dnext ? p->x : nullptr;  // (without the entry's gradient x is not looked at)

@@ -585,7 +585,7 @@ int cl3d_transpose16(const void *src, int B, int R, int C, void *dst, cl3d_strea
  * backward pass needs of the forward pass, besides its inputs (NULL: no backward pass follows).
  * Backward (x, y and the parameters as in the forward pass, out and next not read): dout, dnext are the gradients of out and
  * next (either may be NULL: zero); dx, dy and the parameters' gradients (shapes and types of what they belong to) NULL where not
- * wanted.  ws, 16-byte aligned: cl3d_workspace_bytes(CL3D_OP_POINT_NORM, B, N, 0, flags, C), copies being the number of feature
+ * wanted; a parameter that is not given has none.  ws, 16-byte aligned: cl3d_workspace_bytes(CL3D_OP_POINT_NORM, B, N, 0, flags, C), copies being the number of feature
  * tensors that the call is given, sums whether a parameter's gradient is wanted.  Sums over the points are taken in a fixed
  * order: bit-identical run to run. */
 #define CL3D_NORM_NONE 0

@@ -1,0 +1,33 @@
+"""CPU: what the feed-forward operators refuse before any launch, beyond what test_feed_forward.py asks."""
+import ctypes
+
+import pytest
+
+from closerlook3d_amd import _lib
+
+
+def _block(**kw):
+    base = dict(B=2, N=3, C=8, dtype=0, kind=1, next_kind=1, residual_scale=1.0, eps=1e-6, next_eps=1e-6)
+    return _lib.NormResidual(**{**base, **kw})
+
+
+@pytest.mark.parametrize("order", [0, 1])
+@pytest.mark.parametrize("name", ["weight", "bias", "gate", "next_weight", "next_bias"])
+def test_a_gradient_of_a_parameter_that_is_not_given_is_refused(name, order):
+    """It would be a sum of scratch that no kernel has written."""
+    lib = _lib.lib()
+    a = 1 << 20  # a 16-byte aligned number (no pointer is followed before the checks have passed)
+    given = dict(order=order, x=a, y=a, weight=a, bias=a, gate=a, next_weight=a, next_bias=a, stats=a, dout=a, dnext=a, dx=a, dy=a)
+    given[name] = None
+    rc = lib.cl3d_norm_residual_bwd(ctypes.byref(_block(**given, **{"d" + name: a})), None)
+    assert rc == -1 and "a parameter that is not there" in lib.cl3d_last_error_string().decode()
+
+
+@pytest.mark.parametrize("name", ["weight", "gate", "next_weight"])
+def test_a_gradient_of_a_step_that_is_not_taken_is_refused(name):
+    """A parameter of an exit, or of an entry, that the call does not have."""
+    lib = _lib.lib()
+    a = 1 << 20
+    given = dict(x=a, stats=a, dnext=a, dx=a, next_weight=a) if name != "next_weight" else dict(x=a, y=a, next_kind=0, stats=a, dout=a, next_weight=a)
+    rc = lib.cl3d_norm_residual_bwd(ctypes.byref(_block(**given, **{"d" + name: a})), None)
+    assert rc == -1 and "a parameter that is not there" in lib.cl3d_last_error_string().decode()
