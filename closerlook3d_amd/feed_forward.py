@@ -524,6 +524,7 @@ class CounterRng:
         out = torch.empty_like(self.state)
         with _lib.on_device(out.device):
             _lib.check(_lib.lib().cl3d_rng_take(_p(self.state), (n + 3) // 4, _p(out), _stream(out.device)))
+        torch.autograd.graph.increment_version(self.state)  # (a draw from `state` itself, still waiting for its backward pass)
         return out
 
 

@@ -131,3 +131,18 @@ def test_gradients_around_what_is_not_finite(size, order, kind):
                 b, n = next((b, n) for b, cc, n, _ in places if cc == c)
                 sign = float(given[b, c, n]) * float(coefficient[c])
                 assert float(got[k][c].float()) == sign * value or value != value and bool(got[k][c].isnan()), (p, k, c)
+
+
+# -------------------------------------------------------------------------------------------------------------------- dropout
+def test_a_generator_that_moved_on_is_noticed():
+    """A draw from the generator's own state tensor: take() changes it, and the backward pass says so."""
+    rng = ff.CounterRng(9, "cuda")
+    x = torch.randn((40,), device="cuda", requires_grad=True)
+    y = ff.dropout(x, 0.5, rng.state)
+    kept = rng.take(8)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, [x], torch.ones_like(y))
+    y = ff.dropout(x, 0.5, kept)
+    rng.take(8)  # (a draw of its own is not touched by the next)
+    (d,) = torch.autograd.grad(y, [x], torch.ones_like(y))
+    assert torch.equal(d != 0, y != 0)
