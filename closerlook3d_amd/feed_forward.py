@@ -435,6 +435,8 @@ def norm_gate_residual(x, y, weight=None, bias=None, gate=None, residual_scale=1
         _check_norm(x, next_kind, eps if next_eps is None else next_eps, who)
     _check_param(next_weight, (C,), x, who, 'next_weight')
     _check_param(next_bias, (C,), x, who, 'next_bias')
+    if isinstance(residual_scale, torch.Tensor) and residual_scale.requires_grad and torch.is_grad_enabled():
+        raise TypeError(f"{who}: residual_scale is a number (it has no gradient; a learned one: gate)")
     p = _check_p(p, who)
     if p > 0:
         _check_rng(rng, x, who)

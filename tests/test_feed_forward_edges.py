@@ -2,8 +2,11 @@
 import ctypes
 
 import pytest
+import torch
 
 from closerlook3d_amd import _lib
+from closerlook3d_amd import feed_forward as ff
+from tests.test_feed_forward import fake
 
 
 def _block(**kw):
@@ -31,3 +34,11 @@ def test_a_gradient_of_a_step_that_is_not_taken_is_refused(name):
     given = dict(x=a, stats=a, dnext=a, dx=a, next_weight=a) if name != "next_weight" else dict(x=a, y=a, next_kind=0, stats=a, dout=a, next_weight=a)
     rc = lib.cl3d_norm_residual_bwd(ctypes.byref(_block(**given, **{"d" + name: a})), None)
     assert rc == -1 and "a parameter that is not there" in lib.cl3d_last_error_string().decode()
+
+
+def test_a_learned_residual_scale_is_refused():
+    """The scale is read on the host: a tensor that wants a gradient would get none."""
+    scale = torch.nn.Parameter(torch.ones(()))
+    for x in (fake(4, 8), fake(2, 8, 3)):
+        with pytest.raises(TypeError, match="residual_scale is a number"):
+            ff.norm_gate_residual(x, x, residual_scale=scale)
