@@ -93,6 +93,7 @@ SIGNATURES = {
     "cl3d_norm_residual_fwd": [ctypes.POINTER(NormResidual), _P],
     "cl3d_norm_residual_bwd": [ctypes.POINTER(NormResidual), _P],
     "cl3d_dropout": [_P, _I, ctypes.c_longlong, ctypes.c_double, _P, _P, _P],
+    "cl3d_dropout_point_major": [_P, _I, _I, _I, _I, ctypes.c_double, _P, _P, _P],
     "cl3d_rng_take": [_P, ctypes.c_longlong, _P, _P],
     "cl3d_pwmlp_split_weight": [_P, _I, _I, _P, _P, _P],
     "cl3d_pwmlp_merge_weight_grad": [_P, _P, _I, _I, _I, _P, _P],

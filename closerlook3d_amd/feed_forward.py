@@ -478,10 +478,16 @@ class _Dropout(Function):
 
 
 def _drop(x, p, rng):
+    lib, dtype = _lib.lib(), _DTYPES[x.dtype]
+    if x.dim() == 3 and not x.is_contiguous() and _point_major(x):
+        out = torch.empty_like(x)
+        with _lib.on_device(x.device):
+            _lib.check(lib.cl3d_dropout_point_major(_p(x), dtype, *x.shape, p, _p(rng), _p(out), _stream(x.device)))
+        return out
     x = x.contiguous()
     out = torch.empty_like(x)
     with _lib.on_device(x.device):
-        _lib.check(_lib.lib().cl3d_dropout(_p(x), _DTYPES[x.dtype], x.numel(), p, _p(rng), _p(out), _stream(x.device)))
+        _lib.check(lib.cl3d_dropout(_p(x), dtype, x.numel(), p, _p(rng), _p(out), _stream(x.device)))
     return out
 
 
@@ -491,7 +497,8 @@ def dropout(x, p, rng):
     rng: int64 (2,) on x's device, (seed, offset).  Word i is number i % 4 of block offset + i / 4 of Philox 4x32-10 under the key
     `seed`: a draw of n elements uses ceil(n / 4) blocks (CounterRng hands out draws that do not overlap).  The numbers are read on
     the device, by the backward pass too: they must not be changed in between (autograd notices).  A dropped element is 0 whatever
-    it was.  p = 0 returns x, p = 1 zeros.  x: any shape; float32, bfloat16 or float16."""
+    it was.  p = 0 returns x, p = 1 zeros.  x: any shape; float32, bfloat16 or float16.  The result lies as x does where x is dense or
+    features in point-major memory, and is dense for other views; a gradient lies as the one that comes in."""
     who = 'dropout'
     _check_trace(who)
     if not isinstance(x, torch.Tensor):

@@ -612,6 +612,10 @@ int cl3d_norm_residual_bwd(const cl3d_norm_residual *p, cl3d_stream_t stream);
  * Philox 4x32-10 (counter offset + i / 4, key seed) is at least floor(p 2^32), and is multiplied by 1 / (1 - p); the others
  * become 0.  The same call on a gradient is the backward pass: no mask is stored.  p in [0, 1]. */
 int cl3d_dropout(const void *x, int dtype, long long n, double p, const int64_t *rng, void *out, cl3d_stream_t stream);
+/* The same of features that lie point-major, rows [B,N,C]: element (b, c, n) is number (b C + c) N + n of the draw, as it is where
+ * they lie channel-major. */
+int cl3d_dropout_point_major(const void *x, int dtype, int B, int C, int N, double p, const int64_t *rng, void *out,
+                             cl3d_stream_t stream);
 /* out = state, then state's offset += blocks: the counters of one draw (blocks = ceil(n / 4)), on the stream, so that a captured
  * step draws anew in every replay. */
 int cl3d_rng_take(int64_t *state, long long blocks, int64_t *out, cl3d_stream_t stream);

@@ -42,3 +42,15 @@ def test_a_learned_residual_scale_is_refused():
     for x in (fake(4, 8), fake(2, 8, 3)):
         with pytest.raises(TypeError, match="residual_scale is a number"):
             ff.norm_gate_residual(x, x, residual_scale=scale)
+
+
+def test_the_point_major_dropout_returns_codes_and_says_why():
+    lib = _lib.lib()
+    a = 1 << 20
+    for args, text in (((a, 4, 2, 8, 3, 0.5, a, a, None), "element type"), ((a, 0, 2, 8, -1, 0.5, a, a, None), "bad size"),
+                       ((a, 0, -2, 8, 3, 0.5, a, a, None), "bad size"), ((a, 0, 2, 8, 3, 1.5, a, a, None), "probability"),
+                       ((a, 0, 2, 8, 3, 0.5, None, a, None), "generator state"), ((a, 0, 2, 8, 3, 0.0, None, a, None), "null pointer"),
+                       ((None, 0, 2, 8, 3, 0.5, a, a, None), "null pointer"), ((a, 0, 2, 8, 3, 0.5, a, None, None), "null pointer")):
+        assert lib.cl3d_dropout_point_major(*args) == -1 and text in lib.cl3d_last_error_string().decode(), (args, lib.cl3d_last_error_string())
+    for sizes in ((0, 8, 3), (2, 0, 3), (2, 8, 0)):
+        assert lib.cl3d_dropout_point_major(None, 0, *sizes, 0.5, a, None, None) == 0

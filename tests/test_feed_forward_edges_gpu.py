@@ -146,3 +146,39 @@ def test_a_generator_that_moved_on_is_noticed():
     rng.take(8)  # (a draw of its own is not touched by the next)
     (d,) = torch.autograd.grad(y, [x], torch.ones_like(y))
     assert torch.equal(d != 0, y != 0)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("size", [(1, 1, 1), (1, 8, 1), (3, 5, 2), (2, 24, 3), (2, 33, 4), (1, 72, 65), (3, 144, 77), (2, 201, 130), (1, 2304, 9),
+                                  (70, 3, 31), (1, 2, 5001)], ids=lambda s: "x".join(map(str, s)))
+def test_dropout_of_point_major_features(size, kind):
+    """The elements are numbered by the dimensions and the result lies as x does: the values of the dense call, in x's order; the
+    gradient, for one in either order, too."""
+    B, C, N = size
+    dtype, g = TYPES[kind], gen(6)
+    rng = torch.tensor([2 ** 40 + 3, 2 ** 32 - 2], device="cuda")
+    x, d = features(g, B, C, N, dtype), features(g, B, C, N, dtype)
+    leaf = x.detach().requires_grad_(True)
+    dense = x.contiguous().requires_grad_(True)
+    for p in (0.3, 1.0):
+        y, want = ff.dropout(leaf, p, rng), ff.dropout(dense, p, rng)
+        assert torch.equal(y, want) and y.stride() == torch.empty_like(x).stride()
+        (dw,) = torch.autograd.grad(want, [dense], d.contiguous())
+        for given in (d, d.contiguous()):
+            (dx,) = torch.autograd.grad(y, [leaf], given, retain_graph=True)
+            assert torch.equal(dx, dw)
+    off = torch.zeros((x.numel() + 1,), dtype=dtype, device="cuda")[1:].view(B, N, C).transpose(1, 2).copy_(x)  # (off 16 bytes)
+    assert torch.equal(ff.dropout(off, 0.3, rng), ff.dropout(dense.detach(), 0.3, rng))
+    bad = torch.full_like(x, float('nan'))
+    assert torch.equal(ff.dropout(bad, 0.3, rng).isnan(), ref.keep(2 ** 40 + 3, 2 ** 32 - 2, 0.3, (B, C, N)).cuda())
+
+
+def test_dropout_in_a_chain_keeps_its_order():
+    """Point-major features through the operators of a block and dropout: no result of the chain changes its order."""
+    g = gen(7)
+    rng = torch.tensor([1, 0], device="cuda")
+    x, ws = ffn_inputs(g, 2, 40, 30, 64, torch.bfloat16)
+    y = ff.dropout(ff.gated_feed_forward(ff.point_norm(x), *ws), 0.2, rng)
+    out = ff.dropout(ff.norm_gate_residual(x, y), 0.2, rng)
+    for t in (y, out):
+        assert ff._point_major(t) and not t.is_contiguous()
