@@ -36,6 +36,7 @@ _NORMS = {'none': 0, 'rms': 1, 'layer': 2}
 _PRECISIONS = {'f32': 0, 'bf16': 1}
 _OP_GATED_FFN, _OP_POINT_NORM = 17, 18
 _MAX_NORM_CHANNELS = 4096
+_MAX_SIZE = 2 ** 31 - 1  # the C entries take 32-bit sizes
 
 
 def _p(t):
@@ -51,6 +52,11 @@ def _check_trace(who):
         raise RuntimeError(f"{who}: cannot be traced by torch.jit.trace (capture a HIP graph instead)")
 
 
+def _check_sizes(t, who, name):
+    if max(t.shape) > _MAX_SIZE:
+        raise ValueError(f"{who}: {name} has the shape {tuple(t.shape)}, no size is above {_MAX_SIZE}")
+
+
 def _check_features(x, who, name='x'):
     _check_trace(who)
     if not isinstance(x, torch.Tensor):
@@ -61,6 +67,7 @@ def _check_features(x, who, name='x'):
         raise TypeError(f"{who}: {name} is float32, bfloat16 or float16, got {x.dtype}")
     if x.dim() not in (2, 3):
         raise ValueError(f"{who}: {name} is (B, C, N) features or (R, C) rows, got {tuple(x.shape)}")
+    _check_sizes(x, who, name)
 
 
 def _sizes(x):
@@ -295,6 +302,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down=None, activation='silu', precisio
     _check_param(w_gate, (w_gate.shape[0] if isinstance(w_gate, torch.Tensor) and w_gate.dim() == 2 else 'H', C), x, who, 'w_gate',
                  optional=False, f32=False)
     H = w_gate.shape[0]
+    _check_sizes(w_gate, who, 'w_gate')
     _check_param(w_up, (H, C), x, who, 'w_up', optional=False, f32=False)
     _check_param(w_down, (C, H), x, who, 'w_down', f32=False)
     if C == 0 or H == 0:
@@ -480,6 +488,7 @@ class _Dropout(Function):
 def _drop(x, p, rng):
     lib, dtype = _lib.lib(), _DTYPES[x.dtype]
     if x.dim() == 3 and not x.is_contiguous() and _point_major(x):
+        _check_sizes(x, 'dropout', 'x')
         out = torch.empty_like(x)
         with _lib.on_device(x.device):
             _lib.check(lib.cl3d_dropout_point_major(_p(x), dtype, *x.shape, p, _p(rng), _p(out), _stream(x.device)))

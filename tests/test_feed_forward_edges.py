@@ -54,3 +54,29 @@ def test_the_point_major_dropout_returns_codes_and_says_why():
         assert lib.cl3d_dropout_point_major(*args) == -1 and text in lib.cl3d_last_error_string().decode(), (args, lib.cl3d_last_error_string())
     for sizes in ((0, 8, 3), (2, 0, 3), (2, 8, 0)):
         assert lib.cl3d_dropout_point_major(None, 0, *sizes, 0.5, a, None, None) == 0
+
+
+@pytest.mark.parametrize("shape", [(2 ** 31, 1), (2 ** 32 + 5, 1), (2 ** 32 + 5, 1, 1), (1, 1, 2 ** 32 + 5), (1, 2 ** 32 + 1, 2)], ids=str)
+def test_sizes_past_31_bits_are_refused(shape):
+    """The C entries take 32-bit sizes; a longer axis would arrive with its high half cut off."""
+    x = fake(1).expand(shape)
+    C = shape[1]
+    calls = [lambda: ff.point_norm(x), lambda: ff.norm_gate_residual(x, x)]
+    if C == 1:
+        calls.append(lambda: ff.gated_feed_forward(x, fake(8, 1), fake(8, 1), fake(1, 8)))
+        many = fake(1).expand(2 ** 32 + 3, 1)
+        calls.append(lambda: ff.gated_feed_forward(fake(4, 1), many, many))
+    if len(shape) == 3:
+        calls += [lambda: ff.to_point_major(x), lambda: ff.to_channel_major(x)]
+    for call in calls:
+        with pytest.raises(ValueError, match="2147483647"):
+            call()
+
+
+def test_dropout_of_point_major_features_past_31_bits_is_refused():
+    x = fake(1).expand(2, 2 ** 32 + 4, 2)
+    rng = torch.zeros(2, dtype=torch.int64)
+    with pytest.MonkeyPatch.context() as patch:
+        patch.setattr(ff, "_point_major", lambda t: True)  # (no memory for features that are)
+        with pytest.raises(ValueError, match="2147483647"):
+            ff.dropout(x, 0.5, rng)
