@@ -788,7 +788,9 @@ __global__ __launch_bounds__(1024) void norm_sums_kernel(NormSums a) {
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------
-constexpr int kNormMaxC = 4096;
+// up to kNormMaxC channels any number, up to kNormWideC multiples of 8 (the last stage of a backbone of width 288: 4608) in memory
+// that starts on 16 bytes
+constexpr int kNormMaxC = 4096, kNormWideC = 6144;
 
 // workgroups of a cloud and rows of each
 static void norm_grid(NormArgs &a, int rows_per_pass, int target) {
@@ -815,6 +817,7 @@ static NormMap norm_map(int dtype, int C, bool aligned) {
   if (v > 1 && pieces <= 32) return {32, 1, v};
   if (pieces <= 64) return {64, 1, v};
   if (need <= 2) return {256, need, v};
+  if (C > kNormMaxC) return {256, kNormWideC / 256 / v, v};
   if (v > 1 || need <= 4) return {256, 4, v};
   return {256, need <= 10 ? 10 : 16, v};
 }
@@ -848,7 +851,8 @@ template <typename T> static void norm_pick(const NormMap &m, bool backward, con
   if (m.tpr == 64) return norm_run<T, 64, 1, V>(backward, a, st);
   if (m.nv == 1) return norm_run<T, 256, 1, V>(backward, a, st);
   if (m.nv == 2) return norm_run<T, 256, 2, V>(backward, a, st);
-  if constexpr (V == 4) norm_run<T, 256, 4, V>(backward, a, st);  // (16-bit: two pieces hold kNormMaxC)
+  if constexpr (V == 4) if (m.nv == 4) return norm_run<T, 256, 4, V>(backward, a, st);  // (16-bit: two pieces hold kNormMaxC)
+  norm_run<T, 256, kNormWideC / 256 / V, V>(backward, a, st);
 }
 static void norm_launch(int dtype, const NormMap &m, bool backward, const NormArgs &a, hipStream_t st) {
   if (dtype == CL3D_F32) norm_pick<F32>(m, backward, a, st);
@@ -897,6 +901,10 @@ static void norm_cm_launch(int dtype, bool backward, const NormArgs &a, hipStrea
   else norm_cm_pick<F16>(backward, a, st);
 }
 
+static bool params_aligned(const cl3d_norm_residual *p) {
+  return aligned16(p->weight) && aligned16(p->bias) && aligned16(p->gate) && aligned16(p->next_weight) && aligned16(p->next_bias);
+}
+
 static int norm_checks(const cl3d_norm_residual *p, bool backward, const char *who) {
   CL3D_REQUIRE(p != nullptr, "%s: null argument block", who);
   CL3D_REQUIRE(p->dtype == CL3D_F32 || p->dtype == CL3D_BF16 || p->dtype == CL3D_F16, "%s: unknown element type %d", who, p->dtype);
@@ -906,8 +914,11 @@ static int norm_checks(const cl3d_norm_residual *p, bool backward, const char *w
                "%s: unknown norm", who);
   CL3D_REQUIRE(p->y != nullptr || p->next_kind != CL3D_NORM_NONE, "%s: neither a block to leave nor a norm to enter", who);
   CL3D_REQUIRE(p->y != nullptr || (!p->weight && !p->bias && !p->gate && p->p == 0.0), "%s: a gate, dropout or norm of a block that is not there", who);
-  if (p->C > kNormMaxC || (long long)p->B * p->N > 0x7fffff00ll)
-    return fail(CL3D_E_UNSUPPORTED, "%s: more than %d channels, or points than 31 bits count", who, kNormMaxC);
+  if (p->C > kNormWideC || (p->C > kNormMaxC && p->C % 8 != 0) || (long long)p->B * p->N > 0x7fffff00ll)
+    return fail(CL3D_E_UNSUPPORTED, "%s: more than %d channels (multiples of 8: %d), or points than 31 bits count", who, kNormMaxC, kNormWideC);
+  if (p->C > kNormMaxC && !(params_aligned(p) && aligned16(p->x) && aligned16(p->y) && aligned16(p->out) && aligned16(p->next) && aligned16(p->dout) &&
+                            aligned16(p->dnext) && aligned16(p->dx) && aligned16(p->dy)))
+    return fail(CL3D_E_UNSUPPORTED, "%s: tensors of more than %d channels start on 16 bytes", who, kNormMaxC);
   if (p->gate_cloud && p->B > 65535) return fail(CL3D_E_UNSUPPORTED, "%s: a gate per cloud for more than 65535 clouds", who);
   return CL3D_OK;
 }
@@ -930,10 +941,6 @@ static void norm_args(NormArgs &a, const cl3d_norm_residual *p) {
 // workgroups: as many as are resident with the registers of the 16-bit variants (four a CU forward, three backward); more would
 // load their parameters again, one round too few leaves CUs idle (backward 81 920 x 288: 512 156 us, 768 125, 1024 167)
 constexpr int kNormFwdGroups = 1024, kNormBwdGroups = 768;
-
-static bool params_aligned(const cl3d_norm_residual *p) {
-  return aligned16(p->weight) && aligned16(p->bias) && aligned16(p->gate) && aligned16(p->next_weight) && aligned16(p->next_bias);
-}
 
 // point-major copies of channel-major tensors, and back
 struct NormCopies {

@@ -35,7 +35,7 @@ _ACTIVATIONS = {'silu': 0, 'gelu': 1, 'relu': 2}
 _NORMS = {'none': 0, 'rms': 1, 'layer': 2}
 _PRECISIONS = {'f32': 0, 'bf16': 1}
 _OP_GATED_FFN, _OP_POINT_NORM = 17, 18
-_MAX_NORM_CHANNELS = 4096
+_MAX_NORM_CHANNELS, _WIDE_NORM_CHANNELS = 4096, 6144  # any number up to the first, multiples of 8 up to the second
 _MAX_SIZE = 2 ** 31 - 1  # the C entries take 32-bit sizes
 
 
@@ -331,6 +331,7 @@ def _norm_forward(x, y, weight, bias, gate, next_weight, next_bias, rng, opts, n
     for t in params:  # (one type for all of them: a mixture goes to f32)
         if t is not None:
             t = (t if not f32 or t.dtype == torch.float32 else t.float()).contiguous()
+            t = _aligned(t) if C > _MAX_NORM_CHANNELS else t
         held.append(t)
     out = torch.empty_like(x) if y is not None else None
     nxt = torch.empty_like(x) if next_kind else None
@@ -392,20 +393,24 @@ class _NormResidual(Function):
         return (dx, dy, *grads, None, None)
 
 
+def _check_channels(C, who):
+    if not 0 < C <= _MAX_NORM_CHANNELS and not (0 < C <= _WIDE_NORM_CHANNELS and C % 8 == 0):
+        raise ValueError(f"{who}: 1 to {_MAX_NORM_CHANNELS} channels, or a multiple of 8 up to {_WIDE_NORM_CHANNELS}, got {C}")
+
+
 def _check_norm(x, kind, eps, who, none=False):
     if kind not in _NORMS or (kind == 'none' and not none):
         raise ValueError(f"{who}: a norm is one of {[k for k in _NORMS if none or k != 'none']}, got {kind!r}")
     if not eps >= 0:
         raise ValueError(f"{who}: eps is not negative, got {eps}")
-    if not 0 < x.shape[1] <= _MAX_NORM_CHANNELS:
-        raise ValueError(f"{who}: 1 to {_MAX_NORM_CHANNELS} channels, got {x.shape[1]}")
+    _check_channels(x.shape[1], who)
 
 
 def point_norm(x, weight=None, bias=None, kind='rms', eps=1e-6):
     """norm(x) weight + bias over the channels of every point: the entry of a block.
 
     kind 'rms': x / sqrt(mean x^2 + eps); 'layer': (x - mean) / sqrt(var + eps), the variance over all C.  weight, bias (C,), of x's
-    type or float32; None: 1 and 0."""
+    type or float32; None: 1 and 0.  Up to 4096 channels, or a multiple of 8 up to 6144."""
     who = 'point_norm'
     _check_features(x, who)
     _check_norm(x, kind, eps, who)
@@ -424,7 +429,8 @@ def norm_gate_residual(x, y, weight=None, bias=None, gate=None, residual_scale=1
 
     x: the residual stream, y: the block's result, same shape and type.  kind 'rms', 'layer' or 'none' (y is added as it is).  gate
     (C,), or (B, C) for a gate of each cloud (for rows: of each row), or None.  p, rng: as in dropout(); element (b, c, n) is number
-    (b N + n) C + c of the draw.  next is formed from out before out is rounded.  Returns out, or (out, next) with next_kind."""
+    (b N + n) C + c of the draw.  next is formed from out before out is rounded.  Channels as in
+    point_norm().  Returns out, or (out, next) with next_kind."""
     who = 'norm_gate_residual'
     _check_features(x, who)
     _check_features(y, who, 'y')
@@ -615,6 +621,7 @@ class FeedForwardBlock(nn.Module):
         super().__init__()
         if pre_norm not in ('rms', 'layer') or post_norm not in _NORMS:
             raise ValueError(f"FeedForwardBlock: norms are 'rms' or 'layer' (post_norm: or 'none'), got {pre_norm!r}, {post_norm!r}")
+        _check_channels(channels, 'FeedForwardBlock')
         self.pre_norm, self.post_norm, self.eps, self.residual_scale = pre_norm, post_norm, eps, residual_scale
         self.p = _check_p(dropout, 'FeedForwardBlock')
         self._draws = _Draws(seed)

@@ -579,6 +579,7 @@ int cl3d_transpose16(const void *src, int B, int R, int C, void *dst, cl3d_strea
  * multiple of 4: by way of transposed copies in ws):
  *     n = norm(y) weight + bias;  out = residual_scale x + gate * drop(n);  next = next_norm(out) next_weight + next_bias
  * y NULL: there is no block to leave, next = next_norm(x) next_weight + next_bias.  next_kind CL3D_NORM_NONE: no entry.
+ * Up to 4096 channels, or multiples of 8 up to 6144 in tensors that start on 16 bytes.
  * rms: v / sqrt(mean v^2 + eps); layer: (v - mean) / sqrt(var + eps), over the channels of a point.  weight, bias, gate,
  * next_weight, next_bias: [C] (gate [B,C] with gate_cloud), NULL: 1, 0, 1, 1, 0; of the tensors' type, or f32 with param_f32.
  * p, rng: as in cl3d_dropout, element (b, n, c) being number (b N + n) C + c.  stats [B,N,4], 16-byte aligned: what the

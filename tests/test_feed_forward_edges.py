@@ -80,3 +80,26 @@ def test_dropout_of_point_major_features_past_31_bits_is_refused():
         patch.setattr(ff, "_point_major", lambda t: True)  # (no memory for features that are)
         with pytest.raises(ValueError, match="2147483647"):
             ff.dropout(x, 0.5, rng)
+
+
+@pytest.mark.parametrize("channels", [0, 4098, 4100, 4612, 6150, 6152])
+def test_a_block_of_too_many_channels_is_refused_where_it_is_made(channels):
+    with pytest.raises(ValueError, match="channels, or a multiple of 8"):
+        ff.FeedForwardBlock(channels, 16)
+    if channels:
+        with pytest.raises(ValueError, match="channels, or a multiple of 8"):
+            ff.point_norm(fake(2, channels))
+
+
+def test_wide_norms_start_on_16_bytes():
+    lib = _lib.lib()
+    a = 1 << 20
+    names = ("x", "y", "weight", "bias", "gate", "next_weight", "next_bias", "out", "next")
+    for name in names:
+        given = {n: a for n in names}
+        given[name] = a + 4
+        rc = lib.cl3d_norm_residual_fwd(ctypes.byref(_block(C=4608, **given)), None)
+        assert rc == -4 and "16 bytes" in lib.cl3d_last_error_string().decode(), name
+    for C in (4100, 6152):
+        rc = lib.cl3d_norm_residual_fwd(ctypes.byref(_block(C=C, **{n: a for n in names})), None)
+        assert rc == -4 and "channels" in lib.cl3d_last_error_string().decode()

@@ -182,3 +182,35 @@ def test_dropout_in_a_chain_keeps_its_order():
     out = ff.dropout(ff.norm_gate_residual(x, y), 0.2, rng)
     for t in (y, out):
         assert ff._point_major(t) and not t.is_contiguous()
+
+
+# ----------------------------------------------------------------------------------------------------------- the widest stages
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("size", [(1, 4608, 5), (2, 4104, 3), (1, 5120, 2), (3, 6144, 1), (1, 4608, 1030)], ids=lambda s: "x".join(map(str, s)))
+def test_norms_of_the_widest_stages(size, kind):
+    """A backbone of width 288 ends in 4608 channels: above 4096, multiples of 8 up to 6144."""
+    norm_check(size, kind, "layer", "rms", "cloud", 0.25, "point", kind)
+    if size[2] < 100:
+        norm_check(size, kind, "none", "layer", "channel", 0.0, "channel", "f32", bias=False)
+        norm_check(size, kind, "rms", None, "none", 0.5, "point", kind, bias=False)
+
+
+def test_parameters_of_a_wide_norm_need_not_be_aligned():
+    g = gen(8)
+    x = vector(g, 6, 4608, dtype=torch.bfloat16)
+    w = vector(g, 4609, dtype=torch.bfloat16)
+    assert torch.equal(ff.point_norm(x, w[1:]), ff.point_norm(x, w[1:].clone()))
+
+
+def test_feed_forward_block_of_the_widest_stage():
+    g = gen(9)
+    block = ff.FeedForwardBlock(4608, 64, post_norm='layer', dropout=0.1, seed=3).cuda()
+    x = features(g, 1, 4608, 9, torch.float32, "channel").requires_grad_(True)
+    y = block(x)
+    grads = torch.autograd.grad(y, [x] + list(block.parameters()), torch.ones_like(y))
+    with torch.no_grad():
+        h = ff.point_norm(x, block.pre_weight, None, 'rms', block.eps)
+        want = ff.norm_gate_residual(x, block.feed_forward(h), block.post_weight, block.post_bias, block.gate, 1.0, 'layer', block.eps, 0.1,
+                                     torch.tensor([3, 0], device="cuda"))
+    # (the same kernels on the other memory order: the same bits)
+    assert torch.equal(y, want) and all(bool(t.isfinite().all()) and t.shape == s.shape for t, s in zip(grads, [x] + list(block.parameters())))
