@@ -789,7 +789,8 @@ __global__ __launch_bounds__(1024) void norm_sums_kernel(NormSums a) {
 
 // ---- host side -----------------------------------------------------------------------------------------------------
 // up to kNormMaxC channels any number, up to kNormWideC multiples of 8 (the last stage of a backbone of width 288: 4608) in memory
-// that starts on 16 bytes
+// that starts on 16 bytes.  4096 x 4608 bf16, exit and next norm: 71 us forward, 180 backward (the wider variants hold a wave a SIMD;
+// 4096 x 4096: 36 and 139)
 constexpr int kNormMaxC = 4096, kNormWideC = 6144;
 
 // workgroups of a cloud and rows of each

@@ -116,9 +116,10 @@ static void tile_shape(int R, int C, int *tr, int *tc) {
   int TR = tile_extent(R), TC = tile_extent(C);
   const auto fits = [](int a, int b) { return a * (b + 1) <= kTrFloats; };
   if (!fits(TR, TC) && C > kTrMax) TC = 32;
-  if (!fits(TR, TC) && R > kTrMax) TR = 32;
+  // (as many rows a tile as the 65535 tiles of a grid's second axis leave, 64 at most: the other axis gives way below)
+  if (!fits(TR, TC) && R > kTrMax && ceil_div(R, 32) <= 65535) TR = 32;
   while (!fits(TR, TC)) {  // both axes short and the plane still too large: halve the longer extent
-    if (TR >= TC) TR = ((TR / 2) + 3) & ~3; else TC = ((TC / 2) + 3) & ~3;
+    if (TR >= TC && ceil_div(R, 32) <= 65535) TR = ((TR / 2) + 3) & ~3; else TC = ((TC / 2) + 3) & ~3;
   }
   *tr = TR;
   *tc = TC;

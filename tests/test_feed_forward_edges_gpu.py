@@ -214,3 +214,16 @@ def test_feed_forward_block_of_the_widest_stage():
                                      torch.tensor([3, 0], device="cuda"))
     # (the same kernels on the other memory order: the same bits)
     assert torch.equal(y, want) and all(bool(t.isfinite().all()) and t.shape == s.shape for t, s in zip(grads, [x] + list(block.parameters())))
+
+
+# ------------------------------------------------------------------------------------------------------------- clouds of millions
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_memory_orders_of_a_cloud_of_millions(kind):
+    """2 200 000 points x 72 channels: there, back, and a feed-forward in either order."""
+    B, C, N = 1, 72, 2200000
+    x = vector(gen(10), B, C, N, dtype=TYPES[kind])
+    y = ff.to_point_major(x)
+    assert ff._point_major(y) and torch.equal(y, x)
+    assert torch.equal(ff.to_channel_major(y), x)
+    ws = [vector(gen(11), 8, C, dtype=TYPES[kind], std=0.1), vector(gen(12), 8, C, dtype=TYPES[kind], std=0.1), vector(gen(13), C, 8, dtype=TYPES[kind])]
+    assert torch.equal(ff.gated_feed_forward(x, *ws), ff.gated_feed_forward(y, *ws))
