@@ -20,6 +20,7 @@ CPU fallback.  The operators can be captured into HIP graphs, forward and backwa
 gradient and a torch.jit.trace are refused.
 """
 import ctypes
+import threading
 import weakref
 
 import torch
@@ -204,6 +205,7 @@ def _recorded(*tensors):
 # joins: ending it takes the process down.  Every eager graph of these operators is therefore known by its context while it lives
 # (autograd frees the context with the graph), and a captured backward pass of the same leaves says so instead.
 _LIVE = weakref.WeakSet()
+_LIVE_LOCK = threading.RLock()  # (a set that another thread adds to cannot be walked; contexts may go meanwhile)
 
 
 def _track(ctx, *inputs):
@@ -211,7 +213,8 @@ def _track(ctx, *inputs):
     ctx.leaves = [weakref.ref(t) for t in inputs if t is not None and t.requires_grad and t.is_leaf]
     if ctx.leaves and not torch.cuda.is_current_stream_capturing():
         ctx.made_on = _raw_stream(inputs[0].device.index)
-        _LIVE.add(ctx)
+        with _LIVE_LOCK:
+            _LIVE.add(ctx)
 
 
 def _check_capture(ctx, device):
@@ -220,7 +223,9 @@ def _check_capture(ctx, device):
         return
     mine = {id(t) for t in (r() for r in ctx.leaves) if t is not None}
     stream = _raw_stream(device.index)
-    for other in list(_LIVE):
+    with _LIVE_LOCK:
+        others = list(_LIVE)
+    for other in others:
         if other is not ctx and other.made_on != stream and any(id(r()) in mine for r in other.leaves if r() is not None):
             raise RuntimeError("a backward pass is being captured while an eager graph of the same leaves, made on another stream, is "
                                "alive: delete its outputs first, or warm up and capture on one stream (closerlook3d_amd.step_stream())")

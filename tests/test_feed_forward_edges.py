@@ -103,3 +103,51 @@ def test_wide_norms_start_on_16_bytes():
     for C in (4100, 6152):
         rc = lib.cl3d_norm_residual_fwd(ctypes.byref(_block(C=C, **{n: a for n in names})), None)
         assert rc == -4 and "channels" in lib.cl3d_last_error_string().decode()
+
+
+def test_capture_checks_beside_threads_that_make_graphs(monkeypatch):
+    """A captured backward pass looks through the living eager graphs while other threads make and drop theirs."""
+    import sys
+    import threading
+    monkeypatch.setattr(ff, "_raw_stream", lambda index: 1)
+    leaf = torch.nn.Parameter(torch.zeros(3))
+
+    class Context:
+        pass
+
+    capturing = threading.local()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: getattr(capturing, "yes", False))
+    stop, failed = threading.Event(), []
+    alive = [Context() for _ in range(400)]
+    for ctx in alive:
+        ff._track(ctx, leaf)
+
+    def make():
+        kept = []
+        try:
+            while not stop.is_set():
+                kept.append(Context())
+                ff._track(kept[-1], leaf)
+                if len(kept) > 50:
+                    kept.clear()
+        except Exception as e:  # noqa: BLE001 (what a thread raises is looked at below)
+            failed.append(e)
+
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    threads = [threading.Thread(target=make) for _ in range(3)]
+    try:
+        for t in threads:
+            t.start()
+        mine = Context()
+        mine.leaves, mine.made_on = [], 1
+        capturing.yes = True
+        for _ in range(300):
+            ff._check_capture(mine, torch.device("cuda", 0))
+    finally:
+        stop.set()
+        for t in threads:
+            t.join()
+        sys.setswitchinterval(interval)
+    assert not failed
+    del alive, ctx
