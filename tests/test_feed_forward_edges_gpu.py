@@ -227,3 +227,36 @@ def test_memory_orders_of_a_cloud_of_millions(kind):
     assert torch.equal(ff.to_channel_major(y), x)
     ws = [vector(gen(11), 8, C, dtype=TYPES[kind], std=0.1), vector(gen(12), 8, C, dtype=TYPES[kind], std=0.1), vector(gen(13), C, 8, dtype=TYPES[kind])]
     assert torch.equal(ff.gated_feed_forward(x, *ws), ff.gated_feed_forward(y, *ws))
+
+
+# ------------------------------------------------------------------------------------------------------------------ long sums
+# up to 64 points, one, two and more turns of the direct kernel's loop over k (1024 elements of 16 bits, half as many of 32, half of
+# either above 32 points), whole vectors and ragged; above, sums and tiles past every listed training width
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("size", [(1, 1160, 1, 2320), (16, 2304, 1, 4608), (1, 513, 17, 1025), (33, 1031, 1, 2057), (64, 545, 1, 1100), (4, 2056, 16, 1032),
+                                  (2, 520, 31, 264)], ids=lambda s: "x".join(map(str, s)))
+def test_few_points_of_many_channels(size, kind):
+    B, C, N, H = size
+    dtype, g = TYPES[kind], gen(14)
+    order = "channel" if N > 1 and C % 2 else "point"
+    x, ws = ffn_inputs(g, B, C, N, H, dtype, order)
+    ffn_check(x, ws, ["silu", "gelu", "relu"][(C + N) % 3], dtype, features(g, B, C, N, dtype, order), order, tag=(size, kind))
+
+
+@pytest.mark.parametrize("kind, precision, size", [("bf16", "f32", (130, 2304, 1, 4608)), ("f16", "f32", (1, 1153, 200, 2305)), ("f32", "f32", (2, 1153, 100, 2305)),
+                                                   ("f32", "bf16", (1, 2304, 256, 1160)), ("bf16", "f32", (2, 577, 513, 1152)),
+                                                   ("f32", "f32", (1, 576, 1030, 1152))], ids=str)
+def test_wide_products_and_their_gradients(kind, precision, size):
+    B, C, N, H = size
+    dtype, g = TYPES[kind], gen(15)
+    order = "channel" if N > 1 and C % 2 else "point"
+    x, ws = ffn_inputs(g, B, C, N, H, dtype, order)
+    ffn_check(x, ws, "gelu" if C % 2 else "silu", dtype, features(g, B, C, N, dtype, order), order, precision, tag=(size, kind))
+
+
+def test_wide_projections_alone():
+    for kind, size in (("bf16", (16, 2304, 1, 4608)), ("f32", (33, 1031, 1, 2057)), ("f16", (130, 1153, 1, 2305))):
+        B, C, N, H = size
+        g = gen(16)
+        x, ws = ffn_inputs(g, B, C, N, H, TYPES[kind], down=False)
+        ffn_check(x, ws, "gelu", TYPES[kind], features(g, B, H, N, TYPES[kind]), "point", tag=(kind, size))
