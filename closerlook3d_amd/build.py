@@ -29,14 +29,12 @@ FLAGS = [
     "-ffp-contract=off",
     # native global_atomic_add_f32 for the large-N scatter fallback
     "-munsafe-fp-atomics",
-    # no compiler-made packed FP32: the SLP vectoriser pairs scalar FMAs into v_pk_* instructions and, for an operand in
-    # the high half of a register pair, sets op_sel on it -- the form that read zeros beside bf16 MFMA kernels (round 6,
-    # DESIGN 6; csrc/fused_pwmlp.hip pk_low).  The packed code that is left is written out by hand and checked by
-    # tests/test_isa_packed_operands.py
-    "-fno-slp-vectorize",
-    # ... and none from hand-written float pairs either: without the feature the compiler emits the two scalar instructions
-    # for each pair (the same bits; PseudoGrid, the last user of packed pairs, measured 0.8-1 % slower).  hipcc's host pass
+    # no packed FP32 at all: the SLP vectoriser pairs scalar FMAs into v_pk_* instructions and, for an operand in the high half
+    # of a register pair, sets op_sel on it -- the form that read zeros beside bf16 MFMA kernels.  Without the feature the
+    # compiler emits two scalar instructions for a hand-written float pair too (the same bits; PseudoGrid, the last user of
+    # packed pairs, measured 0.8-1 % slower).  tests/test_isa_no_packed_fp32.py checks the built library.  hipcc's host pass
     # warns that it does not know the feature: harmless
+    "-fno-slp-vectorize",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wextra", "-Wno-unused-parameter",
 ]

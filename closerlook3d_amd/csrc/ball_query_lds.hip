@@ -17,9 +17,8 @@
 //           cell, as records + a list of tasks (<= kTlQT queries of one cell) in LDS;
 //   query   waves draw tasks from an LDS ticket (dynamic balance at LDS-atomic cost).  A task's candidate window -- the
 //           <= 9 runs of `sorted` around its cell -- is read out of LDS ONCE into registers (<= 384 records, 24 VGPRs)
-//           and serves all the task's queries, two at a time: the two distances of a candidate are one chain of packed
-//           FP32 instructions (v_pk_add / v_pk_mul / v_pk_fma: per-lane IEEE, the same bits as the scalar chain of
-//           cl3d::dist2), and every in-radius candidate leaves (d2, original index) in the query's LDS list.  The
+//           and serves all the task's queries, two at a time: the two distances of a candidate are two chains of
+//           cl3d::dist2 side by side, and every in-radius candidate leaves (d2, original index) in the query's LDS list.  The
 //           reference's order-dependent rule is then restated order-independently exactly as ball_query_cells.hip
 //           does (see its header): <= 3K in-radius candidates -> all of them; more -> the 3K smallest original indices
 //           with the strict minimum patched into the last slot; result ranked by (distance, original index).
@@ -28,7 +27,7 @@
 //           collects those 3K candidates and the strict minimum.  Slow (a dozen window passes) and rare; no flag
 //           array, no second launch.
 //
-// Round 4 (this form): window in registers across the queries of a cell, packed distance arithmetic, distances stored
+// Round 4 (this form): window in registers across the queries of a cell, distances stored
 // by the candidate pass instead of being recomputed at selection -- 375 -> ~215 vector instructions per query.
 #include "ball_query.h"
 
@@ -55,7 +54,7 @@ constexpr int kTlQChunk = 512;                    // query records staged per ro
 #define CL3D_TL_MINWAVES 4  // waves per SIMD the register budget is set for (5 -> 96 VGPRs: room for a second kernel's waves)
 #endif
 constexpr int kTlQT = CL3D_TL_QT;                 // queries per task (of one cell): they share one window read
-constexpr int kTlQW = 2;                          // queries tested per candidate pass (one packed-FP32 chain)
+constexpr int kTlQW = 2;                          // queries tested per candidate pass (two chains)
 constexpr int kTlCapMul = 6;                      // candidate list holds kTlCapMul*K entries per query
 #ifndef CL3D_TL_FLAT
 #define CL3D_TL_FLAT 6
@@ -64,20 +63,10 @@ constexpr int kTlFlat = CL3D_TL_FLAT;             // window batches (of 64) whos
 constexpr int kTlIdxRounds = 4;                   // rank-by-index rounds held in registers: kTlCapMul*K <= 256
 constexpr int kTlRankRounds = 2;                  // rank-by-distance rounds held in registers: 3*K <= 128
 
-// both queries of a pass: CL3D_TL_PK = 1 a packed pair (v_pk_*_f32, rounds 4-6; scripts/micro/kernel_variants.py "bq_packed"),
-// 0 (shipped since round 6, session 66) two scalar chains -- the packed chain never had fewer cycles (a packed FP32
-// instruction takes two slots on gfx950; round 4 said so of its own gain), the scalar one measures the same or 1 % faster
-// (67.0-67.3 against 67.5-68.2 us alone, the replayed step 0.2807 against 0.2817 ms, alternating), returns the same bits (it
-// IS cl3d::dist2), and leaves no packed operand in the kernel for the fault of DESIGN 6 to find -- the candidate's y comes
-// out of ds_read_b128 in the high half of a register pair, exactly the operand that read zeros in the gather pass.
-#ifndef CL3D_TL_PK
-#define CL3D_TL_PK 0
-#endif
-#if CL3D_TL_PK
-typedef float tl_v2f __attribute__((ext_vector_type(2)));
-#else
-struct tl_v2f { float x, y; };
-#endif
+// both queries of a pass, as two scalar chains: one packed chain (v_pk_*_f32, two slots an instruction on gfx950) never had fewer
+// cycles (67.5-68.2 us alone against 67.0-67.3, the replayed step 0.2817 against 0.2807 ms, alternating) and has operands that
+// read the high half of a register pair, which came back as 0.0 beside bf16 MFMA kernels
+struct tl_pair { float x, y; };
 
 __host__ __device__ inline int tl_pad4(int x) { return (x + 3) & ~3; }
 
@@ -116,31 +105,9 @@ __device__ __forceinline__ float tl_uniform(float v) {
   return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
 }
 
-// cl3d::dist2 for two queries against one candidate, as packed FP32 (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32 are
-// IEEE per element: each half is bit for bit the scalar chain of dist2; the library is built with -ffp-contract=off,
-// so nothing is fused or split behind this).  Same CL3D_D2_FORM switch as cl3d_common.h.
-__device__ __forceinline__ tl_v2f tl_dist2_pair(tl_v2f qx, tl_v2f qy, tl_v2f qz, float x, float y, float z) {
-#if !CL3D_TL_PK
-  tl_v2f r;  // (the scalar chain itself: cl3d::dist2)
-  r.x = dist2(qx.x, qy.x, qz.x, x, y, z);
-  r.y = dist2(qx.y, qy.y, qz.y, x, y, z);
-  return r;
-#else
-  const tl_v2f dx = qx - x, dy = qy - y, dz = qz - z;
-#if CL3D_D2_FORM == 0
-  const tl_v2f xx = dx * dx;
-  const tl_v2f zz = dz * dz;
-  return __builtin_elementwise_fma(dy, dy, xx) + zz;
-#elif CL3D_D2_FORM == 1
-  const tl_v2f xx = dx * dx;
-  const tl_v2f yy = dy * dy;
-  const tl_v2f zz = dz * dz;
-  return (xx + yy) + zz;
-#else
-  const tl_v2f xx = dx * dx;
-  return __builtin_elementwise_fma(dz, dz, __builtin_elementwise_fma(dy, dy, xx));
-#endif
-#endif
+// cl3d::dist2 for two queries against one candidate
+__device__ __forceinline__ tl_pair tl_dist2_pair(tl_pair qx, tl_pair qy, tl_pair qz, float x, float y, float z) {
+  return {dist2(qx.x, qy.x, qz.x, x, y, z), dist2(qx.y, qy.y, qz.y, x, y, z)};
 }
 
 template <bool SAME>  // SAME: the queries ARE the support points (every non-strided layer): one set of registers for both roles
@@ -553,13 +520,13 @@ __global__ __launch_bounds__(kTlThreads, CL3D_TL_MINWAVES) void bq_tile_kernel(c
           qzs[u] = tl_uniform(qq.z);
           cnt[u] = 0;
         }
-        const tl_v2f qx2 = {qxs[0], qxs[1]}, qy2 = {qys[0], qys[1]}, qz2 = {qzs[0], qzs[1]};
+        const tl_pair qx2 = {qxs[0], qxs[1]}, qy2 = {qys[0], qys[1]}, qz2 = {qzs[0], qzs[1]};
         // ---- candidates: every in-radius candidate of the window leaves (distance, original index) in the query's LDS
         // list (unordered: the selection below restates the reference's order-dependent rule), one ballot + prefix
         // count per query and 64 candidates
         auto test = [&](float4 rec, bool live) {
           // (a lane past the end gets a NaN coordinate: its distances are NaN and never "in radius")
-          const tl_v2f d2 = tl_dist2_pair(qx2, qy2, qz2, live ? rec.x : __builtin_nanf(""), rec.y, rec.z);
+          const tl_pair d2 = tl_dist2_pair(qx2, qy2, qz2, live ? rec.x : __builtin_nanf(""), rec.y, rec.z);
 #pragma unroll
           for (int u = 0; u < kTlQW; ++u) {
             const float d = u == 0 ? d2.x : d2.y;

@@ -37,16 +37,11 @@
 #include <stdlib.h>
 #include <type_traits>
 
-// The TRAIN walk's arithmetic: 0 (shipped since round 6, session 65) = scalar FMAs, two channels' chains interleaved by the
-// compiler; 1 = packed pairs (v_pk_fma_f32, rounds 4-6: scripts/micro/kernel_variants.py "train_packed").  A packed FP32
-// instruction occupies the vector pipe for two slots on gfx950, so the packed walk never had fewer cycles, only fewer
-// instructions -- and its four-deep dependent chains stalled the issue (round 5's ISA account: 34 % of the pass).  Scalar,
-// same box, alternating runs: TRAIN 66.2-66.5 -> 62.6-63.4 us, the replayed step 0.2842-0.2856 -> 0.2809-0.2824 ms, 110
-// VGPRs against 115, the same bits (each packed half WAS the scalar operation); and no packed operand is left in the
-// pass for the fault of DESIGN 6 to find (profiles/r06/session65_summary.txt).
-#ifndef CL3D_TRAIN_PK
-#define CL3D_TRAIN_PK 0
-#endif
+// The TRAIN walk is scalar FMAs, two channels' chains interleaved by the compiler.  As packed pairs (v_pk_fma_f32) it had fewer
+// instructions but no fewer cycles -- a packed FP32 instruction occupies the vector pipe for two slots on gfx950 -- and its
+// four-deep dependent chains stalled the issue: TRAIN 66.2-66.5 us packed, 62.6-63.4 scalar, the replayed step 0.2842-0.2856 and
+// 0.2809-0.2824 ms, 115 VGPRs and 110, the same bits.  And a packed operand that reads the high half of a register pair came back as
+// 0.0 beside bf16 MFMA kernels: the library is built without packed FP32 (tests/test_isa_packed_operands.py).
 
 namespace cl3d {
 
@@ -86,24 +81,6 @@ __device__ __forceinline__ float pw_preact(const float w[3], float rx, float ry,
 }
 
 // (div_k / div_magic: cl3d_common.h)
-typedef float pw_f2 __attribute__((ext_vector_type(2)));
-
-// A scalar that every lane pair of a packed instruction reads, in a register pair of its own with the value in the pair's
-// LOW dword (the other dword is never read: both result lanes take the low one, `op_sel_hi` = 0 on that operand).  Left
-// to itself the compiler feeds v_pk_fma_f32 the slot record's registers as ds_read_b128 delivered them, and for rel.z --
-// the record's last dword, the HIGH half of an aligned pair -- sets `op_sel` on the operand (the low result lane reads
-// the pair's high dword).  That form returned 0.0 to the low lane, in the wave's last sixteen lanes, a few hundred
-// times per launch whenever a dense bf16 MFMA contraction -- the engine's or the vendor library's, in this process or
-// in another one -- ran on the same CUs: sum y / y* / the batch statistics wrong by W_r[c][z] * rel.z of one slot in the
-// even channels (round 6, sessions 37-62; DESIGN 6 "What may run beside a bf16 contraction").  Without `op_sel`: 0 wrong
-// elements in 240 launches against 60-100 % of the launches with it.  tests/test_isa_packed_operands.py holds the
-// library to it.
-__device__ __forceinline__ pw_f2 pk_low(float x) {
-  pw_f2 p = __builtin_shufflevector((pw_f2)(x), (pw_f2)(x), 0, -1);  // (element 1 left undefined: one move, not two)
-  asm("" : "+v"(p));
-  return __builtin_shufflevector(p, p, 0, 0);
-}
-
 // query-major gather passes.  Persistent blocks: tile = 4*QW*QPG queries of one cloud (every lane group walks QPG
 // queries of a tile one after the other).
 // V == 4 is only used when Co % 4 == 0 and V == 1 rows are single elements, so a lane with c0 < Co always
@@ -179,22 +156,13 @@ __global__ __launch_bounds__(256, WPE) void pwmlp_query_kernel(PwArgs a) {
     // atomics, and half the VGPRs of double register accumulators, which the gather loop's occupancy needs
     constexpr int kFlushTiles = 8 / QPG;  // <= 8 queries x K slots per running float sum
     constexpr int NF = NACC > 0 ? 5 : 1;
-    // (CL3D_TRAIN_PK = 1 only -- V == 4: the running sums live as two packed pairs per quantity, the TRAIN walk below is v_pk_fma_f32 / v_pk_add_f32
-    // on channel pairs: per-element IEEE, the same bits as the scalar chain, two channels per VALU slot)
-    constexpr bool PK = CL3D_TRAIN_PK && V == 4 && MODE == PW_TRAIN;
-    constexpr int VA = PK ? 2 : V;
-    using acc_t = typename std::conditional<PK, pw_f2, float>::type;
-    acc_t accf[NF][VA];
+    float accf[NF][V];
     float accr[3] = {0.f, 0.f, 0.f};
-    auto acc_get = [&](int p, int v) -> float {
-      if constexpr (PK) return accf[p][v >> 1][v & 1];
-      else return accf[p][v];
-    };
     auto acc_zero = [&]() {
 #pragma unroll
       for (int p = 0; p < NF; ++p)
 #pragma unroll
-        for (int v = 0; v < VA; ++v) accf[p][v] = acc_t(0.f);
+        for (int v = 0; v < V; ++v) accf[p][v] = 0.f;
     };
     acc_zero();
     int since_flush = 0;
@@ -217,7 +185,7 @@ __global__ __launch_bounds__(256, WPE) void pwmlp_query_kernel(PwArgs a) {
 #pragma unroll
       for (int p = 0; p < NF; ++p)
 #pragma unroll
-        for (int v = 0; v < V; ++v) f[p][v] = fold_groups(acc_get(p, v)) * (p >= 2 ? sgn[v] : 1.f);  // S_a held primed
+        for (int v = 0; v < V; ++v) f[p][v] = fold_groups(accf[p][v]) * (p >= 2 ? sgn[v] : 1.f);  // S_a held primed
       if (g == 0) {
         double *mine = red + (size_t)wave * LVN + cl * V * NACC;
 #pragma unroll
@@ -396,60 +364,6 @@ __global__ __launch_bounds__(256, WPE) void pwmlp_query_kernel(PwArgs a) {
           kb[v] = 0;
           hs[v] = sgn[v] * hc.v[v];
         }
-        if constexpr (PK) {
-        if (q_on) {
-          pw_f2 w0[2], w1[2], w2[2], sg[2], h2[2], s2[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            w0[h] = (pw_f2){ws[2 * h][0], ws[2 * h + 1][0]};
-            w1[h] = (pw_f2){ws[2 * h][1], ws[2 * h + 1][1]};
-            w2[h] = (pw_f2){ws[2 * h][2], ws[2 * h + 1][2]};
-            sg[h] = (pw_f2){sgn[2 * h], sgn[2 * h + 1]};
-            h2[h] = (pw_f2){hs[2 * h], hs[2 * h + 1]};
-            s2[h] = (pw_f2)(0.f);
-          }
-          walk([&](auto first, int k, const float4 &sr_, const Vec<V> &gr_) {
-            accr[0] += sr_.y;
-            accr[1] += sr_.z;
-            accr[2] += sr_.w;
-            const pw_f2 rx = pk_low(sr_.y), ry = pk_low(sr_.z), rz = pk_low(sr_.w);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              pw_f2 t = __builtin_elementwise_fma(w0[h], rx, h2[h]);
-              t = __builtin_elementwise_fma(w1[h], ry, t);
-              t = __builtin_elementwise_fma(w2[h], rz, t);
-              const pw_f2 y = __builtin_elementwise_fma((pw_f2){gr_.v[2 * h], gr_.v[2 * h + 1]}, sg[h], t);
-              s2[h] += y;
-              accf[1][h] = __builtin_elementwise_fma(y, y, accf[1][h]);
-              accf[2][h] = __builtin_elementwise_fma(y, rx, accf[2][h]);
-              accf[3][h] = __builtin_elementwise_fma(y, ry, accf[3][h]);
-              accf[4][h] = __builtin_elementwise_fma(y, rz, accf[4][h]);
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                if (decltype(first)::value || y[e] > best[2 * h + e]) {  // first extreme
-                  best[2 * h + e] = y[e];
-                  kb[2 * h + e] = k;
-                }
-              }
-            }
-          });
-          Vec<V> ys, sy;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            s2[h] *= sg[h];
-            accf[0][h] += s2[h];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              ys.v[2 * h + e] = sgn[2 * h + e] * best[2 * h + e];
-              sy.v[2 * h + e] = s2[h][e];
-            }
-          }
-          store_row<V>(a.ystar_t + orow, ys);
-          store_row<V>(a.sy_t + orow, sy);
-          *reinterpret_cast<unsigned *>(a.kstar_out + orow) =
-              (unsigned)kb[0] | ((unsigned)kb[1] << 8) | ((unsigned)kb[2] << 16) | ((unsigned)kb[3] << 24);
-        }
-        } else {
         if (q_on) {
         walk([&](auto first, int k, const float4 &sr_, const Vec<V> &gr_) {
           accr[0] += sr_.y;
@@ -489,7 +403,6 @@ __global__ __launch_bounds__(256, WPE) void pwmlp_query_kernel(PwArgs a) {
           a.kstar_out[orow] = (unsigned char)kb[0];
         }
         }  // q_on
-        }  // scalar walk
       } else {  // PW_FWD
         float best[V];
         int kb[V];

@@ -41,40 +41,12 @@ struct ReduceArgs {
   float inv_radius, pfloat;        // pfloat: 1/extent (pseudo grid)
 };
 
-// Packed fp32 (v_pk_fma_f32 / v_pk_mul_f32: two lanes' worth of fp32 per VALU slot).  PseudoGrid spends
-// P x V = 15 x 4 FMAs per (slot, lane); with the V = 4 channels of a lane held as two float pairs the same
-// arithmetic (each product and sum rounded exactly as before) issues half as many instructions.
-// CL3D_PG_PK = 0: the same pairs as two scalar FMAs each (scripts/micro/kernel_variants.py "pg_scalar").  Measured in round 6,
-// session 67, because the TRAIN walk and the ball query got FASTER as scalar code: here the packed form stays -- the operator
-// step 0.3896-0.3904 against 0.3927-0.3935 ms, config 3 4.63-4.66 against 4.69-4.70, every pair (15 influences x 4 channels per
-// slot: the instruction count matters).  Its packed operands carry `op_sel` but come out of VALU arithmetic, not
-// out of ds_read_b128, and the kernels stayed bit-exact beside bf16 contractions in every survey (up to 400 launches).
-#ifndef CL3D_PG_PK
-#define CL3D_PG_PK 1
-#endif
-#if CL3D_PG_PK
+// Two channels at a time: PseudoGrid spends P x V = 15 x 4 FMAs per (slot, lane), its V = 4 channels held as two float pairs.  The
+// library is built without packed FP32 (operands that read the high half of a register pair came back as 0.0 beside bf16 MFMA
+// kernels), so a pair is two scalar FMAs, with the same bits; packed, the operator step measured 0.8-1 % less.
 typedef float f2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f2 pk_fma(f2 a, f2 b, f2 c) { return __builtin_elementwise_fma(a, b, c); }
 __device__ __forceinline__ f2 pk_splat(float x) { return (f2)(x); }
-#else
-struct f2 {
-  float e[2];
-  __device__ __forceinline__ float &operator[](int i) { return e[i]; }
-  __device__ __forceinline__ const float &operator[](int i) const { return e[i]; }
-};
-__device__ __forceinline__ f2 pk_fma(f2 a, f2 b, f2 c) {
-  f2 r;
-  r.e[0] = __builtin_fmaf(a.e[0], b.e[0], c.e[0]);
-  r.e[1] = __builtin_fmaf(a.e[1], b.e[1], c.e[1]);
-  return r;
-}
-__device__ __forceinline__ f2 pk_splat(float x) {
-  f2 r;
-  r.e[0] = x;
-  r.e[1] = x;
-  return r;
-}
-#endif
 
 __device__ __forceinline__ float kp_influence(float rx, float ry, float rz, const float *kp, float inv_extent,
                                               int constant) {
@@ -93,7 +65,7 @@ __device__ __forceinline__ float kp_influence(float rx, float ry, float rz, cons
 // pairs, evaluated ONCE (by the forward pass's staging threads) and kept next to slotrec for the backward passes, and
 // the slot's per-channel weight is formed from them,
 //     out_c = sum_k (sum_{(p,h) in pairs(k)} h * kw[p,c]) * f_c[idx_k],
-// with kw rows read from an LDS table: ~8 packed FMAs per (slot, lane) instead of 32.  Unused pairs hold h = 0, p = 0
+// with kw rows read from an LDS table: ~8 FMA pairs per (slot, lane) instead of 32.  Unused pairs hold h = 0, p = 0
 // (they add 0 * kw[0]); a slot with more than kPgPairs influences (constant influence: all of them) is flagged
 // p[3] = -1 and takes the dense sum.  Same terms as the reference's sum over kernel points, added per slot instead of
 // per kernel point.
@@ -343,7 +315,7 @@ __global__ __launch_bounds__(256) void fused_reduce_fwd_kernel(ReduceArgs a) {
     if (c0 >= C) continue;
     Vec<V> out;
     if constexpr (OP == OP_PSEUDOGRID) {
-      constexpr int H = V == 4 ? 2 : 1;   // V == 4: two packed pairs per lane; V == 1: scalar
+      constexpr int H = V == 4 ? 2 : 1;   // V == 4: two pairs per lane; V == 1: scalar
       constexpr int KB = 4;               // row gathers in flight per lane
       f2 wf2[kMaxKP][H];
       float wf1[kMaxKP];
@@ -1074,7 +1046,7 @@ extern "C" int cl3d_fused_reduce_bwd(int op, const float *gout_t, const float *f
   // side the two take 167 + 105 us instead of 83 + 96 one behind the other -- both are bound by issue and L2 requests, not
   // by exposed latency -- and the step 0.389-0.390 against 0.384-0.386 ms; as in round 3, dropped)
   // (a sparse form of this pass -- per-lane-group accumulators in LDS, updated per pair -- was built and measured: 188 us
-  // against 95 us for the dense loop, whose 32 packed FMAs per slot cost no more than the ballots, address arithmetic
+  // against 95 us for the dense loop, whose 32 FMA pairs per slot cost no more than the ballots, address arithmetic
   // and dependent LDS read-modify-writes of ~1.2 updates; the gradient of the kernel weights stays dense)
   if (V == 4) hipLaunchKernelGGL((pg_dkw_kernel<4>), grid_dkw, dim3(256), lds_dkw, (hipStream_t)stream, a);
   else hipLaunchKernelGGL((pg_dkw_kernel<1>), grid_dkw, dim3(256), lds_dkw, (hipStream_t)stream, a);
