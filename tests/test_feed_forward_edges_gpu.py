@@ -260,3 +260,61 @@ def test_wide_projections_alone():
         g = gen(16)
         x, ws = ffn_inputs(g, B, C, N, H, TYPES[kind], down=False)
         ffn_check(x, ws, "gelu", TYPES[kind], features(g, B, H, N, TYPES[kind]), "point", tag=(kind, size))
+
+
+# --------------------------------------------------------------------------------------------------------------- as they are used
+@pytest.mark.parametrize("precision", ["f32", "bf16"])
+def test_a_whole_model_with_feed_forward_blocks_is_captured(precision):
+    """A classifier whose bottlenecks end in feed-forward blocks and whose head drops by the counter: a training step, captured with
+    its backward pass, gives in every replay what the eager step gives from the same numbers."""
+    import closerlook3d_amd
+    from closerlook3d_amd import compat
+    torch.manual_seed(0)
+    cfg = compat.default_config()
+    cfg.width, cfg.nsamples, cfg.npoints, cfg.radius, cfg.sampleDl = 24, [8] * 5, [128, 64, 32, 16], 0.2, 0.08
+    cfg.cl3d_feed_forward, cfg.cl3d_feed_forward_dropout, cfg.cl3d_counter_dropout, cfg.cl3d_precision = 2.0, 0.2, True, precision
+    model = compat.build_model(cfg, 'classification').cuda().train()
+    draws = [m._draws for m in model.modules() if hasattr(m, "_draws")]
+    assert len(draws) > 8
+    g = gen(17)
+    xyz = torch.rand((4, 512, 3), device="cuda", generator=g)
+    mask = torch.ones((4, 512), dtype=torch.int32, device="cuda")
+    features = torch.randn((4, 3, 512), device="cuda", generator=g)
+    probe = torch.randn((4, cfg.num_classes), device="cuda", generator=g)
+    params = list(model.parameters())
+    buffers = [b for b in model.buffers()]
+    start = [b.clone() for b in buffers]
+
+    def step():
+        for b, s in zip(buffers, start):
+            b.copy_(s)
+        out = model(xyz, mask, features)
+        return [out] + list(torch.autograd.grad(out, params, probe))
+
+    def at(n):
+        for d in draws:
+            d.rng.state[1] = n
+
+    side = closerlook3d_amd.step_stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+        wants = []
+        for n in (0, 500, 1000):
+            at(n)
+            wants.append([t.detach().clone() for t in step()])
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert not torch.equal(wants[0][0], wants[1][0])
+    graph = torch.cuda.CUDAGraph()
+    with closerlook3d_amd.whole_step_capture(), torch.cuda.graph(graph, stream=side):
+        static = step()
+    for turn in range(2):
+        for n, want in zip((0, 500, 1000), wants):
+            at(n)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            for k, (a, b) in enumerate(zip(static, want)):
+                assert bool(a.isfinite().all()) and torch.equal(a, b), (turn, n, k)
