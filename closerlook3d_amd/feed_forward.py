@@ -566,6 +566,9 @@ class _Draws:
         self.seed, self.rng, self.rngs = seed, None, {}  # rng: that of the last draw
 
     def take(self, x):
+        if torch._C._current_graph_task_id() != -1:
+            raise RuntimeError("dropout: a module draws its own numbers, which a backward pass that runs it again (activation "
+                               "checkpointing) would not have a second time: draw outside of what is run twice and call dropout() there")
         rng = self.rngs.get(x.device)
         if rng is None:
             if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
@@ -578,9 +581,9 @@ class _Draws:
 
 
 class CounterDropout(nn.Module):
-    """nn.Dropout by dropout(): no mask in memory.  Every call in training mode is a draw of its own, also one that activation
-    checkpointing makes a second time (draw outside of what is run twice and call dropout() there).  The generator's state is not part
-    of the state dict."""
+    """nn.Dropout by dropout(): no mask in memory.  Every call in training mode is a draw of its own; one that activation checkpointing
+    makes a second time is refused (draw outside of what is run twice and call dropout() there).  The generator's state is not part of
+    the state dict."""
 
     def __init__(self, p=0.5, seed=None):
         super().__init__()

@@ -318,3 +318,27 @@ def test_a_whole_model_with_feed_forward_blocks_is_captured(precision):
             torch.cuda.synchronize()
             for k, (a, b) in enumerate(zip(static, want)):
                 assert bool(a.isfinite().all()) and torch.equal(a, b), (turn, n, k)
+
+
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_a_draw_made_again_in_a_backward_pass_is_refused(reentrant):
+    """Activation checkpointing runs a module a second time, which would draw another mask than the forward pass had; numbers drawn
+    outside give the gradients of the mask that was."""
+    from torch.utils.checkpoint import checkpoint
+    g = gen(18)
+    x = features(g, 2, 24, 30, torch.float32).detach().requires_grad_(True)
+    block = ff.FeedForwardBlock(24, 48, dropout=0.5, seed=1).cuda()
+    drop = ff.CounterDropout(0.5, seed=2)
+    for module in (block, drop):
+        y = checkpoint(module, x, use_reentrant=reentrant)
+        with pytest.raises(RuntimeError, match="draws its own numbers"):
+            torch.autograd.backward(y, torch.ones_like(y))
+        assert torch.autograd.grad(module(x).sum(), [x])[0].shape == x.shape
+    rng = torch.tensor([4, 0], device="cuda")
+    x.grad = None
+    y = checkpoint(lambda t: ff.dropout(ff.point_norm(t), 0.5, rng), x, use_reentrant=reentrant)
+    y.sum().backward()
+    (want,) = torch.autograd.grad(ff.dropout(ff.point_norm(x), 0.5, rng).sum(), [x])
+    assert torch.equal(x.grad, want)
+    block.eval()
+    checkpoint(block, x, use_reentrant=reentrant).sum().backward()
