@@ -12,7 +12,8 @@ Tensors are features (B, C, N), as everywhere in this package, or rows (R, C): p
 features may lie channel-major (dense) or point-major (a transposed view of dense (B, N, C) rows); results lie as the first
 input does.  The norms read channel-major features as they lie (up to 1024 channels, a multiple of four); otherwise the kernels work
 on point-major rows and take and leave a transposed copy, so a chain of these operators is best kept point-major (to_point_major,
-once, at its beginning; FeedForwardBlock does).  Types: float32, bfloat16, float16.  Everything is formed in f32 and rounded once, to the type of the result.
+once, at its beginning; FeedForwardBlock does).  Types: float32, bfloat16, float16.  Everything is formed in f32 and rounded once, to
+the type of the result (a gated feed-forward of 16-bit tensors: once more in front of its second products).
 
 Points are independent of each other (only parameter gradients sum over them); padding points are computed like the others.  The
 results of a point depend on no other point, and every gradient is summed in a fixed order: bit-identical run to run.  There is no
@@ -38,6 +39,7 @@ _PRECISIONS = {'f32': 0, 'bf16': 1}
 _OP_GATED_FFN, _OP_POINT_NORM = 17, 18
 _MAX_NORM_CHANNELS, _WIDE_NORM_CHANNELS = 4096, 6144  # any number up to the first, multiples of 8 up to the second
 _MAX_SIZE = 2 ** 31 - 1  # the C entries take 32-bit sizes
+_MAX_GATES = 65535       # a grid's third axis
 
 
 def _p(t):
@@ -54,7 +56,7 @@ def _check_trace(who):
 
 
 def _check_sizes(t, who, name):
-    if max(t.shape) > _MAX_SIZE:
+    if t.numel() > _MAX_SIZE and max(t.shape) > _MAX_SIZE:  # (the first is the cheaper)
         raise ValueError(f"{who}: {name} has the shape {tuple(t.shape)}, no size is above {_MAX_SIZE}")
 
 
@@ -182,7 +184,8 @@ class _Reorder(Function):
 
 
 def to_point_major(features):
-    """(B, C, N) features as a view of dense (B, N, C) rows, by the engine's transpose where they do not lie so already."""
+    """(B, C, N) features as a view of dense (B, N, C) rows, by the engine's transpose where they do not lie so already (up to 65535
+    clouds of up to 4194240 points)."""
     _check_features(features, 'to_point_major', 'features')
     return features if _point_major(features) else _Reorder.apply(features, _POINT)
 
@@ -300,7 +303,9 @@ def gated_feed_forward(x, w_gate, w_up, w_down=None, activation='silu', precisio
     w_gate, w_up (H, C) and w_down (C, H) have x's type; w_down None: the product of the two projections itself, with H channels.
     activation 'silu', 'gelu' (by the error function) or 'relu'.  precision, of float32 tensors: 'f32' multiplies at f32 accuracy,
     'bf16' rounds what enters a product to bfloat16, as in the other operators of this package; 16-bit tensors enter as they are.
-    The hidden activations are rounded to the tensors' type (f32: kept) in front of the last product."""
+    16-bit tensors: what enters a second product -- the hidden activations h, in the backward pass the gradients of the two
+    projections -- is rounded to their type once more (f32 keeps its accuracy); in float16 it has that type's range too: above 65504 an
+    infinity, below 2^-25 nothing.  Channel-major features: up to 65535 clouds of up to 4194240 points."""
     who = 'gated_feed_forward'
     _check_features(x, who)
     C = x.shape[1]
@@ -433,9 +438,9 @@ def norm_gate_residual(x, y, weight=None, bias=None, gate=None, residual_scale=1
         out = residual_scale * x + gate * dropout(norm(y) weight + bias, p)          next = norm(out) next_weight + next_bias
 
     x: the residual stream, y: the block's result, same shape and type.  kind 'rms', 'layer' or 'none' (y is added as it is).  gate
-    (C,), or (B, C) for a gate of each cloud (for rows: of each row), or None.  p, rng: as in dropout(); element (b, c, n) is number
-    (b N + n) C + c of the draw.  next is formed from out before out is rounded.  Channels as in
-    point_norm().  Returns out, or (out, next) with next_kind."""
+    (C,), or (B, C) for a gate of each cloud (for rows: of each row; up to 65535 of them), or None.  p, rng: as in dropout(); element
+    (b, c, n) is number (b N + n) C + c of the draw.  next is formed from out before out is rounded.  Channels as in point_norm().
+    Returns out, or (out, next) with next_kind."""
     who = 'norm_gate_residual'
     _check_features(x, who)
     _check_features(y, who, 'y')
@@ -445,7 +450,10 @@ def norm_gate_residual(x, y, weight=None, bias=None, gate=None, residual_scale=1
     B, C, _ = _sizes(x)
     _check_param(weight, (C,), x, who, 'weight')
     _check_param(bias, (C,), x, who, 'bias')
-    _check_param(gate, (B, C) if isinstance(gate, torch.Tensor) and gate.dim() == 2 else (C,), x, who, 'gate')
+    per_cloud = isinstance(gate, torch.Tensor) and gate.dim() == 2
+    _check_param(gate, (B, C) if per_cloud else (C,), x, who, 'gate')
+    if per_cloud and B > _MAX_GATES:
+        raise ValueError(f"{who}: a gate of each cloud for up to {_MAX_GATES} clouds, got {B}")
     if next_kind is None:
         if next_weight is not None or next_bias is not None:
             raise ValueError(f"{who}: a weight or bias of a norm that is not asked for (next_kind)")

@@ -151,3 +151,10 @@ def test_capture_checks_beside_threads_that_make_graphs(monkeypatch):
         sys.setswitchinterval(interval)
     assert not failed
     del alive, ctx
+
+
+def test_a_gate_of_each_cloud_has_a_limit():
+    for shape in ((70000, 8), (70000, 8, 3)):
+        x = fake(1).expand(shape)
+        with pytest.raises(ValueError, match="up to 65535 clouds"):
+            ff.norm_gate_residual(x, x, gate=fake(1).expand(70000, 8))
