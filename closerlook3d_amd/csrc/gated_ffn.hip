@@ -8,6 +8,10 @@
 // writes dG, dU (h is kept from the forward pass where the caller has room for it, or formed again).  Against storing G and U that
 // is 8 R H bytes less traffic for 4 R C H operations more -- at 5.1 TB/s and 1.28 PFLOP/s (a large copy, a large product) it pays
 // below C = 500 -- and dG, dU come from f32 values of G, U, dh: one rounding in front of the last products instead of two.
+// That rounding, of 16-bit tensors: h in front of Y and dWd, dG and dU in front of dX, dWg and dWu are rounded to the tensors' type.
+// The matrix units take 16-bit operands, and a second plane of each (what f32 tensors have) would double six of the eleven products
+// of a training pass.  Beside the rounding of the results themselves it is a second one of the same size: 2.3e-3 of a result's norm in bf16
+// instead of 1.7e-3, 2.9e-4 instead of 2.1e-4 in f16, whose range is theirs too (above 65504 an infinity, below 2^-25 nothing).
 //
 // One kernel template.  D[j][i] = sum_k P(i, k) Q(j, k), i contiguous in the result; P is the first MFMA operand, so a lane of
 // v_mfma_f32_16x16x32 holds four consecutive i of one j.
@@ -26,8 +30,8 @@
 // f32 product.  Six passes at the bf16 rate outrun the f32 MFMA (1/16 of it).  A tile holds the three planes of 32 k, so each
 // fragment is read once for its two or three products.  A value that is not finite takes part in the product of the leading planes
 // only, so an infinity stays one (not_finite below).
-// Measured at 16 384 x 288 x 1152 in bf16: projections 37 us (590 TFLOP/s), their backward twin 68 (480), Y 19 (570), dX 35 (620),
-// the three weight gradients 61 (535); 16 384 x 144 x 576 in f32, counting f32 operations: 66 (82), 107 (76), 27 (100), 53 (103), 81 (100).
+// Measured at 16 384 x 288 x 1152 in bf16: projections 36 us (610 TFLOP/s), their backward twin 66 (490), Y 19 (575), dX 34 (640),
+// the three weight gradients 59 (555); 16 384 x 144 x 576 in f32, counting f32 operations: 61 (89), 101 (81), 25 (108), 49 (112), 74 (110).
 #include "ff_common.h"
 #include <type_traits>
 
@@ -758,8 +762,8 @@ __global__ __launch_bounds__(64 * kRowsWaves) void ffn_rows_kernel(RowsArgs a) {
 // passes from one product to the next without leaving the lane.  Only the weights travel: a chunk's rows of Wg and Wu and columns
 // of Wd, by way of LDS, the next chunk in flight; x is read and y written once, h is written only if the caller keeps it.
 // CF: 32-channel fragments of x, odd (a row of 64 CF bytes then starts at a quarter of its own of the 64 banks).
-// Measured against the two kernels it replaces (us, bf16): 65 536 x 144 x 576 60 (83), 131 072 x 72 x 288 41 (63), 32 768 x 144 x
-// 576 39 (42), 65 536 x 200 x 800 91 (121); 16 384 x 144 x 576 37 (25): below 32 768 points there are fewer than 256 workgroups of
+// Measured against the two kernels it replaces (us, a launch by itself, bf16): 65 536 x 144 x 576 60 (83; 51 where passes follow each
+// other), 131 072 x 72 x 288 41 (63), 32 768 x 144 x 576 39 (42), 65 536 x 200 x 800 91 (121); 16 384 x 144 x 576 37 (25): below 32 768 points there are fewer than 256 workgroups of
 // 128, one for each CU.  Bound: per chunk a wave waits for its weights, reads each fragment for one or two products and then is in
 // the activation; the two workgroups of a CU cover each other's waits in part.
 constexpr int kFusedMostC = 224, kFusedFewest = 32768;

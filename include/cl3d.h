@@ -539,7 +539,8 @@ int cl3d_reduce_train_backward(const cl3d_reduce_pass *p, cl3d_stream_t stream);
 
 /* ---- per-point feed-forward operators: csrc/gated_ffn.hip, point_norm.hip, dropout.hip ------------------------------------
  * Tensors of one call share an element type and a memory order: features are point-major rows [B,N,C] or, as everywhere else in
- * this header, channel-major [B,C,N].  Arithmetic is f32 inside, a 16-bit result is rounded once. */
+ * this header, channel-major [B,C,N] (up to 65535 clouds of up to 4194240 points where a call moves them to the other order).
+ * Arithmetic is f32 inside, a 16-bit result is rounded once; what enters a second product of cl3d_gated_ffn is rounded to 16 bits too. */
 #define CL3D_F32 0
 #define CL3D_BF16 1
 #define CL3D_F16 2
@@ -572,7 +573,7 @@ int cl3d_gated_ffn_bwd(const void *x, const void *w_gate, const void *w_up, cons
                        void *dx, void *dw_gate,
                        void *dw_up, void *dw_down, void *ws, size_t ws_bytes, cl3d_stream_t stream);
 
-/* [B,R,C] -> [B,C,R] of 16-bit elements (cl3d_transpose: f32) */
+/* [B,R,C] -> [B,C,R] of 16-bit elements (cl3d_transpose: f32); both: up to 65535 planes of up to 4194240 rows */
 int cl3d_transpose16(const void *src, int B, int R, int C, void *dst, cl3d_stream_t stream);
 
 /* Exit of a block and entry of the next, one pass over the points (channel-major tensors of more than 1024 channels, or not a
@@ -580,6 +581,7 @@ int cl3d_transpose16(const void *src, int B, int R, int C, void *dst, cl3d_strea
  *     n = norm(y) weight + bias;  out = residual_scale x + gate * drop(n);  next = next_norm(out) next_weight + next_bias
  * y NULL: there is no block to leave, next = next_norm(x) next_weight + next_bias.  next_kind CL3D_NORM_NONE: no entry.
  * Up to 4096 channels, or multiples of 8 up to 6144 in tensors that start on 16 bytes.
+ * A gate per cloud: up to 65535 clouds.
  * rms: v / sqrt(mean v^2 + eps); layer: (v - mean) / sqrt(var + eps), over the channels of a point.  weight, bias, gate,
  * next_weight, next_bias: [C] (gate [B,C] with gate_cloud), NULL: 1, 0, 1, 1, 0; of the tensors' type, or f32 with param_f32.
  * p, rng: as in cl3d_dropout, element (b, n, c) being number (b N + n) C + c.  stats [B,N,4], 16-byte aligned: what the
