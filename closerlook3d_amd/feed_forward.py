@@ -18,7 +18,7 @@ the type of the result (a gated feed-forward of 16-bit tensors: once more in fro
 Points are independent of each other (only parameter gradients sum over them); padding points are computed like the others.  The
 results of a point depend on no other point, and every gradient is summed in a fixed order: bit-identical run to run.  There is no
 CPU fallback.  The operators can be captured into HIP graphs, forward and backward.  A forward-mode tangent, a derivative of a
-gradient and a torch.jit.trace are refused.
+gradient and a trace (torch.jit.trace, make_fx) are refused.
 """
 import ctypes
 import threading
@@ -28,6 +28,7 @@ import torch
 import torch.nn as nn
 from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib
 
@@ -46,13 +47,13 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-_is_tracing = torch._C._is_tracing
+_is_tracing, _dispatch_modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
 
 
 def _check_trace(who):
     # (a trace holds the allocations of a call and nothing of what the launches put there)
-    if _is_tracing():
-        raise RuntimeError(f"{who}: cannot be traced by torch.jit.trace (capture a HIP graph instead)")
+    if _is_tracing() or (_dispatch_modes() and get_proxy_mode() is not None):
+        raise RuntimeError(f"{who}: cannot be traced by torch.jit.trace or make_fx (capture a HIP graph instead)")
 
 
 def _check_sizes(t, who, name):
@@ -61,7 +62,6 @@ def _check_sizes(t, who, name):
 
 
 def _check_features(x, who, name='x'):
-    _check_trace(who)
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{who}: {name} is a tensor, got {type(x).__name__}")
     if not x.is_cuda:
@@ -186,12 +186,14 @@ class _Reorder(Function):
 def to_point_major(features):
     """(B, C, N) features as a view of dense (B, N, C) rows, by the engine's transpose where they do not lie so already (up to 65535
     clouds of up to 4194240 points)."""
+    _check_trace('to_point_major')
     _check_features(features, 'to_point_major', 'features')
     return features if _point_major(features) else _Reorder.apply(features, _POINT)
 
 
 def to_channel_major(features):
     """(B, C, N) features as dense channel-major memory, what the other operators of this package read."""
+    _check_trace('to_channel_major')
     _check_features(features, 'to_channel_major', 'features')
     return features if features.is_contiguous() else _Reorder.apply(features, _CHANNEL)
 
@@ -307,6 +309,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down=None, activation='silu', precisio
     projections -- is rounded to their type once more (f32 keeps its accuracy); in float16 it has that type's range too: above 65504 an
     infinity, below 2^-25 nothing.  Channel-major features: up to 65535 clouds of up to 4194240 points."""
     who = 'gated_feed_forward'
+    _check_trace(who)
     _check_features(x, who)
     C = x.shape[1]
     _check_param(w_gate, (w_gate.shape[0] if isinstance(w_gate, torch.Tensor) and w_gate.dim() == 2 else 'H', C), x, who, 'w_gate',
@@ -422,6 +425,7 @@ def point_norm(x, weight=None, bias=None, kind='rms', eps=1e-6):
     kind 'rms': x / sqrt(mean x^2 + eps); 'layer': (x - mean) / sqrt(var + eps), the variance over all C.  weight, bias (C,), of x's
     type or float32; None: 1 and 0.  Up to 4096 channels, or a multiple of 8 up to 6144."""
     who = 'point_norm'
+    _check_trace(who)
     _check_features(x, who)
     _check_norm(x, kind, eps, who)
     C = x.shape[1]
@@ -442,6 +446,7 @@ def norm_gate_residual(x, y, weight=None, bias=None, gate=None, residual_scale=1
     (b, c, n) is number (b N + n) C + c of the draw.  next is formed from out before out is rounded.  Channels as in point_norm().
     Returns out, or (out, next) with next_kind."""
     who = 'norm_gate_residual'
+    _check_trace(who)
     _check_features(x, who)
     _check_features(y, who, 'y')
     if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device:

@@ -46,6 +46,7 @@ def test_a_tangent_is_refused_and_not_lost(name, grad):
                                   "to_point_major", "take"])
 def test_a_trace_is_refused(name):
     """A trace would hold a call's allocations and nothing of what the launches put there: its results would be memory as it was."""
+    from torch.fx.experimental.proxy_tensor import make_fx
     x, calls = _calls()
     rng = ff.CounterRng(5, "cuda")
     calls["to_point_major"] = lambda t: ff.to_point_major(t.contiguous())
@@ -53,6 +54,8 @@ def test_a_trace_is_refused(name):
     for grad in (False, True):
         with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="traced"):
             torch.jit.trace(calls[name], (x.clone().requires_grad_(grad),), check_trace=False)
+        with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="traced"):
+            make_fx(calls[name])(x.clone().requires_grad_(grad))
     assert rng.state.tolist() == [5, 0]
 
 
