@@ -21,6 +21,7 @@ CPU fallback.  The operators can be captured into HIP graphs, forward and backwa
 gradient and a trace (torch.jit.trace, make_fx) are refused.
 """
 import ctypes
+import functools
 import threading
 import weakref
 
@@ -198,6 +199,25 @@ def to_channel_major(features):
     return features if features.is_contiguous() else _Reorder.apply(features, _CHANNEL)
 
 
+def _once(backward):
+    """once_differentiable, also where the incoming gradient is a constant: that decorator takes the gradients it returns for constants
+    then, and a second derivative through the saved tensors would silently be zero.  (ctx.linear: it is.)"""
+
+    @functools.wraps(backward)
+    def once(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled() or (ctx.linear and not any(g is not None and g.requires_grad for g in grads)):
+            return out
+        given = [t for t in out if t is not None]
+        refuse = torch._C._functions.DelayedError(b"trying to differentiate twice a function that has one derivative", len(given))
+        marked = refuse(*[t.detach().requires_grad_(True) for t in given])
+        marked = iter(marked if isinstance(marked, tuple) else (marked,))
+        return tuple(None if t is None else next(marked) for t in out)
+
+    return once
+
+
 def _recorded(*tensors):
     """Whether a call goes through its autograd function: a gradient is wanted, or a forward-mode level is open (the function refuses
     a tangent; the launches alone would lose it).  Other calls do without the node, which costs as much host time as the rest of a
@@ -271,10 +291,11 @@ class _GatedFeedForward(Function):
         _track(ctx, x, w_gate, w_up, w_down)
         y, kept, ctx.args = _ffn_forward(x, w_gate, w_up, w_down, activation, precision, ctx.needs_input_grad[3])
         ctx.save_for_backward(*kept)
+        ctx.linear = False
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x, w_gate, w_up, w_down, hidden = ctx.saved_tensors
         _check_capture(ctx, x.device)
@@ -373,10 +394,11 @@ class _NormResidual(Function):
         out, nxt, kept, ctx.args = _norm_forward(x, y, weight, bias, gate, next_weight, next_bias, rng, opts, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(*kept)
+        ctx.linear = opts[0] == opts[1] == 0 and weight is None and gate is None  # (neither norm)
         return out, nxt
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout, dnext):
         x, y, weight, bias, gate, next_weight, next_bias, rng, stats = ctx.saved_tensors
         order, sizes, types = ctx.args

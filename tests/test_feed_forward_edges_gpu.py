@@ -345,3 +345,30 @@ def test_a_draw_made_again_in_a_backward_pass_is_refused(reentrant):
     assert torch.equal(x.grad, want)
     block.eval()
     checkpoint(block, x, use_reentrant=reentrant).sum().backward()
+
+
+@pytest.mark.parametrize("name", ["gated_feed_forward", "point_norm", "norm_gate_residual", "norm_gate_residual_next"])
+def test_a_derivative_of_a_gradient_is_refused_and_not_zero(name):
+    """A penalty on the gradients of a constant sum beside another term: without the refusal the penalty's part would silently be
+    nothing."""
+    x, calls = _calls()
+    scale = torch.full((24,), 2.0, device="cuda", requires_grad=True)
+    if name == "norm_gate_residual":
+        calls[name] = lambda t: ff.norm_gate_residual(t, t, gate=scale, kind='none')  # (its gradient is the gate's, not x's)
+    x = x.requires_grad_(True)
+    (g,) = torch.autograd.grad(calls[name](x).sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        ((g * g).sum() + (x * x).sum() + (scale * scale).sum()).backward()
+    (plain,) = torch.autograd.grad(calls[name](x).sum(), [x])
+    assert torch.equal(g, plain) and not plain.requires_grad
+
+
+def test_second_derivatives_that_are_zero_are_zero():
+    """Dropout, a memory order and a sum without parameters are linear: their gradient does not depend on x."""
+    x, calls = _calls()
+    x = x.contiguous().requires_grad_(True)
+    rng = torch.tensor([3, 0], device="cuda")
+    for call in (calls["dropout"], ff.to_point_major, lambda t: ff.norm_gate_residual(t, t, kind='none', p=0.3, rng=rng)):
+        (g,) = torch.autograd.grad(call(x).sum(), [x], create_graph=True)
+        (d,) = torch.autograd.grad((g * x).sum(), [x])
+        assert torch.equal(d, g)
