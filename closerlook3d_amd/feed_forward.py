@@ -22,7 +22,6 @@ gradient and a trace (torch.jit.trace, make_fx) are refused.
 """
 import ctypes
 import functools
-import threading
 import weakref
 
 import torch
@@ -229,8 +228,20 @@ def _recorded(*tensors):
 # graph of the leaf lives.  A backward pass captured meanwhile, on another stream, is handed over to that stream, which no capture
 # joins: ending it takes the process down.  Every eager graph of these operators is therefore known by its context while it lives
 # (autograd frees the context with the graph), and a captured backward pass of the same leaves says so instead.
-_LIVE = weakref.WeakSet()
-_LIVE_LOCK = threading.RLock()  # (a set that another thread adds to cannot be walked; contexts may go meanwhile)
+_LIVE = {}  # id -> weak reference.  Threads add and drop meanwhile: every use is one step of the interpreter (no walk in Python)
+
+
+def _forget(ref, live=_LIVE):  # (bound: it may be called when the module's names are gone)
+    if live.get(ref.key) is ref:
+        live.pop(ref.key, None)
+
+
+class _Ref(weakref.ref):
+    __slots__ = ("key",)
+
+    def __init__(self, ctx, callback):
+        super().__init__(ctx, callback)
+        self.key = id(ctx)
 
 
 def _track(ctx, *inputs):
@@ -238,8 +249,7 @@ def _track(ctx, *inputs):
     ctx.leaves = [weakref.ref(t) for t in inputs if t is not None and t.requires_grad and t.is_leaf]
     if ctx.leaves and not torch.cuda.is_current_stream_capturing():
         ctx.made_on = _raw_stream(inputs[0].device.index)
-        with _LIVE_LOCK:
-            _LIVE.add(ctx)
+        _LIVE[id(ctx)] = _Ref(ctx, _forget)
 
 
 def _check_capture(ctx, device):
@@ -248,10 +258,10 @@ def _check_capture(ctx, device):
         return
     mine = {id(t) for t in (r() for r in ctx.leaves) if t is not None}
     stream = _raw_stream(device.index)
-    with _LIVE_LOCK:
-        others = list(_LIVE)
-    for other in others:
-        if other is not ctx and other.made_on != stream and any(id(r()) in mine for r in other.leaves if r() is not None):
+    for other in [r() for r in list(_LIVE.values())]:
+        if other is None or other is ctx or other.made_on == stream:
+            continue
+        if any(id(t) in mine for t in (r() for r in other.leaves) if t is not None):
             raise RuntimeError("a backward pass is being captured while an eager graph of the same leaves, made on another stream, is "
                                "alive: delete its outputs first, or warm up and capture on one stream (closerlook3d_amd.step_stream())")
 

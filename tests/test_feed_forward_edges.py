@@ -158,3 +158,47 @@ def test_a_gate_of_each_cloud_has_a_limit():
         x = fake(1).expand(shape)
         with pytest.raises(ValueError, match="up to 65535 clouds"):
             ff.norm_gate_residual(x, x, gate=fake(1).expand(70000, 8))
+
+
+def test_capture_checks_beside_threads_that_drop_graphs(monkeypatch):
+    """The same while other threads free graphs one by one: a context that goes in another thread changes nothing under the walk."""
+    import sys
+    import threading
+    monkeypatch.setattr(ff, "_raw_stream", lambda index: 1)
+    leaf = torch.nn.Parameter(torch.zeros(3))
+
+    class Context:
+        pass
+
+    capturing = threading.local()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: getattr(capturing, "yes", False))
+    stop, failed = threading.Event(), []
+    alive = [Context() for _ in range(50)]
+    for ctx in alive:
+        ff._track(ctx, leaf)
+
+    def drop():
+        try:
+            while not stop.is_set():
+                ff._track(Context(), leaf)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    threads = [threading.Thread(target=drop) for _ in range(3)]
+    try:
+        for t in threads:
+            t.start()
+        mine = Context()
+        mine.leaves, mine.made_on = [], 1
+        capturing.yes = True
+        for _ in range(4000):
+            ff._check_capture(mine, torch.device("cuda", 0))
+        assert not failed
+    finally:
+        stop.set()
+        for t in threads:
+            t.join()
+        sys.setswitchinterval(interval)
+    del alive, ctx
